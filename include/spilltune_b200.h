@@ -280,6 +280,40 @@ size_t fl_ce_workspace_bytes(int64_t T, int64_t V);
 int fl_ce_chunk(const uint16_t* h, int64_t T, int64_t H, const uint16_t* head, int64_t V, const int64_t* targets,
                 float inv_norm, float* loss_sum, uint16_t* dh, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Rotary position embedding of queries and keys, with an optional RMS norm of
+ * every head in the same pass (the reference's q/k norms and rotation,
+ * ram_vram_finetune/adapters/dense.py:131-141).  Inputs are bf16 rows of D
+ * columns at x + token * token_stride + head * head_stride (elements; the
+ * columns of a row are adjacent), outputs contiguous bf16 [T, heads, D].
+ *   positions   int32 or int64 [T] (position_bytes 4 or 8);
+ *   inv_freq    fp32 [rot / 2]: pair p of token t turns by position * inv_freq[p],
+ *               cosine and sine multiplied by `factor`; columns >= rot pass;
+ *   interleaved 0: columns (p, p + rot/2) pair up; 1: columns (2p, 2p + 1);
+ *   weight_bytes 0: no norm; 2 / 4: bf16 / fp32 norm weights [D], x is first
+ *               x * rsqrt(mean(x^2) + eps) * weight.
+ * Hk = 0: queries only.  2 <= D <= 256.  Rows that are 16-byte aligned with D
+ * and rot multiples of 16 take the vectorised form.
+ *
+ * fl_rotary_bwd: gradients of the inputs (contiguous) from those of the
+ * outputs (strided); q and k, the forward's inputs, are read with a norm only.
+ * dq_weight / dk_weight: fp32 [D] or NULL; when given, workspace holds
+ * fl_rotary_bwd_workspace_bytes(D) bytes (4-byte aligned) and the sums run in a fixed order.
+ */
+int fl_rotary_fwd(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, int Hq, const uint16_t* k,
+                  int64_t k_token_stride, int64_t k_head_stride, int Hk, int64_t T, int D, const void* positions,
+                  int position_bytes, const float* inv_freq, int rot, int interleaved, float factor,
+                  const void* q_weight, const void* k_weight, int weight_bytes, float eps, uint16_t* q_out,
+                  uint16_t* k_out, void* stream);
+size_t fl_rotary_bwd_workspace_bytes(int D);
+int fl_rotary_bwd(const uint16_t* dq, int64_t dq_token_stride, int64_t dq_head_stride, const uint16_t* dk,
+                  int64_t dk_token_stride, int64_t dk_head_stride, const uint16_t* q, int64_t q_token_stride,
+                  int64_t q_head_stride, int Hq, const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,
+                  int Hk, int64_t T, int D, const void* positions, int position_bytes, const float* inv_freq, int rot,
+                  int interleaved, float factor, const void* q_weight, const void* k_weight, int weight_bytes,
+                  float eps, uint16_t* dq_out, uint16_t* dk_out, float* dq_weight, float* dk_weight, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

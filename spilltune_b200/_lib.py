@@ -48,6 +48,11 @@ SIGNATURES = {
                          _P], _INT),
     "fl_ce_workspace_bytes": ([_I64, _I64], _SZ),
     "fl_ce_chunk": ([_P, _I64, _I64, _P, _I64, _P, _F, _P, _P, _P, _SZ, _P], _INT),
+    "fl_rotary_fwd": ([_P, _I64, _I64, _INT, _P, _I64, _I64, _INT, _I64, _INT, _P, _INT, _P, _INT, _INT, _F, _P, _P,
+                       _INT, _F, _P, _P, _P], _INT),
+    "fl_rotary_bwd_workspace_bytes": ([_INT], _SZ),
+    "fl_rotary_bwd": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _INT, _P, _I64, _I64, _INT, _I64, _INT, _P,
+                       _INT, _P, _INT, _INT, _F, _P, _P, _INT, _F, _P, _P, _P, _P, _P, _SZ, _P], _INT),
     "fl_grouped_workspace_bytes": ([_I64, _INT, _I64, _I64, _INT], _SZ),
     "fl_grouped_fwd": ([_P, _P, _I64, _I64, _INT, _P, _P, _P, _I64, _P, _P, _INT, _F, _P, _P, _SZ, _P], _INT),
     "fl_grouped_bwd": ([_P, _P, _P, _I64, _I64, _I64, _INT, _P, _P, _P, _P, _P, _INT, _F, _P, _P, _P, _INT, _P,

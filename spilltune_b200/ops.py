@@ -11,6 +11,8 @@ unchanged and accumulates into ``grad_A``/``grad_B`` exactly as before.
 All work runs on the current CUDA stream.  CPU tensors are rejected: the path
 has no CPU fallback.
 """
+import contextlib
+
 import torch
 
 from . import _lib
@@ -31,6 +33,19 @@ def _need_cuda(*tensors):
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(t):
+    """Context in which t's device is the current one (none is entered when it is already)."""
+    return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def stream_of(t):
+    """The current stream of t's device."""
+    return torch.cuda.current_stream(t.device).cuda_stream
 
 
 def dequant(weight: PackedWeight, out=None):

@@ -1,0 +1,264 @@
+"""Rotary position embedding of queries and keys, with an optional norm of every head.
+
+The reference's dense block norms each head (Qwen3) and rotates queries and
+keys in about a dozen elementwise passes (ram_vram_finetune/adapters/dense.py:
+131-141, rms at :115-117).  Here both are one pass over the data, forward and
+backward (csrc/fl_rotary.cu): the inputs may be strided views of a fused
+projection's output, angles are formed from the positions in the kernel, and
+each result is rounded once.
+
+* ``rotate(q, k, positions, inv_freq)`` and ``norm_rotate(...)``: autograd.
+* ``fwd`` / ``bwd``: the two passes directly, as ``ops.fwd`` / ``ops.bwd``.
+* ``frequencies(...)``: inverse frequencies under the usual long-context
+  scalings, and the factor that cosines and sines are multiplied by.
+
+CUDA only; no CPU fallback.
+"""
+import math
+
+import torch
+
+from . import _lib
+from .ops import _need_cuda, _ptr, on_device, stream_of
+
+_INTS = {torch.int32: 4, torch.int64: 8}
+_WEIGHTS = {torch.bfloat16: 2, torch.float32: 4}
+MAX_HEAD_DIM = 256
+
+
+def frequencies(dim, theta=10000.0, scaling=None):
+    """(inv_freq fp32 [dim / 2] on the CPU, factor) for `dim` rotated columns.
+
+    `scaling`: None, or a dict with "type" and its parameters:
+      * "linear": factor.  Positions are compressed by it.
+      * "llama3": factor, low_freq_factor, high_freq_factor, original_length.
+        Wavelengths under original_length / high_freq_factor are kept, those
+        over original_length / low_freq_factor divided by `factor`, and blended
+        linearly in original_length / wavelength between.
+      * "yarn": factor, original_length, beta_fast = 32, beta_slow = 1,
+        attention_factor = 0.1 ln(factor) + 1.  Frequencies that turn over
+        beta_fast times within original_length are kept, those under beta_slow
+        times divided by `factor`, with a linear ramp over the index between.
+    """
+    if not isinstance(dim, int) or dim < 2 or dim % 2:
+        raise ValueError("rotated columns must be a positive even number")
+    if not theta > 0:
+        raise ValueError("theta must be positive")
+    index = torch.arange(0, dim, 2, dtype=torch.float64) / dim
+    inv = 1.0 / float(theta) ** index
+    if scaling is None:
+        return inv.float(), 1.0
+    opt = dict(scaling)
+    kind = opt.pop("type", None)
+    need = {"linear": ("factor",), "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_length"),
+            "yarn": ("factor", "original_length")}
+    more = {"yarn": ("beta_fast", "beta_slow", "attention_factor")}
+    if kind not in need:
+        raise ValueError(f"unsupported_capability: rotary scaling {kind!r} (linear, llama3 and yarn are)")
+    unknown = set(opt) - set(need[kind]) - set(more.get(kind, ()))
+    missing = [n for n in need[kind] if n not in opt]
+    if unknown or missing:
+        raise ValueError(f"rotary scaling {kind!r}: missing {missing}, unknown {sorted(unknown)}")
+    by = float(opt["factor"])
+    if not by >= 1.0:
+        raise ValueError("rotary scaling factor must be >= 1")
+    if kind == "linear":
+        return (inv / by).float(), 1.0
+    length = float(opt["original_length"])
+    if not length > 0:
+        raise ValueError("rotary scaling original_length must be positive")
+    if kind == "llama3":
+        low, high = float(opt["low_freq_factor"]), float(opt["high_freq_factor"])
+        if not high > low > 0:
+            raise ValueError("rotary scaling needs high_freq_factor > low_freq_factor > 0")
+        turns = length * inv / (2 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
+        return (keep * inv + (1 - keep) * inv / by).float(), 1.0
+    fast, slow = float(opt.get("beta_fast", 32.0)), float(opt.get("beta_slow", 1.0))
+    if not fast > slow > 0:
+        raise ValueError("rotary scaling needs beta_fast > beta_slow > 0")
+
+    def column(turns):  # the (real) pair index whose wavelength turns this often in original_length
+        return dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(float(theta)))
+
+    first, last = max(math.floor(column(fast)), 0), min(math.ceil(column(slow)), dim - 1)
+    ramp = ((torch.arange(dim // 2, dtype=torch.float64) - first) / max(last - first, 1e-3)).clamp(0.0, 1.0)
+    factor = opt.get("attention_factor")
+    if factor is None:
+        factor = 0.1 * math.log(by) + 1.0
+    return (inv * (1 - ramp) + inv / by * ramp).float(), float(factor)
+
+
+def _rows(x, what):
+    """x [..., heads, D] as (tensor, tokens, token stride, head stride): no copy
+    where the leading dimensions have one stride between tokens."""
+    if x.dim() < 3:
+        raise ValueError(f"{what} must be [..., heads, head size]")
+    if x.dtype != torch.bfloat16:
+        raise ValueError(f"{what} must be bf16")
+    tokens = 1
+    for n in x.shape[:-2]:
+        tokens *= n
+    if x.dim() == 3 and (x.stride(-1) == 1 or x.shape[-1] == 1):
+        return x, tokens, x.stride(0), x.stride(1)
+    step, reach, even = None, 1, x.stride(-1) == 1
+    for n, s in zip(reversed(x.shape[:-2]), reversed(x.stride()[:-2])):
+        if n == 1:
+            continue
+        if step is None:
+            step = s
+        even = even and s == step * reach
+        reach *= n
+    if not even:
+        x = x.contiguous()
+        return x, tokens, x.shape[-2] * x.shape[-1], x.shape[-1]
+    return x, tokens, step or 0, x.stride(-2)
+
+
+def _setup(q, k, positions, inv_freq, q_weight, k_weight, eps):
+    """Argument checks shared by both passes; returns the call's common values."""
+    _need_cuda(q, k, positions, inv_freq, q_weight, k_weight)
+    dev = q.device
+    for t in (k, positions, inv_freq, q_weight, k_weight):
+        if t is not None and t.device != dev:
+            raise ValueError("rotary arguments must be on one device")
+    if q.dim() < 3:
+        raise ValueError("q must be [..., heads, head size]")
+    D, lead = q.shape[-1], q.shape[:-2]
+    if k is not None and (k.dim() != q.dim() or k.shape[-1] != D or k.shape[:-2] != lead):
+        raise ValueError("q and k must agree in their leading dimensions and head size")
+    if positions.dtype not in _INTS:
+        raise ValueError("positions must be int32 or int64")
+    if positions.shape != lead:
+        try:
+            positions = positions.expand(lead)
+        except RuntimeError:
+            raise ValueError(f"positions {tuple(positions.shape)} do not fit the tokens {tuple(lead)}") from None
+    positions = positions.contiguous()
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
+        raise ValueError("inv_freq must be fp32 [rotated columns / 2]")
+    inv_freq = inv_freq.contiguous()
+    rot = 2 * inv_freq.shape[0]
+    if rot < 2 or rot > D:
+        raise ValueError(f"{rot} rotated columns do not fit a head of {D}")
+    if D > MAX_HEAD_DIM:
+        raise ValueError(f"unsupported_capability: head size {D} > {MAX_HEAD_DIM}")
+    wbytes = 0
+    if (q_weight is None) != (k_weight is None) and k is not None:
+        raise ValueError("give both norm weights or neither")
+    if q_weight is not None:
+        for w in (q_weight, k_weight):
+            if w is not None and (w.shape != (D,) or w.dtype not in _WEIGHTS or w.dtype != q_weight.dtype):
+                raise ValueError("norm weights must be bf16 or fp32 [head size], of one type")
+        if eps is None or not eps >= 0:
+            raise ValueError("a norm needs eps >= 0")
+        wbytes = _WEIGHTS[q_weight.dtype]
+        q_weight = q_weight.contiguous()
+        k_weight = None if k_weight is None else k_weight.contiguous()
+    return positions, inv_freq, rot, q_weight, k_weight, wbytes, float(eps or 0.0)
+
+
+def _out(shape, like):
+    return torch.empty(shape, dtype=torch.bfloat16, device=like.device)
+
+
+def fwd(q, k, positions, inv_freq, *, interleaved=False, factor=1.0, q_weight=None, k_weight=None, eps=None):
+    """(q', k'): q [..., Hq, D] and k [..., Hk, D] (or None), bf16, with the first
+    2 * len(inv_freq) columns of every head rotated by positions * inv_freq,
+    after an RMS norm of each head when the weights are given.  Contiguous.
+
+    positions: int32 or int64, broadcastable to the leading dimensions.
+    interleaved: columns (2p, 2p + 1) pair up, not (p, p + rot / 2).
+    factor: multiplies cosine and sine (see ``frequencies``)."""
+    positions, inv_freq, rot, q_weight, k_weight, wbytes, eps = _setup(q, k, positions, inv_freq, q_weight, k_weight,
+                                                                       eps)
+    qr, T, qt, qh = _rows(q, "q")
+    kr, _, kt, kh = _rows(k, "k") if k is not None else (None, T, 0, 0)
+    yq = _out(q.shape, q)
+    yk = _out(k.shape, k) if k is not None else None
+    Hk = 0 if k is None else k.shape[-2]
+    if q.shape[-2] + Hk == 0 or T == 0:
+        return yq, yk
+    with on_device(q):
+        _lib.call("fl_rotary_fwd", _ptr(qr), qt, qh, q.shape[-2], _ptr(kr), kt, kh, Hk, T, q.shape[-1],
+                  _ptr(positions), _INTS[positions.dtype], _ptr(inv_freq), rot, int(bool(interleaved)), float(factor),
+                  _ptr(q_weight), _ptr(k_weight), wbytes, eps, _ptr(yq), _ptr(yk), stream_of(q))
+    return yq, yk
+
+
+def bwd(dq, dk, q, k, positions, inv_freq, *, interleaved=False, factor=1.0, q_weight=None, k_weight=None, eps=None,
+        weight_grads=False):
+    """Gradients of fwd(): (dq, dk, dq_weight, dk_weight) from those of its results.
+    q and k are the forward's inputs, read only with a norm; dq and dk may be
+    any views.  Weight gradients (fp32 [D], summed in a fixed order) are formed
+    with weight_grads=True, else None."""
+    if k is None and dk is not None or k is not None and dk is None:
+        raise ValueError("dk goes with k")
+    positions, inv_freq, rot, q_weight, k_weight, wbytes, eps = _setup(q, k, positions, inv_freq, q_weight, k_weight,
+                                                                       eps)
+    _need_cuda(dq, dk)
+    if dq.shape != q.shape or k is not None and dk.shape != k.shape:
+        raise ValueError("dq and dk must have the shapes of q and k")
+    if dq.device != q.device or dk is not None and dk.device != q.device:
+        raise ValueError("rotary arguments must be on one device")
+    if weight_grads and not wbytes:
+        raise ValueError("weight gradients need the norm weights")
+    dqr, T, dqt, dqh = _rows(dq, "dq")
+    dkr, _, dkt, dkh = _rows(dk, "dk") if k is not None else (None, T, 0, 0)
+    qr, qt, qh, kr, kt, kh = None, 0, 0, None, 0, 0
+    if wbytes:
+        qr, _, qt, qh = _rows(q, "q")
+        if k is not None:
+            kr, _, kt, kh = _rows(k, "k")
+    D, Hk = q.shape[-1], 0 if k is None else k.shape[-2]
+    gq = _out(q.shape, q)
+    gk = _out(k.shape, k) if k is not None else None
+    gqw = gkw = ws = None
+    nbytes = 0
+    if weight_grads:
+        gqw = torch.zeros(D, dtype=torch.float32, device=q.device) if T == 0 else \
+            torch.empty(D, dtype=torch.float32, device=q.device)
+        gkw = None if k is None else torch.empty_like(gqw) if T else torch.zeros_like(gqw)
+        nbytes = _lib.load().fl_rotary_bwd_workspace_bytes(D)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    if T:
+        with on_device(q):
+            _lib.call("fl_rotary_bwd", _ptr(dqr), dqt, dqh, _ptr(dkr), dkt, dkh, _ptr(qr), qt, qh, q.shape[-2],
+                      _ptr(kr), kt, kh, Hk, T, D, _ptr(positions), _INTS[positions.dtype], _ptr(inv_freq), rot,
+                      int(bool(interleaved)), float(factor), _ptr(q_weight), _ptr(k_weight), wbytes, eps, _ptr(gq),
+                      _ptr(gk), _ptr(gqw), _ptr(gkw), _ptr(ws), nbytes, stream_of(q))
+    return gq, gk, gqw, gkw
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, inv_freq, interleaved, factor, eps):
+        ctx.opt = dict(interleaved=interleaved, factor=factor, eps=eps)
+        ctx.save_for_backward(q, k, q_weight, k_weight, positions, inv_freq)
+        ctx.set_materialize_grads(True)
+        yq, yk = fwd(q.detach(), None if k is None else k.detach(), positions, inv_freq, q_weight=q_weight,
+                     k_weight=k_weight, **ctx.opt)
+        return (yq,) if yk is None else (yq, yk)
+
+    @staticmethod
+    def backward(ctx, dq, dk=None):
+        q, k, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
+        weights = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
+        gq, gk, gqw, gkw = bwd(dq, dk, q, k, positions, inv_freq, q_weight=q_weight, k_weight=k_weight,
+                               weight_grads=weights, **ctx.opt)
+        return (gq, gk, gqw.to(q_weight.dtype) if ctx.needs_input_grad[2] else None,
+                gkw.to(k_weight.dtype) if ctx.needs_input_grad[3] else None, None, None, None, None, None)
+
+
+def rotate(q, k, positions, inv_freq, *, interleaved=False, factor=1.0):
+    """fwd() without a norm, differentiable in q and k.  k None: returns (q', None)."""
+    out = _Rotary.apply(q, k, None, None, positions, inv_freq, bool(interleaved), float(factor), None)
+    return out[0], out[1] if k is not None else None
+
+
+def norm_rotate(q, k, q_weight, k_weight, positions, inv_freq, *, eps, interleaved=False, factor=1.0):
+    """fwd() with the norm of every head, differentiable in q, k and the norm weights."""
+    if q_weight is None:
+        raise ValueError("norm_rotate needs the norm weights (rotate has none)")
+    out = _Rotary.apply(q, k, q_weight, k_weight, positions, inv_freq, bool(interleaved), float(factor), eps)
+    return out[0], out[1] if k is not None else None
