@@ -314,6 +314,38 @@ int fl_rotary_bwd(const uint16_t* dq, int64_t dq_token_stride, int64_t dq_head_s
                   float eps, uint16_t* dq_out, uint16_t* dk_out, float* dq_weight, float* dk_weight, void* workspace,
                   size_t workspace_bytes, void* stream);
 
+/*
+ * Attention over row ranges (the reference's eager attention with its additive
+ * mask, ram_vram_finetune/adapters/dense.py:142-148).  Query i of sequence b
+ * sees the keys begin[b, i] <= j < end[b, i] (clamped to [0, Sk); none where
+ * begin >= end: its output is 0 and its log sum -inf):
+ *   x_ij = scale q_i . k_j;  softcap > 0: x = softcap tanh(x / softcap);
+ *   slopes: x -= slopes[h] |i + Sk - Sq - j|;  out_i = sum_j softmax(x_i)_j v_j.
+ * q [B, Sq, Hq, D], k and v [B, Sk, Hkv, D] bf16 with element strides
+ * (a HOST array: batch, token, head of q, k, v[, dout]; columns adjacent); head
+ * h reads key/value head h / (Hq / Hkv).  D a multiple of 8, 8 <= D <= 128;
+ * scale > 0; pointers 16-byte aligned, strides positive multiples of 8.
+ *   begin, end  int32 [B, Sq];  slopes fp32 [Hq] or NULL;
+ *   out         bf16 [B, Sq, Hq, D];  lse fp32 [B, Sq, Hq], the natural log of
+ *               the softmax's denominator.
+ * Values in keys no row sees do not reach the result where whole 128-key tiles
+ * are unseen; inside a tile that some row sees they must be finite (a product
+ * with the probability 0), as in the eager form.
+ * fl_attn_bwd: dq, dk, dv (contiguous bf16) from dout; out and lse as the
+ * forward left them.  No atomics: equal inputs give equal bits.
+ * Workspaces: the *_workspace_bytes sizes, 16-byte aligned.
+ */
+size_t fl_attn_fwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D);
+int fl_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* strides, int64_t B, int64_t Sq,
+                int64_t Sk, int Hq, int Hkv, int D, const int32_t* begin, const int32_t* end, float scale,
+                float softcap, const float* slopes, uint16_t* out, float* lse, void* workspace,
+                size_t workspace_bytes, void* stream);
+size_t fl_attn_bwd_workspace_bytes(int64_t B, int64_t Sq, int Hq, int Hkv);
+int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* strides,
+                const uint16_t* out, const float* lse, int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D,
+                const int32_t* begin, const int32_t* end, float scale, float softcap, const float* slopes,
+                uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

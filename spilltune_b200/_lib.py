@@ -53,6 +53,12 @@ SIGNATURES = {
     "fl_rotary_bwd_workspace_bytes": ([_INT], _SZ),
     "fl_rotary_bwd": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _INT, _P, _I64, _I64, _INT, _I64, _INT, _P,
                        _INT, _P, _INT, _INT, _F, _P, _P, _INT, _F, _P, _P, _P, _P, _P, _SZ, _P], _INT),
+    "fl_attn_fwd_workspace_bytes": ([_I64, _I64, _I64, _INT, _INT, _INT], _SZ),
+    "fl_attn_fwd": ([_P, _P, _P, _P, _I64, _I64, _I64, _INT, _INT, _INT, _P, _P, _F, _F, _P, _P, _P, _P, _SZ, _P],
+                    _INT),
+    "fl_attn_bwd_workspace_bytes": ([_I64, _I64, _INT, _INT], _SZ),
+    "fl_attn_bwd": ([_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _INT, _INT, _INT, _P, _P, _F, _F, _P, _P, _P, _P,
+                     _P, _SZ, _P], _INT),
     "fl_grouped_workspace_bytes": ([_I64, _INT, _I64, _I64, _INT], _SZ),
     "fl_grouped_fwd": ([_P, _P, _I64, _I64, _INT, _P, _P, _P, _I64, _P, _P, _INT, _F, _P, _P, _SZ, _P], _INT),
     "fl_grouped_bwd": ([_P, _P, _P, _I64, _I64, _I64, _INT, _P, _P, _P, _P, _P, _INT, _F, _P, _P, _P, _INT, _P,

@@ -1,0 +1,196 @@
+"""Attention of a decoder block over row ranges.
+
+The reference's dense block repeats the key/value heads, forms every score in
+memory and adds a [S, S] mask (ram_vram_finetune/adapters/dense.py:142-148).
+Here query i sees the keys begin[i] <= j < end[i], one pass over the keys with
+a running softmax (csrc/fl_attn.cu) and a backward that forms the scores again
+(csrc/fl_attn_bwd.cu).  ``row_ranges`` builds the ranges of causal, document,
+prefix, sliding-window and padding masks; scores may be capped by a tanh
+(``softcap``) and lowered with the distance (``slopes``).
+
+* ``attend(q, k, v, begin, end, ...)``: autograd in q, k and v.
+* ``fwd`` / ``bwd``: the two passes directly, as ``ops.fwd`` / ``ops.bwd``.
+
+CUDA only; no CPU fallback.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .ops import _need_cuda, _ptr, on_device, stream_of
+
+MAX_HEAD_DIM = 128
+
+
+def row_ranges(batch, length, *, documents=None, prefix=None, window=None, lengths=None, causal=True, device=None):
+    """(begin, end) int32 [batch, length]: the keys that each token of a
+    [batch, length] block sees.
+
+    causal: tokens up to itself; else all of them.
+    documents: int [batch, length] ids; a token sees its own document only (the
+        tokens with its id around it, ids in runs).
+    prefix: int [batch]; the first prefix[b] tokens are seen by every token of
+        their document.
+    window: int >= 1; only the last `window` tokens up to itself (causal masks).
+    lengths: int [batch]; tokens from lengths[b] on are padding: they see
+        nothing and nothing sees them."""
+    if length < 0 or batch < 0:
+        raise ValueError("batch and length must not be negative")
+    if window is not None and (not causal or window < 1):
+        raise ValueError("a window needs a causal mask and a size >= 1")
+    for t in (documents, prefix, lengths):
+        if t is not None and device is None:
+            device = t.device
+    at = torch.arange(length, device=device, dtype=torch.int64).expand(batch, length)
+    begin = torch.zeros_like(at)
+    stop = torch.full_like(at, length)
+    if documents is not None:
+        if documents.shape != (batch, length):
+            raise ValueError("documents must be [batch, length]")
+        change = documents[:, 1:] != documents[:, :-1]
+        edge = torch.cat((torch.ones_like(documents[:, :1], dtype=torch.bool), change), 1) if length else change
+        begin = torch.where(edge, at, torch.zeros_like(at)).cummax(1).values if length else begin
+        tail = torch.cat((change, torch.ones_like(documents[:, :1], dtype=torch.bool)), 1) if length else change
+        stop = torch.where(tail, at + 1, torch.full_like(at, length)).flip(1).cummin(1).values.flip(1) \
+            if length else stop
+    end = torch.minimum(at + 1, stop) if causal else stop
+    if prefix is not None:
+        if prefix.shape != (batch,):
+            raise ValueError("prefix must be [batch]")
+        end = torch.maximum(end, torch.minimum(prefix.to(torch.int64)[:, None], stop))
+    if window is not None:
+        begin = torch.maximum(begin, at + 1 - window)
+    if lengths is not None:
+        if lengths.shape != (batch,):
+            raise ValueError("lengths must be [batch]")
+        live = lengths.to(torch.int64)[:, None]
+        end = torch.where(at < live, torch.minimum(end, live), torch.zeros_like(end))
+    end = torch.maximum(end, torch.zeros_like(end))
+    return begin.to(torch.int32).contiguous(), end.to(torch.int32).contiguous()
+
+
+def _view(x):
+    """x where the kernels can read it in place (adjacent columns, 16-byte rows, real strides), else a copy."""
+    st, sh = x.stride(), x.shape
+    if st[3] == 1 and x.data_ptr() % 16 == 0:
+        for i in (0, 1, 2):
+            if sh[i] > 1 and (st[i] <= 0 or st[i] % 8):
+                break
+        else:
+            return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _check(q, k, v, begin, end, scale, softcap, slopes):
+    _need_cuda(q, k, v, begin, end, slopes)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4 or t.dtype != torch.bfloat16:
+            raise ValueError(f"{name} must be bf16 [batch, tokens, heads, head size]")
+    dev = q.device
+    for t in (k, v, begin, end, slopes):
+        if t is not None and t.device != dev:
+            raise ValueError("attention arguments must be on one device")
+    B, Sq, Hq, D = q.shape
+    Sk, Hkv = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"{Hq} query heads do not share {Hkv} key/value heads evenly")
+    if D > MAX_HEAD_DIM or D < 8 or D % 8:
+        raise ValueError(f"unsupported_capability: head size {D} (multiples of 8 up to {MAX_HEAD_DIM})")
+    for name, t in (("begin", begin), ("end", end)):
+        if t.dtype != torch.int32 or t.shape != (B, Sq):
+            raise ValueError(f"{name} must be int32 [batch, query tokens]")
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (Hq,)):
+        raise ValueError("slopes must be fp32 [query heads]")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError("scale must be positive and finite")
+    softcap = float(softcap or 0.0)
+    if not (softcap >= 0 and math.isfinite(softcap)):
+        raise ValueError("softcap must be >= 0 and finite")
+    return B, Sq, Sk, Hq, Hkv, D, scale, softcap
+
+
+def _strides(*tensors):
+    return (ctypes.c_int64 * (3 * len(tensors)))(*(s for t in tensors for s in t.stride()[:3]))
+
+
+def _contiguous(t):
+    return None if t is None else t.contiguous()
+
+
+def fwd(q, k, v, begin, end, *, scale=None, softcap=0.0, slopes=None):
+    """(out bf16 [B, Sq, Hq, D], lse fp32 [B, Sq, Hq]) of q [B, Sq, Hq, D] over
+    k, v [B, Sk, Hkv, D] (bf16, any views; head h reads key/value head
+    h // (Hq // Hkv)).
+
+    begin, end: int32 [B, Sq], the keys each query sees (see ``row_ranges``); a
+    query that sees none gets 0 and a log sum of -inf.
+    scale: of q . k, default D ** -0.5.  softcap > 0: softcap * tanh(x / softcap).
+    slopes: fp32 [Hq]; x -= slopes[h] * |i + Sk - Sq - j|."""
+    B, Sq, Sk, Hq, Hkv, D, scale, softcap = _check(q, k, v, begin, end, scale, softcap, slopes)
+    out = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=q.device)
+    lse = torch.empty((B, Sq, Hq), dtype=torch.float32, device=q.device)
+    if out.numel() == 0:
+        return out, lse
+    q, k, v = _view(q), _view(k), _view(v)
+    begin, end, slopes = begin.contiguous(), end.contiguous(), _contiguous(slopes)
+    with on_device(q):
+        n = _lib.load().fl_attn_fwd_workspace_bytes(B, Sq, Sk, Hq, Hkv, D)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        _lib.call("fl_attn_fwd", _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v), B, Sq, Sk, Hq, Hkv, D, _ptr(begin),
+                  _ptr(end), scale, softcap, _ptr(slopes), _ptr(out), _ptr(lse), _ptr(ws), n, stream_of(q))
+    return out, lse
+
+
+def bwd(dout, q, k, v, out, lse, begin, end, *, scale=None, softcap=0.0, slopes=None):
+    """(dq, dk, dv) of fwd(): bf16, contiguous; dk and dv summed over the query
+    heads that share them, in a fixed order.  out and lse: what fwd() returned."""
+    B, Sq, Sk, Hq, Hkv, D, scale, softcap = _check(q, k, v, begin, end, scale, softcap, slopes)
+    _need_cuda(dout, out, lse)
+    if dout.shape != q.shape or out.shape != q.shape or dout.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+        raise ValueError("dout and out must be bf16 of q's shape")
+    if lse.shape != (B, Sq, Hq) or lse.dtype != torch.float32:
+        raise ValueError("lse must be fp32 [batch, query tokens, query heads]")
+    if any(t.device != q.device for t in (dout, out, lse)):
+        raise ValueError("attention arguments must be on one device")
+    dq = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=q.device)
+    dk = torch.empty((B, Sk, Hkv, D), dtype=torch.bfloat16, device=q.device)
+    dv = torch.empty_like(dk)
+    if dq.numel() + dk.numel() == 0:
+        return dq, dk, dv
+    q, k, v, dout = _view(q), _view(k), _view(v), _view(dout)
+    out, lse = out.contiguous(), lse.contiguous()
+    begin, end, slopes = begin.contiguous(), end.contiguous(), _contiguous(slopes)
+    with on_device(q):
+        n = _lib.load().fl_attn_bwd_workspace_bytes(B, Sq, Hq, Hkv)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        _lib.call("fl_attn_bwd", _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v, dout), _ptr(out), _ptr(lse),
+                  B, Sq, Sk, Hq, Hkv, D, _ptr(begin), _ptr(end), scale, softcap, _ptr(slopes), _ptr(dq), _ptr(dk),
+                  _ptr(dv), _ptr(ws), n, stream_of(q))
+    return dq, dk, dv
+
+
+class _Attend(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, begin, end, scale, softcap, slopes):
+        out, lse = fwd(q, k, v, begin, end, scale=scale, softcap=softcap, slopes=slopes)
+        ctx.scale, ctx.softcap = scale, softcap
+        ctx.save_for_backward(q, k, v, out, lse, begin, end, slopes)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse, begin, end, slopes = ctx.saved_tensors
+        dq, dk, dv = bwd(dout, q, k, v, out, lse, begin, end, scale=ctx.scale, softcap=ctx.softcap, slopes=slopes)
+        return dq, dk, dv, None, None, None, None, None
+
+
+def attend(q, k, v, begin, end, *, scale=None, softcap=0.0, slopes=None):
+    """fwd()'s output, differentiable in q, k and v (the ranges and slopes are constants)."""
+    if slopes is not None and slopes.requires_grad:
+        raise ValueError("unsupported_capability: slopes get no gradient")
+    return _Attend.apply(q, k, v, begin, end, scale, softcap, slopes)

@@ -1,0 +1,551 @@
+// Attention forward over row ranges (see fl_attn.cuh for the formulas).
+//
+// A CTA takes a tile of 128 (packed) query rows and walks the 128-key tiles
+// that its rows see, with the running maximum m and sum l of a softmax:
+//   S = Q K^T (tcgen05, accumulator in TMEM)
+//   p = 2^(x - m) in FP32, l += sum p, P = bf16(p) over S's columns in TMEM
+//   O += P V (tcgen05, A operand from TMEM)
+// Roles: one warp issues TMA loads, one the MMAs, four own the rows (a thread
+// per row, so row maxima and sums need no exchange).  Two CTAs share an SM:
+// one's softmax runs under the other's products.
+//
+// O is rescaled only when a row's maximum has grown by more than 2^8 over the
+// one in use (the sums then stay far inside FP32's range); otherwise the old
+// reference stays.  P is rounded to bf16 as the second product's operand: half
+// a step of each probability, of the same size as rounding the result.
+//
+// Few rows over many keys (a decode step): the key tiles are split over
+// several CTAs whose normalised FP32 results and log sums are joined by a
+// second kernel.
+#include <cuda_bf16.h>
+#include <cstdint>
+#include <map>
+#include <mutex>
+
+#include "fl_attn.cuh"
+
+namespace fl {
+namespace attn {
+
+constexpr int kFwdThreads = 192;
+constexpr float kRescale = 8.0f;   // growth of the maximum (in powers of two) that rescales O
+
+template <int HD>
+struct Fwd {
+  static constexpr int kStages = HD == 64 ? 2 : 1;       // K and V tiles in flight
+  static constexpr int kTileBytes = HD / 64 * kTile * 128;
+  static constexpr int kSmem = 1024 + (1 + 2 * kStages) * kTileBytes + 256;
+  static constexpr int kTmem = 256;                      // S (P over it) + O
+};
+
+struct FwdArgs {
+  Shape s;
+  __nv_bfloat16* out;   // [B, Sq, Hq, D]
+  float* lse;           // [B, Sq, Hq]
+  float* part_o;        // [splits][B Sq Hq][D] (splits > 1)
+  float* part_lse;      // [splits][B Sq Hq]
+  uint32_t* status;
+  int tiles, splits;
+};
+
+struct __align__(16) FwdBars {
+  uint64_t q_full, qk_done, p_full, pv_done;
+  uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2];
+  uint32_t tmem, abort_word;
+};
+
+template <int HD, bool kBias>
+__global__ void __launch_bounds__(kFwdThreads, 2)
+    fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+               const __grid_constant__ CUtensorMap tm_v, const FwdArgs a) {
+  using C = Fwd<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* qs = smem;
+  uint8_t* ks = qs + C::kTileBytes;
+  uint8_t* vs = ks + C::kStages * C::kTileBytes;
+  FwdBars* bars = reinterpret_cast<FwdBars*>(vs + C::kStages * C::kTileBytes);
+  volatile uint32_t* abort_word = &bars->abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Shape& s = a.s;
+
+  // Late tiles first: under a causal mask they see the most keys.
+  const int per = s.Hkv * s.groups * s.B * a.splits;
+  const int tile = a.tiles - 1 - static_cast<int>(blockIdx.x) / per;
+  int rest = static_cast<int>(blockIdx.x) % per;
+  const int hg = rest % (s.Hkv * s.groups);
+  rest /= s.Hkv * s.groups;
+  const int b = rest % s.B, split = rest / s.B;
+  const int kvh = hg / s.groups;
+  const int h0 = hg << s.lgp;
+  const int t0 = tile * (kTile >> s.lgp);
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->q_full, 1);
+    mbar_init(&bars->qk_done, 1);
+    mbar_init(&bars->p_full, 4);
+    mbar_init(&bars->pv_done, 1);
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&bars->k_full[i], 1);
+      mbar_init(&bars->v_full[i], 1);
+      mbar_init(&bars->k_empty[i], 1);
+      mbar_init(&bars->v_empty[i], 1);
+    }
+    bars->abort_word = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem, C::kTmem);
+    tmem_relinquish();
+  }
+  // Every warp finds the tile's key range itself.
+  const Range r = tile_range(s, b, t0, kTile >> s.lgp);
+  int k_first = 0, n = 0;
+  if (r.min_lo < r.max_hi) {
+    k_first = r.min_lo / kTile;
+    n = (r.max_hi + kTile - 1) / kTile - k_first;
+  }
+  if (a.splits > 1) {
+    const int from = static_cast<int>(static_cast<int64_t>(n) * split / a.splits);
+    const int to = static_cast<int>(static_cast<int64_t>(n) * (split + 1) / a.splits);
+    k_first += from;
+    n = to - from;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_s = bars->tmem, tmem_o = bars->tmem + kTile;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      tma_prefetch_desc(&tm_q);
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+      mbar_arrive_expect_tx(&bars->q_full, C::kTileBytes);
+      for (int c = 0; c < HD / 64; ++c) tma_load_4d(qs + c * kTile * 128, &tm_q, 64 * c, h0, t0, b, &bars->q_full);
+      bool ok = true;
+      int kn = 0, vn = 0;  // loads issued
+      for (int j = 0; j < n && ok; ++j) {
+        const int st = j % C::kStages;
+        const uint32_t ph = (j / C::kStages - 1) & 1;
+        const int key = (k_first + j) * kTile;
+        if (j >= C::kStages && !mbar_wait(&bars->k_empty[st], ph, abort_word, a.status, kStatusTimeoutEmpty)) break;
+        mbar_arrive_expect_tx(&bars->k_full[st], C::kTileBytes);
+        for (int c = 0; c < HD / 64; ++c)
+          tma_load_4d(ks + st * C::kTileBytes + c * kTile * 128, &tm_k, 64 * c, kvh, key, b, &bars->k_full[st]);
+        ++kn;
+        if (j >= C::kStages && !mbar_wait(&bars->v_empty[st], ph, abort_word, a.status, kStatusTimeoutEmpty)) break;
+        mbar_arrive_expect_tx(&bars->v_full[st], C::kTileBytes);
+        for (int c = 0; c < HD / 64; ++c)
+          tma_load_4d(vs + st * C::kTileBytes + c * kTile * 128, &tm_v, 64 * c, kvh, key, b, &bars->v_full[st]);
+        ++vn;
+      }
+      // No copy may be in flight when the CTA leaves.
+      uint32_t none = 0;
+      mbar_wait(&bars->q_full, 0, &none, a.status, kStatusTimeoutDrain);
+      for (int i = max(kn - C::kStages, 0); i < kn; ++i)
+        mbar_wait(&bars->k_full[i % C::kStages], (i / C::kStages) & 1, &none, a.status, kStatusTimeoutDrain);
+      for (int i = max(vn - C::kStages, 0); i < vn; ++i)
+        mbar_wait(&bars->v_full[i % C::kStages], (i / C::kStages) & 1, &none, a.status, kStatusTimeoutDrain);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0) {
+      const uint32_t id_s = idesc_bf16_f32(kTile, kTile), id_o = idesc_bf16_f32_bmn(kTile, HD);
+      bool ok = mbar_wait(&bars->q_full, 0, abort_word, a.status, kStatusTimeoutFull);
+      int pv = 0, qk = 0;
+      for (int j = 0; j < n && ok; ++j) {
+        const int st = j % C::kStages;
+        const uint32_t ph = (j / C::kStages) & 1;
+        // S shares its columns with P: the product that reads P(j - 1) has to be done.
+        if (!mbar_wait(&bars->k_full[st], ph, abort_word, a.status, kStatusTimeoutFull) ||
+            (j > 0 && !mbar_wait(&bars->pv_done, (j - 1) & 1, abort_word, a.status, kStatusTimeoutAccum)))
+          break;
+        tc_fence_after();
+        mma_rows<HD>(tmem_s, smem_u32(qs), smem_u32(ks + st * C::kTileBytes), kTile, id_s);
+        tc_commit(&bars->k_empty[st]);
+        tc_commit(&bars->qk_done);
+        ++qk;
+        if (!mbar_wait(&bars->v_full[st], ph, abort_word, a.status, kStatusTimeoutFull) ||
+            !mbar_wait(&bars->p_full, j & 1, abort_word, a.status, kStatusTimeoutFull))
+          break;
+        tc_fence_after();
+        mma_cols<HD, kTile>(tmem_o, tmem_s, smem_u32(vs + st * C::kTileBytes), id_o, j > 0);
+        tc_commit(&bars->v_empty[st]);
+        tc_commit(&bars->pv_done);
+        ++pv;
+      }
+      // The products still under way read shared memory and TMEM.
+      uint32_t none = 0;
+      if (qk) mbar_wait(&bars->qk_done, (qk - 1) & 1, &none, a.status, kStatusTimeoutDrain);
+      if (pv) mbar_wait(&bars->pv_done, (pv - 1) & 1, &none, a.status, kStatusTimeoutDrain);
+    }
+  } else {
+    const int quarter = warp & 3;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const int row = quarter * 32 + lane;
+    const int tok = t0 + (row >> s.lgp), head = h0 + (row & ((1 << s.lgp) - 1));
+    int lo = 0, hi = 0;
+    if (tok < s.Sq) row_range(s, b, tok, lo, hi);
+    const float slope2 = kBias && s.slopes ? s.slopes[head] * kLog2e : 0.f;
+    const int qpos = tok + s.Sk - s.Sq;
+    const float mult = kBias ? 1.0f : s.sl2;   // from what TMEM holds to powers of two
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      const int key0 = (k_first + j) * kTile;
+      const bool whole = r.max_lo <= key0 && r.min_hi >= key0 + kTile;
+      if (!mbar_wait_warp(&bars->qk_done, j & 1, abort_word, a.status, kStatusTimeoutAccum)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int lo_c = lo - key0, hi_c = hi - key0;
+      float mx = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < kTile; c += 32) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tmem_s + lanes + c, v);
+        tmem_wait_ld();
+        if constexpr (kBias) {
+          // The transformed scores go back into TMEM for the second look.
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float th;
+            float x = score2(s, __uint_as_float(v[i]), slope2, qpos - (key0 + c + i), th);
+            if (!whole && (c + i < lo_c || c + i >= hi_c)) x = -INFINITY;
+            v[i] = __float_as_uint(x);
+          }
+          tmem_st_32x32b_x32(tmem_s + lanes + c, v);
+          tmem_wait_st();
+        } else if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c + i < lo_c || c + i >= hi_c) v[i] = 0xff800000u;
+        }
+        float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          m0 = fmaxf(m0, __uint_as_float(v[i]));
+          m1 = fmaxf(m1, __uint_as_float(v[i + 1]));
+          m2 = fmaxf(m2, __uint_as_float(v[i + 2]));
+          m3 = fmaxf(m3, __uint_as_float(v[i + 3]));
+        }
+        mx = fmaxf(fmaxf(mx, fmaxf(m0, m1)), fmaxf(m2, m3));
+      }
+      mx *= mult;
+      if (j == 0) {
+        m = mx;
+      } else {
+        const bool grow = mx > m + kRescale;
+        if (__any_sync(0xffffffffu, grow)) {
+          // O is at rest: S(j) was issued after P(j - 1) V had completed.
+          const float by = grow ? ex2(m - mx) : 1.0f;
+          if (grow) m = mx;
+          l *= by;
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(tmem_o + lanes + c, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * by);
+            tmem_st_32x32b_x32(tmem_o + lanes + c, v);
+          }
+          tmem_wait_st();
+        }
+      }
+      const float neg = m == -INFINITY ? 0.f : -m;
+      float l0 = 0.f, l1 = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < kTile; c += 32) {
+        uint32_t v[32], w[16];
+        tmem_ld_32x32b_x32(tmem_s + lanes + c, v);
+        tmem_wait_ld();
+        if (!kBias && !whole) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c + i < lo_c || c + i >= hi_c) v[i] = 0xff800000u;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p0 = ex2(fmaf(__uint_as_float(v[2 * i]), mult, neg));
+          const float p1 = ex2(fmaf(__uint_as_float(v[2 * i + 1]), mult, neg));
+          l0 += p0;
+          l1 += p1;
+          w[i] = pack_bf16x2(p0, p1);
+        }
+        // P's columns lie in the part of S that has been read.
+        tmem_st_32x32b_x16(tmem_s + lanes + c / 2, w);
+      }
+      l += l0 + l1;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->p_full);
+    }
+    if (n > 0 && ok)
+      ok = mbar_wait_warp(&bars->pv_done, (n - 1) & 1, abort_word, a.status, kStatusTimeoutAccum);
+    tc_fence_after();
+    if (n == 0 || ok) {
+      const int64_t at = (static_cast<int64_t>(b) * s.Sq + tok) * s.Hq + head;
+      const int64_t rows = static_cast<int64_t>(s.B) * s.Sq * s.Hq;
+      const bool live = tok < s.Sq, seen = n > 0 && l != 0.f;
+      const float inv = seen ? 1.0f / l : 0.f;
+      if (live) {
+        const float lse = seen ? (m + log2f(l)) * kLn2 : -INFINITY;
+        if (a.splits > 1)
+          a.part_lse[split * rows + at] = lse;
+        else
+          a.lse[at] = lse;
+      }
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t v[32];
+        if (n > 0) {
+          tmem_ld_32x32b_x32(tmem_o + lanes + c, v);
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = seen ? __float_as_uint(__uint_as_float(v[i]) * inv) : 0u;
+        if (!live) continue;
+        if (a.splits > 1) {
+          float4* o = reinterpret_cast<float4*>(a.part_o + (split * rows + at) * s.D + c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (c + 4 * i < s.D)
+              o[i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
+                                 __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+        } else {
+          uint4* o = reinterpret_cast<uint4*>(a.out + at * s.D + c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (c + 8 * i < s.D) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = pack_bf16x2(__uint_as_float(v[8 * i + 2 * e]), __uint_as_float(v[8 * i + 2 * e + 1]));
+              o[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(bars->tmem, C::kTmem);
+  }
+}
+
+// Joins the splits of a row: weights 2^(lse_s - max) over their sum, splits in
+// order.  16 lanes to a row, 8 columns to a lane.
+__global__ void join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse, int splits,
+                            int64_t rows, int D, __nv_bfloat16* __restrict__ out, float* __restrict__ lse) {
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
+  const int d = (threadIdx.x & 15) * 8;
+  if (row >= rows) return;
+  float top = -INFINITY;
+  for (int i = 0; i < splits; ++i) top = fmaxf(top, part_lse[i * rows + row]);
+  float sum = 0.f, o[8] = {};
+  if (top != -INFINITY) {
+    for (int i = 0; i < splits; ++i) {
+      const float w = ex2((part_lse[i * rows + row] - top) * kLog2e);
+      sum += w;
+      if (d < D && w != 0.f) {
+        const float4* p = reinterpret_cast<const float4*>(part_o + (i * rows + row) * D + d);
+        const float4 x = p[0], y = p[1];
+        o[0] += w * x.x, o[1] += w * x.y, o[2] += w * x.z, o[3] += w * x.w;
+        o[4] += w * y.x, o[5] += w * y.y, o[6] += w * y.z, o[7] += w * y.w;
+      }
+    }
+  }
+  const float inv = sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum;
+  if (d < D)
+    *reinterpret_cast<uint4*>(out + row * D + d) =
+        make_uint4(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
+                   pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
+  if (d == 0) lse[row] = sum == 0.f ? -INFINITY : top + log2f(sum) * kLn2;
+}
+
+// Splits of the key tiles: none while the row tiles fill half the SMs; else
+// towards two CTAs per SM, each keeping two key tiles at least.
+int fwd_splits(int64_t ctas, int Sk) {
+  const int64_t key_tiles = (Sk + kTile - 1) / kTile;
+  if (ctas > 74 || key_tiles < 4) return 1;
+  int64_t n = 296 / ctas;
+  if (n > key_tiles / 2) n = key_tiles / 2;
+  return n < 1 ? 1 : static_cast<int>(n);
+}
+
+int packed_log2(int Hq, int Hkv) {
+  const int g = Hq / Hkv;
+  if (g & (g - 1)) return 0;
+  int l = 0;
+  while ((1 << l) < g && l < 6) ++l;
+  return l;
+}
+
+void fill_shape(Shape& s, int B, int Sq, int Sk, int Hq, int Hkv, int D, const int* begin, const int* end, float scale,
+                float cap, const float* slopes) {
+  s.B = B;
+  s.Sq = Sq;
+  s.Sk = Sk;
+  s.Hq = Hq;
+  s.Hkv = Hkv;
+  s.D = D;
+  s.lgp = packed_log2(Hq, Hkv);
+  s.groups = (Hq / Hkv) >> s.lgp;
+  s.scale = scale;
+  s.sl2 = scale * kLog2e;
+  s.cap2 = cap * kLog2e;
+  s.icap2 = cap != 0.f ? 2.0f * kLog2e * scale / cap : 0.f;
+  s.begin = begin;
+  s.end = end;
+  s.slopes = slopes;
+}
+
+int64_t fwd_ctas(int B, int Sq, int Hq, int Hkv) {
+  const int lgp = packed_log2(Hq, Hkv);
+  const int64_t tiles = (static_cast<int64_t>(Sq) + (kTile >> lgp) - 1) / (kTile >> lgp);
+  return tiles * B * (Hq >> lgp);
+}
+
+template <int HD, bool kBias>
+int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdArgs& a, int64_t grid,
+               cudaStream_t stream) {
+  int rc = allow_smem(reinterpret_cast<const void*>(&fwd_kernel<HD, kBias>), Fwd<HD>::kSmem);
+  if (rc) return rc;
+  fwd_kernel<HD, kBias><<<static_cast<unsigned>(grid), kFwdThreads, Fwd<HD>::kSmem, stream>>>(q, k, v, a);
+  return FL_OK;
+}
+
+}  // namespace attn
+
+// Raises `kernel`'s dynamic shared-memory limit once per device.
+int allow_smem(const void* kernel, int bytes) {
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, bool> done;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return set_error(FL_ERR_CUDA, "cudaGetDevice: %s", cudaGetErrorString(e));
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count({kernel, dev})) return FL_OK;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return set_error(FL_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  done[{kernel, dev}] = true;
+  return FL_OK;
+}
+
+int attn_map(CUtensorMap* map, const void* base, int64_t batch_stride, int64_t token_stride, int64_t head_stride, int B,
+             int S, int H, int D, int heads, int tokens) {
+  // A dimension of one element may have any stride: give it one that the map accepts.
+  const uint64_t row = static_cast<uint64_t>(D) * 2;
+  const uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(H), static_cast<uint64_t>(S),
+                            static_cast<uint64_t>(B)};
+  const uint64_t strides[3] = {H > 1 ? static_cast<uint64_t>(head_stride) * 2 : row,
+                               S > 1 ? static_cast<uint64_t>(token_stride) * 2 : row,
+                               B > 1 ? static_cast<uint64_t>(batch_stride) * 2 : row};
+  const uint32_t box[4] = {64, static_cast<uint32_t>(heads), static_cast<uint32_t>(tokens), 1};
+  return make_tensor_map(map, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, dims, strides, box,
+                         CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int attn_check(const char* who, int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D, const int64_t* strides,
+               int tensors, const void* const* bases, const int* begin, const int* end, float scale, float cap) {
+  if (B < 0 || Sq < 0 || Sk < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv)
+    return set_error(FL_ERR_ARG, "%s: bad batch, length or head counts", who);
+  if (B > (1 << 16) || Sq > (1 << 30) || Sk > (1 << 30) || Hq > (1 << 12))
+    return set_error(FL_ERR_ARG, "%s: batch, length or head count too large", who);
+  if (D < 8 || D > 128 || D % 8) return set_error(FL_ERR_ARG, "%s: head size must be a multiple of 8 in [8, 128]", who);
+  if (!(scale > 0.f) || scale > 3.0e38f) return set_error(FL_ERR_ARG, "%s: scale must be positive and finite", who);
+  if (!(cap >= 0.f) || cap > 3.0e38f) return set_error(FL_ERR_ARG, "%s: the cap must be >= 0 and finite", who);
+  if (B == 0 || Sq == 0) return FL_OK;
+  if (!begin || !end) return set_error(FL_ERR_ARG, "%s: null pointer", who);
+  if (attn::fwd_ctas(static_cast<int>(B), static_cast<int>(Sq), Hq, Hkv) > (int64_t(1) << 30))
+    return set_error(FL_ERR_ARG, "%s: too many row tiles", who);
+  if (!strides) return set_error(FL_ERR_ARG, "%s: null strides", who);
+  const int64_t S[4] = {Sq, Sk, Sk, Sq};
+  const int H[4] = {Hq, Hkv, Hkv, Hq};
+  for (int i = 0; i < tensors; ++i) {
+    if (S[i] == 0) continue;
+    if (!bases[i] || (reinterpret_cast<uintptr_t>(bases[i]) & 15u))
+      return set_error(FL_ERR_ARG, "%s: tensors must be non-null and 16-byte aligned", who);
+    const int64_t n[3] = {B, S[i], H[i]};
+    for (int d = 0; d < 3; ++d) {
+      const int64_t st = strides[3 * i + d];
+      if (n[d] > 1 && (st <= 0 || st % 8 || st >= (int64_t(1) << 38)))
+        return set_error(FL_ERR_ARG, "%s: strides must be positive multiples of 8 elements", who);
+    }
+  }
+  return FL_OK;
+}
+
+}  // namespace fl
+
+using namespace fl;
+
+extern "C" {
+
+size_t fl_attn_fwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D) {
+  if (B <= 0 || Sq <= 0 || Sk <= 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 8 || B > (1 << 16) || Sq > (1 << 30) ||
+      Sk > (1 << 30))
+    return 0;
+  const int splits = attn::fwd_splits(attn::fwd_ctas((int)B, (int)Sq, Hq, Hkv), (int)Sk);
+  if (splits == 1) return 0;
+  return static_cast<size_t>(splits) * B * Sq * Hq * (D + 1) * sizeof(float);
+}
+
+int fl_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* strides, int64_t B, int64_t Sq,
+                int64_t Sk, int Hq, int Hkv, int D, const int32_t* begin, const int32_t* end, float scale,
+                float softcap, const float* slopes, uint16_t* out, float* lse, void* workspace,
+                size_t workspace_bytes, void* stream) {
+  const void* bases[3] = {q, k, v};
+  int rc = attn_check("fl_attn_fwd", B, Sq, Sk, Hq, Hkv, D, strides, 3, bases, begin, end, scale, softcap);
+  if (rc || B == 0 || Sq == 0) return rc;
+  if (!out || !lse || (reinterpret_cast<uintptr_t>(out) & 15u))
+    return set_error(FL_ERR_ARG, "fl_attn_fwd: out and lse must be given, out 16-byte aligned");
+  const size_t need = fl_attn_fwd_workspace_bytes(B, Sq, Sk, Hq, Hkv, D);
+  if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
+    return set_error(FL_ERR_ARG, "fl_attn_fwd: workspace missing, short or not 16-byte aligned");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  attn::FwdArgs a{};
+  attn::fill_shape(a.s, (int)B, (int)Sq, (int)Sk, Hq, Hkv, D, begin, end, scale, softcap, slopes);
+  a.out = reinterpret_cast<__nv_bfloat16*>(out);
+  a.lse = lse;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || !(a.status = status_word(dev)))
+    return set_error(FL_ERR_CUDA, "fl_attn_fwd: status word unavailable");
+  const int pg = 1 << a.s.lgp;
+  const int64_t ctas = attn::fwd_ctas((int)B, (int)Sq, Hq, Hkv);
+  a.tiles = static_cast<int>(ctas / B / (Hq >> a.s.lgp));
+  a.splits = Sk ? attn::fwd_splits(ctas, (int)Sk) : 1;
+  const int64_t rows = B * Sq * Hq;
+  if (a.splits > 1) {
+    a.part_o = static_cast<float*>(workspace);
+    a.part_lse = a.part_o + a.splits * rows * D;
+  }
+  CUtensorMap mq{}, mk{}, mv{};
+  if ((rc = attn_map(&mq, q, strides[0], strides[1], strides[2], (int)B, (int)Sq, Hq, D, pg, attn::kTile >> a.s.lgp)))
+    return rc;
+  if (Sk && ((rc = attn_map(&mk, k, strides[3], strides[4], strides[5], (int)B, (int)Sk, Hkv, D, 1, attn::kTile)) ||
+             (rc = attn_map(&mv, v, strides[6], strides[7], strides[8], (int)B, (int)Sk, Hkv, D, 1, attn::kTile))))
+    return rc;
+  const bool bias = softcap != 0.f || slopes;
+  const int64_t grid = ctas * a.splits;
+  rc = D <= 64 ? (bias ? attn::launch_fwd<64, true>(mq, mk, mv, a, grid, st)
+                       : attn::launch_fwd<64, false>(mq, mk, mv, a, grid, st))
+               : (bias ? attn::launch_fwd<128, true>(mq, mk, mv, a, grid, st)
+                       : attn::launch_fwd<128, false>(mq, mk, mv, a, grid, st));
+  if (rc) return rc;
+  if (a.splits > 1)
+    attn::join_kernel<<<static_cast<unsigned>((rows * 16 + 127) / 128), 128, 0, st>>>(a.part_o, a.part_lse, a.splits,
+                                                                                     rows, D, a.out, lse);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_error(FL_ERR_CUDA, "fl_attn_fwd: %s", cudaGetErrorString(e));
+  return FL_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,166 @@
+// Shared pieces of the attention kernels (fl_attn.cu, fl_attn_bwd.cu).
+//
+// Row i of a sequence sees the keys begin[i] <= j < end[i].  Scores:
+//   x_ij = scale q_i . k_j,  [cap tanh(x / cap)],  [- slope_h |i + Sk - Sq - j|]
+// and o_i = sum_j softmax(x_i)_j v_j over the seen keys (0 for a row that sees
+// none).  Query heads share key/value heads in groups of Hq / Hkv.
+//
+// Packed rows: where a group's size is a power of two, a tile's rows are the
+// group's heads of consecutive tokens (row r = token r >> lgp, head r & (pg - 1)),
+// so a key/value tile is read once for the whole group and a few tokens still
+// fill a tile.
+#pragma once
+#include <cuda_bf16.h>
+#include <cstdint>
+
+#include "fl_host.h"
+#include "fl_ptx.cuh"
+
+namespace fl {
+namespace attn {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kTile = 128;        // rows (or keys) of a resident tile: the MMA's M
+constexpr int kBwdTile = 64;      // rows (or keys) of a streamed backward tile
+constexpr int kNone = 0x7fffffff;
+
+struct Shape {
+  int B, Sq, Sk, Hq, Hkv, D;
+  int lgp;       // log2 of the packed heads pg
+  int groups;    // Hq / Hkv / pg
+  float scale;   // of q . k
+  float sl2;     // scale * log2(e)
+  float cap2;    // cap * log2(e), 0 = no cap
+  float icap2;   // 2 log2(e) scale / cap: tanh's argument as a power of two
+  const int* begin;
+  const int* end;
+  const float* slopes;  // [Hq] or null
+};
+
+// What the rows of a tile see: {min begin, max end} over its rows that see
+// anything, {max begin, min end} over all its rows inside the sequence (a row
+// that sees nothing makes those impossible to cover).
+struct Range {
+  int min_lo, max_hi, max_lo, min_hi;
+};
+
+__device__ __forceinline__ void row_range(const Shape& s, int b, int tok, int& lo, int& hi) {
+  const int64_t i = static_cast<int64_t>(b) * s.Sq + tok;
+  lo = max(s.begin[i], 0);
+  hi = min(s.end[i], s.Sk);
+  if (lo >= hi) lo = hi = 0;
+}
+
+// Range of the tokens [t0, t0 + n): one warp, every lane gets the result.
+__device__ __forceinline__ Range tile_range(const Shape& s, int b, int t0, int n) {
+  Range r{kNone, 0, 0, kNone};
+  for (int i = threadIdx.x & 31; i < n; i += 32) {
+    if (t0 + i >= s.Sq) break;
+    int lo, hi;
+    row_range(s, b, t0 + i, lo, hi);
+    if (lo < hi) {
+      r.min_lo = min(r.min_lo, lo);
+      r.max_hi = max(r.max_hi, hi);
+      r.max_lo = max(r.max_lo, lo);
+      r.min_hi = min(r.min_hi, hi);
+    } else {
+      r.max_lo = kNone;
+      r.min_hi = 0;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    r.min_lo = min(r.min_lo, __shfl_xor_sync(0xffffffffu, r.min_lo, o));
+    r.max_hi = max(r.max_hi, __shfl_xor_sync(0xffffffffu, r.max_hi, o));
+    r.max_lo = max(r.max_lo, __shfl_xor_sync(0xffffffffu, r.max_lo, o));
+    r.min_hi = min(r.min_hi, __shfl_xor_sync(0xffffffffu, r.min_hi, o));
+  }
+  return r;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// tanh(y) from 2^(2 y log2 e): absolute error of a few 1e-7 everywhere, which
+// the cap multiplies (the hardware's tanh would leave 2^-11 of the cap).
+__device__ __forceinline__ float tanh_from(float two_y_log2e) { return 1.0f - 2.0f * rcp(1.0f + ex2(two_y_log2e)); }
+
+// A score in units of log2: cap and distance applied.  th receives the tanh.
+__device__ __forceinline__ float score2(const Shape& s, float qk, float slope2, int dist, float& th) {
+  float x;
+  th = 0.f;
+  if (s.cap2 != 0.f) {
+    th = tanh_from(qk * s.icap2);
+    x = s.cap2 * th;
+  } else {
+    x = qk * s.sl2;
+  }
+  return x - slope2 * static_cast<float>(abs(dist));
+}
+
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, int w,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// D[128 x n] (+)= A . B^T, both K-major in shared memory: A 128 rows, B
+// `b_rows` rows, each as HD / 64 chunks of rows of 128 bytes.
+template <int HD>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, int b_rows, uint32_t idesc) {
+#pragma unroll
+  for (int kk = 0; kk < HD / 16; ++kk) {
+    const uint64_t ad = sdesc_kmajor_sw128(a + (kk / 4) * kTile * 128) + 2 * (kk % 4);
+    const uint64_t bd = sdesc_kmajor_sw128(b + (kk / 4) * b_rows * 128) + 2 * (kk % 4);
+    mma_ss(d, ad, bd, idesc, kk != 0);
+  }
+}
+
+// D[128 x HD] (+)= A . B: A bf16 [128 x rows] in TMEM, B [rows x HD] in shared
+// memory (the same chunks, read with the columns as the MN side).
+template <int HD, int kRows>
+__device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a_tmem, uint32_t b, uint32_t idesc, bool accumulate) {
+#pragma unroll
+  for (int kk = 0; kk < kRows / 16; ++kk) {
+    const uint64_t bd = sdesc_mnmajor_sw128(b + kk * 2048, kRows * 128, 1024);
+    mma_ts(d, a_tmem + kk * 8, bd, idesc, accumulate || kk != 0);
+  }
+}
+
+int packed_log2(int Hq, int Hkv);
+// Row tiles of kTile packed rows over all heads and sequences.
+int64_t fwd_ctas(int B, int Sq, int Hq, int Hkv);
+void fill_shape(Shape& s, int B, int Sq, int Sk, int Hq, int Hkv, int D, const int* begin, const int* end, float scale,
+                float cap, const float* slopes);
+
+}  // namespace attn
+
+// Tiled tensor map of any rank: dims and box innermost first, stride_bytes of
+// the dimensions from the second on (fl_gemm.cu).
+int make_tensor_map(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int rank, const uint64_t* dims,
+                    const uint64_t* stride_bytes, const uint32_t* box, CUtensorMapSwizzle swz);
+int allow_smem(const void* kernel, int bytes);
+
+// Argument checks of both directions; bases and strides (batch, token, head) of
+// q, k, v and, with tensors = 4, dout.
+int attn_check(const char* who, int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D, const int64_t* strides,
+               int tensors, const void* const* bases, const int* begin, const int* end, float scale, float cap);
+
+// bf16 [B, S, H, D] with element strides, as boxes of 64 columns x `heads`
+// heads x `tokens` tokens (128-byte swizzle; columns past D read as zero).
+int attn_map(CUtensorMap* map, const void* base, int64_t batch_stride, int64_t token_stride, int64_t head_stride, int B,
+             int S, int H, int D, int heads, int tokens);
+
+}  // namespace fl
