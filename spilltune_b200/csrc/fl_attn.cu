@@ -199,40 +199,32 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
         break;
       }
       tc_fence_after();
-      const int lo_c = lo - key0, hi_c = hi - key0;
-      float mx = -INFINITY;
-#pragma unroll 1
-      for (int c = 0; c < kTile; c += 32) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(tmem_s + lanes + c, v);
-        tmem_wait_ld();
-        if constexpr (kBias) {
-          // The transformed scores go back into TMEM for the second look.
+      // The row's 128 scores, in registers from here on.
+      uint32_t v[kTile];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float th;
-            float x = score2(s, __uint_as_float(v[i]), slope2, qpos - (key0 + c + i), th);
-            if (!whole && (c + i < lo_c || c + i >= hi_c)) x = -INFINITY;
-            v[i] = __float_as_uint(x);
-          }
-          tmem_st_32x32b_x32(tmem_s + lanes + c, v);
-          tmem_wait_st();
-        } else if (!whole) {
+      for (int c = 0; c < kTile; c += 32)
+        tmem_ld_32x32b_x32(tmem_s + lanes + c, reinterpret_cast<uint32_t(&)[32]>(v[c]));
+      tmem_wait_ld();
+      if constexpr (kBias) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c + i < lo_c || c + i >= hi_c) v[i] = 0xff800000u;
+        for (int i = 0; i < kTile; ++i) {
+          float th;
+          v[i] = __float_as_uint(score2(s, __uint_as_float(v[i]), slope2, qpos - (key0 + i), th));
         }
-        float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          m0 = fmaxf(m0, __uint_as_float(v[i]));
-          m1 = fmaxf(m1, __uint_as_float(v[i + 1]));
-          m2 = fmaxf(m2, __uint_as_float(v[i + 2]));
-          m3 = fmaxf(m3, __uint_as_float(v[i + 3]));
-        }
-        mx = fmaxf(fmaxf(mx, fmaxf(m0, m1)), fmaxf(m2, m3));
       }
-      mx *= mult;
+      if (!whole) {
+        const int lo_c = lo - key0, hi_c = hi - key0;
+#pragma unroll
+        for (int i = 0; i < kTile; ++i)
+          if (i < lo_c || i >= hi_c) v[i] = 0xff800000u;
+      }
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < kTile; i += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          m4[e] = fmaxf(m4[e], fmaxf(__uint_as_float(v[i + e]), __uint_as_float(v[i + 4 + e])));
+      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mult;
       if (j == 0) {
         m = mx;
       } else {
@@ -243,40 +235,38 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
           if (grow) m = mx;
           l *= by;
 #pragma unroll 1
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(tmem_o + lanes + c, v);
+          for (int c = 0; c < HD; c += 16) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(tmem_o + lanes + c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * by);
-            tmem_st_32x32b_x32(tmem_o + lanes + c, v);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
+            tmem_st_32x32b_x16(tmem_o + lanes + c, o);
           }
           tmem_wait_st();
         }
       }
       const float neg = m == -INFINITY ? 0.f : -m;
-      float l0 = 0.f, l1 = 0.f;
-#pragma unroll 1
+      const uint64_t mult_2 = pair(mult, mult), neg_2 = pair(neg, neg);
+      uint64_t sum0 = 0, sum1 = 0;   // (0, 0)
+#pragma unroll
       for (int c = 0; c < kTile; c += 32) {
-        uint32_t v[32], w[16];
-        tmem_ld_32x32b_x32(tmem_s + lanes + c, v);
-        tmem_wait_ld();
-        if (!kBias && !whole) {
+        uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c + i < lo_c || c + i >= hi_c) v[i] = 0xff800000u;
+        for (int i = 0; i < 16; i += 2) {
+          float x0, x1, x2, x3;
+          unpair(fma2(pair(v[c + 2 * i], v[c + 2 * i + 1]), mult_2, neg_2), x0, x1);
+          unpair(fma2(pair(v[c + 2 * i + 2], v[c + 2 * i + 3]), mult_2, neg_2), x2, x3);
+          x0 = ex2(x0), x1 = ex2(x1), x2 = ex2(x2), x3 = ex2(x3);
+          sum0 = add2(sum0, pair(x0, x1));
+          sum1 = add2(sum1, pair(x2, x3));
+          w[i] = pack_bf16x2(x0, x1);
+          w[i + 1] = pack_bf16x2(x2, x3);
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p0 = ex2(fmaf(__uint_as_float(v[2 * i]), mult, neg));
-          const float p1 = ex2(fmaf(__uint_as_float(v[2 * i + 1]), mult, neg));
-          l0 += p0;
-          l1 += p1;
-          w[i] = pack_bf16x2(p0, p1);
-        }
-        // P's columns lie in the part of S that has been read.
         tmem_st_32x32b_x16(tmem_s + lanes + c / 2, w);
       }
+      float l0, l1;
+      unpair(add2(sum0, sum1), l0, l1);
       l += l0 + l1;
       tmem_wait_st();
       tc_fence_before();

@@ -1,26 +1,37 @@
 // Attention backward over row ranges (see fl_attn.cuh for the formulas).
 //
-//   delta_i = do_i . o_i,  p = 2^(x - lse),  ds = p (do v^T - delta) [(1 - tanh^2)]
+//   delta_i = sum_j p_ij dp_ij,  dp = do v^T,  p = 2^(x - lse),
+//   ds = p f (dp - delta),  f = 1 - tanh^2 under a cap, else 1
 //   dv = p^T do,  dk = scale ds^T q,  dq = scale ds k
 //
-// Three launches: delta with the row tiles' key ranges; dk and dv, a CTA per
-// 128 keys of a key/value head, walking the query tiles of its whole head
-// group (so the group's sum stays in one accumulator); dq, a CTA per 128
-// (packed) query rows, walking the key tiles.  S and do v^T are formed in both:
-// seven products instead of five, but no sum crosses CTAs, so nothing is added
-// by atomics and equal inputs give equal bits.
+// Two launches: dq, a CTA per 128 (packed) query rows, walking the key tiles;
+// then dk and dv, a CTA per 128 keys of a key/value head, walking the query
+// tiles of its whole head group (so the group's sum stays in one accumulator).
+// S and dp are formed in both: more products than one kernel would need, but no
+// sum crosses CTAs, so nothing is added by atomics and equal inputs give equal
+// bits.
 //
-// Both product kernels are one template.  Two tiles of 128 rows stay in shared
-// memory (k and v, or q and do); tiles of 64 rows of the other two stream
-// through a ring.  Per streamed tile:
+// delta is known only once a row's keys have been walked.  do . o is delta up
+// to the rounding of o, which is too far off for rows with few keys: there p
+// (dp - delta) is a small difference.  So the dq kernel works with d0 = do . o,
+// sums delta in FP32 beside it, and corrects at the end:
+//   dq = scale (sum p f (dp - d0) k - (delta - d0) sum p f k),
+// the last sum being one more product over operands that are there already
+// (delta - d0 is small, so its bf16 operands are exact enough).  The dk/dv
+// kernel gets the summed delta.
+//
+// Both are one template.  Two tiles of 128 rows stay in shared memory (q and
+// do, or k and v); tiles of 64 rows of the other two stream through a ring.
+// Per streamed tile:
 //   S = A1 B1^T, P' = A2 B2^T  (128 x 64 each, TMEM, two buffers)
 //   p and ds in registers -> bf16 over S and P' in TMEM
-//   acc += p B2 and ds B1 (dk, dv: rows are keys), or ds B1 (dq: rows are queries)
+//   acc += ds B1 and p f B1 (dq) or p B2 (dk, dv)
 // Eight warps own the elements, four to a buffer, so one buffer's exponentials
 // run under the other's products.  bf16 p and ds are the products' operands:
 // half a step of each term, of the same size as rounding the result.
 #include <cuda_bf16.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "fl_attn.cuh"
 
@@ -41,9 +52,12 @@ struct Bwd {
 
 struct BwdArgs {
   Shape s;
+  const __nv_bfloat16* out;   // [B, Sq, Hq, D]
+  const __nv_bfloat16* dout;  // strided
+  int64_t do_batch, do_token, do_head;
   const float* lse;      // [B, Sq, Hq]
-  const float* delta;    // [B, Sq, Hq]
-  const Range* ranges;   // [B, q_tiles], tiles of kBwdTile packed rows
+  float* delta;          // [B, Sq, Hq]: written by the dq kernel, read by the other
+  Range* ranges;         // [B, q_tiles], tiles of kBwdTile packed rows: likewise
   __nv_bfloat16* dq;     // [B, Sq, Hq, D]
   __nv_bfloat16* dk;     // [B, Sk, Hkv, D]
   __nv_bfloat16* dv;
@@ -61,41 +75,19 @@ struct __align__(16) BwdBars {
   int first, last;
 };
 
-// delta, and the ranges of the streamed query tiles (the first range_blocks blocks).
-__global__ void __launch_bounds__(256) prep_kernel(const Shape s, const __nv_bfloat16* __restrict__ dout,
-                                                   int64_t db, int64_t dt, int64_t dh,
-                                                   const __nv_bfloat16* __restrict__ out, float* __restrict__ delta,
-                                                   Range* __restrict__ ranges, int q_tiles, int range_blocks) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (static_cast<int>(blockIdx.x) < range_blocks) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + warp;
-    if (i >= static_cast<int64_t>(q_tiles) * s.B) return;
-    const int b = static_cast<int>(i / q_tiles), t = static_cast<int>(i % q_tiles);
-    const Range r = tile_range(s, b, t * (kBwdTile >> s.lgp), kBwdTile >> s.lgp);
-    if (lane == 0) ranges[i] = r;
-    return;
-  }
-  // 16 lanes to a row, 8 columns to a lane.
-  const int64_t row = (static_cast<int64_t>(blockIdx.x - range_blocks) * 256 + threadIdx.x) >> 4;
-  const int64_t rows = static_cast<int64_t>(s.B) * s.Sq * s.Hq;
-  const int d = (lane & 15) * 8;
+// Dot product of two rows of D bf16 values (D a multiple of 8, 16-byte aligned).
+__device__ __forceinline__ float row_dot(const __nv_bfloat16* x, const __nv_bfloat16* y, int D) {
   float sum = 0.f;
-  if (row < rows && d < s.D) {
-    const int h = static_cast<int>(row % s.Hq);
-    const int64_t bt = row / s.Hq;
-    const int64_t t = bt % s.Sq, b = bt / s.Sq;
-    const uint4 x = *reinterpret_cast<const uint4*>(dout + b * db + t * dt + h * dh + d);
-    const uint4 y = *reinterpret_cast<const uint4*>(out + row * s.D + d);
-    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+  for (int d = 0; d < D; d += 8) {
+    const uint4 a = *reinterpret_cast<const uint4*>(x + d), b = *reinterpret_cast<const uint4*>(y + d);
+    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      sum = fmaf(__uint_as_float(xw[i] << 16), __uint_as_float(yw[i] << 16), sum);
-      sum = fmaf(__uint_as_float(xw[i] & 0xFFFF0000u), __uint_as_float(yw[i] & 0xFFFF0000u), sum);
+      sum = fmaf(__uint_as_float(aw[i] << 16), __uint_as_float(bw[i] << 16), sum);
+      sum = fmaf(__uint_as_float(aw[i] & 0xFFFF0000u), __uint_as_float(bw[i] & 0xFFFF0000u), sum);
     }
   }
-#pragma unroll
-  for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (row < rows && (lane & 15) == 0) delta[row] = sum;
+  return sum;
 }
 
 // kDq: rows are packed queries (A1 = q, A2 = do; B1 = k, B2 = v).
@@ -249,12 +241,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_after();
         const int st = i % C::kStages;
         const uint32_t b1 = smem_u32(bs + st * 2 * C::kStr);
-        if constexpr (kDq) {
-          mma_cols<HD, kBwdTile>(tmem + kColAcc, tmem + kColP + kBwdTile * (i & 1), b1, id_acc, i > 0);
-        } else {
-          mma_cols<HD, kBwdTile>(tmem + kColAcc, tmem + kBwdTile * (i & 1), b1 + C::kStr, id_acc, i > 0);
-          mma_cols<HD, kBwdTile>(tmem + kColAcc + HD, tmem + kColP + kBwdTile * (i & 1), b1, id_acc, i > 0);
-        }
+        mma_cols<HD, kBwdTile>(tmem + kColAcc, tmem + kBwdTile * (i & 1), kDq ? b1 : b1 + C::kStr, id_acc, i > 0);
+        mma_cols<HD, kBwdTile>(tmem + kColAcc + HD, tmem + kColP + kBwdTile * (i & 1), b1, id_acc, i > 0);
         tc_commit(&bars->b_empty[st]);
         tc_commit(&bars->acc_done[i & 1]);
       }
@@ -271,7 +259,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     float* my_info = info + group * 2 * 4 * kBwdTile;
     // dq: the row's token, head, range and statistics; else the row's key.
     int tok = 0, head = 0, lo = 0, hi = 0;
-    float lse2 = INFINITY, delta = 0.f;
+    float lse2 = INFINITY, d0 = 0.f;
+    uint64_t dsum2 = 0;                            // (0, 0)
+    const uint64_t sl2_2 = pair(s.sl2, s.sl2);
     const int key = row0 + row;
     if constexpr (kDq) {
       tok = row0 + (row >> s.lgp);
@@ -280,7 +270,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         row_range(s, b, tok, lo, hi);
         const int64_t at = (static_cast<int64_t>(b) * s.Sq + tok) * s.Hq + head;
         lse2 = a.lse[at] * kLog2e;
-        delta = a.delta[at];
+        d0 = row_dot(a.dout + b * a.do_batch + tok * a.do_token + head * a.do_head, a.out + at * s.D, s.D);
+      }
+      // The ranges of this tile's two streamed tiles, for the dk/dv kernel.
+      if (hg == 0 && quarter == 0) {
+        const int t = 2 * tile + group;
+        const Range r = tile_range(s, b, t * q_step, q_step);
+        if (lane == 0 && t < a.q_tiles) a.ranges[static_cast<int64_t>(b) * a.q_tiles + t] = r;
       }
     }
     const float row_slope2 = kDq && kBias && s.slopes ? s.slopes[head] * kLog2e : 0.f;
@@ -301,11 +297,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         // The columns' statistics and ranges, for all rows, through shared memory.
         const int c = tid & (kBwdTile - 1), ct = col0 + (c >> s.lgp);
         if (tid < kBwdTile) {
-          float x = INFINITY, y = 0.f;             // a column past the sequence: p = 0
+          float x = -INFINITY, y = 0.f;            // a column past the sequence: p = 0
           if (ct < s.Sq) {
             const int64_t at = (static_cast<int64_t>(b) * s.Sq + ct) * s.Hq + h_first + (c & (pg - 1));
-            x = a.lse[at] * kLog2e;
-            y = a.delta[at];
+            x = -a.lse[at] * kLog2e;
+            y = -a.delta[at];
           }
           buf[c] = x;
           buf[kBwdTile + c] = y;
@@ -324,64 +320,117 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         continue;                                  // the group's other warps count on the barrier
       }
       tc_fence_after();
-#pragma unroll 1
-      for (int c = 0; c < kBwdTile; c += 32) {
-        uint32_t sv[32], pv[32], w[16];
-        tmem_ld_32x32b_x32(tmem + kBwdTile * group + lanes + c, sv);
-        tmem_ld_32x32b_x32(tmem + kColP + kBwdTile * group + lanes + c, pv);
-        tmem_wait_ld();
+      const uint32_t at_s = tmem + kBwdTile * group + lanes, at_p = at_s + kColP;
+      uint32_t sv[kBwdTile], pv[kBwdTile];
 #pragma unroll
-        for (int q = 0; q < 32; q += 4) {
-          float l4[4], d4[4];
-          int lo4[4], hi4[4];
+      for (int c = 0; c < kBwdTile; c += 32) {
+        tmem_ld_32x32b_x32(at_s + c, reinterpret_cast<uint32_t(&)[32]>(sv[c]));
+        tmem_ld_32x32b_x32(at_p + c, reinterpret_cast<uint32_t(&)[32]>(pv[c]));
+      }
+      tmem_wait_ld();
+      // Columns c .. c + 3 of the row: p (dq: p f) into sv, ds into pv.
+      auto four = [&](int c, auto masked) {
+        uint64_t nl[2], nd[2];                     // -lse2 and -delta of the columns
+        if constexpr (kDq) {
+          nl[0] = nl[1] = pair(-lse2, -lse2);
+          nd[0] = nd[1] = pair(-d0, -d0);
+        } else {
+          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(buf + c);
+          const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(buf + kBwdTile + c);
+          nl[0] = x.x, nl[1] = x.y;
+          nd[0] = y.x, nd[1] = y.y;
+        }
+        bool hide[4] = {};
+        if constexpr (decltype(masked)::value) {
           if constexpr (kDq) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) l4[e] = lse2, d4[e] = delta, lo4[e] = lo, hi4[e] = hi;
+            for (int e = 0; e < 4; ++e) hide[e] = c + e < lo - col0 || c + e >= hi - col0;
           } else {
-            const float4 x = *reinterpret_cast<const float4*>(buf + c + q);
-            const float4 y = *reinterpret_cast<const float4*>(buf + kBwdTile + c + q);
-            l4[0] = x.x, l4[1] = x.y, l4[2] = x.z, l4[3] = x.w;
-            d4[0] = y.x, d4[1] = y.y, d4[2] = y.z, d4[3] = y.w;
-            if (!whole) {
-              const int4 u = *reinterpret_cast<const int4*>(buf + 2 * kBwdTile + c + q);
-              const int4 v = *reinterpret_cast<const int4*>(buf + 3 * kBwdTile + c + q);
-              lo4[0] = u.x, lo4[1] = u.y, lo4[2] = u.z, lo4[3] = u.w;
-              hi4[0] = v.x, hi4[1] = v.y, hi4[2] = v.z, hi4[3] = v.w;
-            }
+            const int4 u = *reinterpret_cast<const int4*>(buf + 2 * kBwdTile + c);
+            const int4 v = *reinterpret_cast<const int4*>(buf + 3 * kBwdTile + c);
+            hide[0] = key < u.x || key >= v.x;
+            hide[1] = key < u.y || key >= v.y;
+            hide[2] = key < u.z || key >= v.z;
+            hide[3] = key < u.w || key >= v.w;
           }
+        }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int col = c + q + e;
-            const int k_at = kDq ? col0 + col : key;
-            float p, ds, th = 0.f;
-            if constexpr (kBias) {
-              const int at = kDq ? tok : col0 + (col >> s.lgp);
+        for (int h = 0; h < 2; ++h) {
+          const int i = c + 2 * h;
+          float p[2];
+          [[maybe_unused]] float f[2];
+          if constexpr (kBias) {
+            float l[2];
+            unpair(nl[h], l[0], l[1]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int col = i + e;
+              const int at = kDq ? tok : col0 + (col >> s.lgp), k_at = kDq ? col0 + col : key;
               const float slope2 =
                   kDq ? row_slope2 : (s.slopes ? s.slopes[h_first + (col & (pg - 1))] * kLog2e : 0.f);
-              p = ex2(score2(s, __uint_as_float(sv[q + e]), slope2, at + s.Sk - s.Sq - k_at, th) - l4[e]);
-            } else {
-              p = ex2(fmaf(__uint_as_float(sv[q + e]), s.sl2, -l4[e]));
+              float th;
+              p[e] = ex2(score2(s, __uint_as_float(sv[col]), slope2, at + s.Sk - s.Sq - k_at, th) + l[e]);
+              f[e] = 1.0f - th * th;
             }
-            ds = p * (__uint_as_float(pv[q + e]) - d4[e]);
-            if constexpr (kBias) ds *= 1.0f - th * th;
-            if (!whole && (k_at < lo4[e] || k_at >= hi4[e])) p = ds = 0.f;
-            sv[q + e] = __float_as_uint(p);
-            pv[q + e] = __float_as_uint(ds);
+          } else {
+            unpair(fma2(pair(sv[i], sv[i + 1]), sl2_2, nl[h]), p[0], p[1]);
+            p[0] = ex2(p[0]);
+            p[1] = ex2(p[1]);
           }
+          if constexpr (decltype(masked)::value) {
+            if (hide[2 * h]) p[0] = 0.f;
+            if (hide[2 * h + 1]) p[1] = 0.f;
+          }
+          const uint64_t dp = pair(pv[i], pv[i + 1]);
+          uint64_t pp = pair(p[0], p[1]);
+          if constexpr (kDq) {
+            if constexpr (decltype(masked)::value) {
+              // 0 times whatever a hidden key's value makes of dp
+              float x, y;
+              unpair(mul2(pp, dp), x, y);
+              dsum2 = add2(dsum2, pair(hide[2 * h] ? 0.f : x, hide[2 * h + 1] ? 0.f : y));
+            } else {
+              dsum2 = fma2(pp, dp, dsum2);
+            }
+          }
+          uint64_t pf = pp;
+          if constexpr (kBias) pf = mul2(pp, pair(f[0], f[1]));
+          float ds[2];
+          unpair(mul2(pf, add2(dp, nd[h])), ds[0], ds[1]);
+          if constexpr (decltype(masked)::value) {
+            if (hide[2 * h]) ds[0] = 0.f;
+            if (hide[2 * h + 1]) ds[1] = 0.f;
+          }
+          float a0, a1;
+          unpair(kDq ? pf : pp, a0, a1);
+          sv[i / 2] = pack_bf16x2(a0, a1);
+          pv[i / 2] = pack_bf16x2(ds[0], ds[1]);
         }
-        if constexpr (!kDq) {
+      };
+      if (whole) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) w[e] = pack_bf16x2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1]));
-          tmem_st_32x32b_x16(tmem + kBwdTile * group + lanes + c / 2, w);
-        }
+        for (int c = 0; c < kBwdTile; c += 4) four(c, std::false_type{});
+      } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = pack_bf16x2(__uint_as_float(pv[2 * e]), __uint_as_float(pv[2 * e + 1]));
-        tmem_st_32x32b_x16(tmem + kColP + kBwdTile * group + lanes + c / 2, w);
+        for (int c = 0; c < kBwdTile; c += 4) four(c, std::true_type{});
       }
+      tmem_st_32x32b_x32(at_s, reinterpret_cast<uint32_t(&)[32]>(sv[0]));
+      tmem_st_32x32b_x32(at_p, reinterpret_cast<uint32_t(&)[32]>(pv[0]));
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->ds_full[group]);
+    }
+    float fix = 0.f;
+    if constexpr (kDq) {
+      // Each group summed delta over its half of the key tiles.
+      float dsum, odd;
+      unpair(dsum2, dsum, odd);
+      info[group * kTile + row] = dsum + odd;
+      named_barrier_sync(1, 256);
+      dsum = info[row] + info[kTile + row];
+      fix = d0 - dsum;
+      if (group == 0 && tok < s.Sq) a.delta[(static_cast<int64_t>(b) * s.Sq + tok) * s.Hq + head] = dsum;
     }
     if (n > 0 && !mbar_wait_warp(&bars->all_done, 0, abort_word, a.status, kStatusTimeoutAccum)) ok = false;
     tc_fence_after();
@@ -399,8 +448,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int c = c_from; c < c_to; c += 32) {
         uint32_t v[32];
         if (n > 0) {
-          tmem_ld_32x32b_x32(tmem + kColAcc + (kDq ? 0 : group * HD) + lanes + c, v);
-          tmem_wait_ld();
+          tmem_ld_32x32b_x32(tmem + kColAcc + (kDq || group ? HD : 0) + lanes + c, v);
+          if constexpr (kDq) {
+            uint32_t u[32];
+            tmem_ld_32x32b_x32(tmem + kColAcc + lanes + c, u);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              v[e] = __float_as_uint(fmaf(fix, __uint_as_float(u[e]), __uint_as_float(v[e])));
+          } else {
+            tmem_wait_ld();
+          }
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = 0u;
@@ -489,6 +547,11 @@ int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, cons
   const int64_t rows = B * Sq * Hq;
   float* delta = static_cast<float*>(workspace);
   auto* ranges = reinterpret_cast<attn::Range*>(static_cast<uint8_t*>(workspace) + attn::a256(rows * sizeof(float)));
+  a.out = reinterpret_cast<const __nv_bfloat16*>(out);
+  a.dout = reinterpret_cast<const __nv_bfloat16*>(dout);
+  a.do_batch = strides[9];
+  a.do_token = strides[10];
+  a.do_head = strides[11];
   a.lse = lse;
   a.delta = delta;
   a.ranges = ranges;
@@ -499,11 +562,6 @@ int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, cons
   const int pg = 1 << a.s.lgp, q_rows = attn::kTile >> a.s.lgp, q_step = attn::kBwdTile >> a.s.lgp;
   const int64_t key_tiles = (Sk + attn::kTile - 1) / attn::kTile;
   if (key_tiles * B * Hkv > (int64_t(1) << 30)) return set_error(FL_ERR_ARG, "fl_attn_bwd: too many key tiles");
-
-  const int64_t range_blocks = (static_cast<int64_t>(a.q_tiles) * B + 7) / 8, delta_blocks = (rows * 16 + 255) / 256;
-  attn::prep_kernel<<<static_cast<unsigned>(range_blocks + delta_blocks), 256, 0, st>>>(
-      a.s, reinterpret_cast<const __nv_bfloat16*>(dout), strides[9], strides[10], strides[11],
-      reinterpret_cast<const __nv_bfloat16*>(out), delta, ranges, a.q_tiles, static_cast<int>(range_blocks));
 
   // Resident (128 rows) and streamed (64 rows) maps of each tensor.
   CUtensorMap q_res, do_res, k_res, v_res, q_str, do_str, k_str, v_str;
@@ -520,19 +578,19 @@ int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, cons
       (rc = keys_map(&k_str, k, strides + 3, attn::kBwdTile)) || (rc = keys_map(&v_str, v, strides + 6, attn::kBwdTile)))
     return rc;
   const bool bias = softcap != 0.f || slopes;
-  a.tiles = static_cast<int>(key_tiles);
-  const int64_t kv_grid = key_tiles * B * Hkv;
-  rc = D <= 64 ? (bias ? attn::launch_bwd<64, false, true>(k_res, v_res, q_str, do_str, a, kv_grid, st)
-                       : attn::launch_bwd<64, false, false>(k_res, v_res, q_str, do_str, a, kv_grid, st))
-               : (bias ? attn::launch_bwd<128, false, true>(k_res, v_res, q_str, do_str, a, kv_grid, st)
-                       : attn::launch_bwd<128, false, false>(k_res, v_res, q_str, do_str, a, kv_grid, st));
-  if (rc) return rc;
   const int64_t q_grid = attn::fwd_ctas(b, sq, Hq, Hkv);
   a.tiles = static_cast<int>(q_grid / B / (Hq >> a.s.lgp));
   rc = D <= 64 ? (bias ? attn::launch_bwd<64, true, true>(q_res, do_res, k_str, v_str, a, q_grid, st)
                        : attn::launch_bwd<64, true, false>(q_res, do_res, k_str, v_str, a, q_grid, st))
                : (bias ? attn::launch_bwd<128, true, true>(q_res, do_res, k_str, v_str, a, q_grid, st)
                        : attn::launch_bwd<128, true, false>(q_res, do_res, k_str, v_str, a, q_grid, st));
+  if (rc) return rc;
+  a.tiles = static_cast<int>(key_tiles);
+  const int64_t kv_grid = key_tiles * B * Hkv;
+  rc = D <= 64 ? (bias ? attn::launch_bwd<64, false, true>(k_res, v_res, q_str, do_str, a, kv_grid, st)
+                       : attn::launch_bwd<64, false, false>(k_res, v_res, q_str, do_str, a, kv_grid, st))
+               : (bias ? attn::launch_bwd<128, false, true>(k_res, v_res, q_str, do_str, a, kv_grid, st)
+                       : attn::launch_bwd<128, false, false>(k_res, v_res, q_str, do_str, a, kv_grid, st));
   if (rc) return rc;
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(FL_ERR_CUDA, "fl_attn_bwd: %s", cudaGetErrorString(e));
