@@ -66,7 +66,8 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
   uint8_t* vs = ks + C::kStages * C::kTileBytes;
   FwdBars* bars = reinterpret_cast<FwdBars*>(vs + C::kStages * C::kTileBytes);
   volatile uint32_t* abort_word = &bars->abort_word;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Broadcast so that the compiler knows a warp to be of one mind.
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const Shape& s = a.s;
 
   // Late tiles first: under a causal mask they see the most keys.
@@ -129,12 +130,12 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
         const int st = j % C::kStages;
         const uint32_t ph = (j / C::kStages - 1) & 1;
         const int key = (k_first + j) * kTile;
-        if (j >= C::kStages && !mbar_wait(&bars->k_empty[st], ph, abort_word, a.status, kStatusTimeoutEmpty)) break;
+        if (j >= C::kStages && !mbar_wait_short(&bars->k_empty[st], ph, abort_word, a.status, kStatusTimeoutEmpty)) break;
         mbar_arrive_expect_tx(&bars->k_full[st], C::kTileBytes);
         for (int c = 0; c < HD / 64; ++c)
           tma_load_4d(ks + st * C::kTileBytes + c * kTile * 128, &tm_k, 64 * c, kvh, key, b, &bars->k_full[st]);
         ++kn;
-        if (j >= C::kStages && !mbar_wait(&bars->v_empty[st], ph, abort_word, a.status, kStatusTimeoutEmpty)) break;
+        if (j >= C::kStages && !mbar_wait_short(&bars->v_empty[st], ph, abort_word, a.status, kStatusTimeoutEmpty)) break;
         mbar_arrive_expect_tx(&bars->v_full[st], C::kTileBytes);
         for (int c = 0; c < HD / 64; ++c)
           tma_load_4d(vs + st * C::kTileBytes + c * kTile * 128, &tm_v, 64 * c, kvh, key, b, &bars->v_full[st]);
@@ -149,35 +150,47 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
         mbar_wait(&bars->v_full[i % C::kStages], (i / C::kStages) & 1, &none, a.status, kStatusTimeoutDrain);
     }
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
+    // The whole warp walks and one lane issues: operands stay uniform, and the
+    // issue takes few slots of the scheduler that the softmax warps share.
+    if (n > 0) {
       const uint32_t id_s = idesc_bf16_f32(kTile, kTile), id_o = idesc_bf16_f32_bmn(kTile, HD);
-      bool ok = mbar_wait(&bars->q_full, 0, abort_word, a.status, kStatusTimeoutFull);
+      const uint64_t dq = sdesc_kmajor_sw128(smem_u32(qs)), dk = sdesc_kmajor_sw128(smem_u32(ks));
+      const uint64_t dv = cols_desc(smem_u32(vs));
+      auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t bit) {
+        return mbar_wait_short_warp(bar, parity, abort_word, a.status, bit);
+      };
+      bool ok = wait(&bars->q_full, 0, kStatusTimeoutFull);
       int pv = 0, qk = 0;
       for (int j = 0; j < n && ok; ++j) {
         const int st = j % C::kStages;
         const uint32_t ph = (j / C::kStages) & 1;
         // S shares its columns with P: the product that reads P(j - 1) has to be done.
-        if (!mbar_wait(&bars->k_full[st], ph, abort_word, a.status, kStatusTimeoutFull) ||
-            (j > 0 && !mbar_wait(&bars->pv_done, (j - 1) & 1, abort_word, a.status, kStatusTimeoutAccum)))
+        if (!wait(&bars->k_full[st], ph, kStatusTimeoutFull) ||
+            (j > 0 && !wait(&bars->pv_done, (j - 1) & 1, kStatusTimeoutAccum)))
           break;
         tc_fence_after();
-        mma_rows<HD>(tmem_s, smem_u32(qs), smem_u32(ks + st * C::kTileBytes), kTile, id_s);
-        tc_commit(&bars->k_empty[st]);
-        tc_commit(&bars->qk_done);
+        if (elected()) {
+          mma_rows<HD>(tmem_s, dq, dk + st * (C::kTileBytes >> 4), id_s);
+          tc_commit(&bars->k_empty[st]);
+          tc_commit(&bars->qk_done);
+        }
+        __syncwarp();
         ++qk;
-        if (!mbar_wait(&bars->v_full[st], ph, abort_word, a.status, kStatusTimeoutFull) ||
-            !mbar_wait(&bars->p_full, j & 1, abort_word, a.status, kStatusTimeoutFull))
-          break;
+        if (!wait(&bars->v_full[st], ph, kStatusTimeoutFull) || !wait(&bars->p_full, j & 1, kStatusTimeoutFull)) break;
         tc_fence_after();
-        mma_cols<HD, kTile>(tmem_o, tmem_s, smem_u32(vs + st * C::kTileBytes), id_o, j > 0);
-        tc_commit(&bars->v_empty[st]);
-        tc_commit(&bars->pv_done);
+        if (elected()) {
+          mma_cols<HD, kTile>(tmem_o, tmem_s, dv + st * (C::kTileBytes >> 4), id_o, j > 0);
+          tc_commit(&bars->v_empty[st]);
+          tc_commit(&bars->pv_done);
+        }
+        __syncwarp();
         ++pv;
       }
       // The products still under way read shared memory and TMEM.
       uint32_t none = 0;
       if (qk) mbar_wait(&bars->qk_done, (qk - 1) & 1, &none, a.status, kStatusTimeoutDrain);
       if (pv) mbar_wait(&bars->pv_done, (pv - 1) & 1, &none, a.status, kStatusTimeoutDrain);
+      __syncwarp();
     }
   } else {
     const int quarter = warp & 3;
@@ -194,7 +207,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
     for (int j = 0; j < n; ++j) {
       const int key0 = (k_first + j) * kTile;
       const bool whole = r.max_lo <= key0 && r.min_hi >= key0 + kTile;
-      if (!mbar_wait_warp(&bars->qk_done, j & 1, abort_word, a.status, kStatusTimeoutAccum)) {
+      if (!mbar_wait_short_warp(&bars->qk_done, j & 1, abort_word, a.status, kStatusTimeoutAccum)) {
         ok = false;
         break;
       }
@@ -274,7 +287,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       if (lane == 0) mbar_arrive(&bars->p_full);
     }
     if (n > 0 && ok)
-      ok = mbar_wait_warp(&bars->pv_done, (n - 1) & 1, abort_word, a.status, kStatusTimeoutAccum);
+      ok = mbar_wait_short_warp(&bars->pv_done, (n - 1) & 1, abort_word, a.status, kStatusTimeoutAccum);
     tc_fence_after();
     if (n == 0 || ok) {
       const int64_t at = (static_cast<int64_t>(b) * s.Sq + tok) * s.Hq + head;

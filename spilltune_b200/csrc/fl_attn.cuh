@@ -21,8 +21,7 @@ namespace attn {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kTile = 128;        // rows (or keys) of a resident tile: the MMA's M
-constexpr int kBwdTile = 64;      // rows (or keys) of a streamed backward tile
+constexpr int kTile = 128;        // rows or keys of a tile
 constexpr int kNone = 0x7fffffff;
 
 struct Shape {
@@ -118,6 +117,31 @@ __device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
   return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
+// 2^x of two values without the special-function unit, whose 16 results a
+// cycle and SM bound the exponentials: x = i + f with i the nearest integer
+// (by adding 1.5 * 2^23), 2^f on [-1/2, 1/2] by the polynomial of degree 5 with
+// value 1 at 0 whose largest relative error is smallest (1.1e-7, less than the
+// special-function unit's), i added to the exponent.  x <= -127 gives 0.
+__device__ __forceinline__ void ex2_pair(float x0, float x1, float& y0, float& y1) {
+  const float round = 12582912.0f;
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-127.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-127.0f));
+  const uint64_t x = pair(x0, x1);
+  const uint64_t i = add2(x, pair(round, round));
+  const uint64_t f = fma2(add2(i, pair(-round, -round)), pair(-1.0f, -1.0f), x);
+  uint64_t p = fma2(f, pair(0.001326472731307149f, 0.001326472731307149f),
+                    pair(0.009671512991189957f, 0.009671512991189957f));
+  p = fma2(f, p, pair(0.05550733581185341f, 0.05550733581185341f));
+  p = fma2(f, p, pair(0.24022242426872253f, 0.24022242426872253f));
+  p = fma2(f, p, pair(0.6931470036506653f, 0.6931470036506653f));
+  p = fma2(f, p, pair(1.0f, 1.0f));
+  float i0, i1;
+  unpair(i, i0, i1);
+  unpair(p, y0, y1);
+  y0 = __int_as_float(__float_as_int(y0) + (__float_as_int(i0) << 23));
+  y1 = __int_as_float(__float_as_int(y1) + (__float_as_int(i1) << 23));
+}
+
 // tanh(y) from 2^(2 y log2 e): absolute error of a few 1e-7 everywhere, which
 // the cap multiplies (the hardware's tanh would leave 2^-11 of the cap).
 __device__ __forceinline__ float tanh_from(float two_y_log2e) { return 1.0f - 2.0f * rcp(1.0f + ex2(two_y_log2e)); }
@@ -144,27 +168,39 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
-// D[128 x n] (+)= A . B^T, both K-major in shared memory: A 128 rows, B
-// `b_rows` rows, each as HD / 64 chunks of rows of 128 bytes.
+// The lane that issues for a warp: always the same one.
+__device__ __forceinline__ bool elected() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// The descriptors' address field counts 16-byte units and a tile does not wrap
+// it, so a step is an addition: the issuing thread shares its scheduler with
+// element warps and has few slots between two products.
+//
+// D[128 x 128] = A . B^T, both K-major in shared memory: 128 rows as HD / 64
+// chunks of rows of 128 bytes; a and b from sdesc_kmajor_sw128.
 template <int HD>
-__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, int b_rows, uint32_t idesc) {
+__device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
 #pragma unroll
   for (int kk = 0; kk < HD / 16; ++kk) {
-    const uint64_t ad = sdesc_kmajor_sw128(a + (kk / 4) * kTile * 128) + 2 * (kk % 4);
-    const uint64_t bd = sdesc_kmajor_sw128(b + (kk / 4) * b_rows * 128) + 2 * (kk % 4);
-    mma_ss(d, ad, bd, idesc, kk != 0);
+    const uint32_t step = (kk / 4) * (kTile * 128 >> 4) + 2 * (kk % 4);
+    mma_ss(d, a + step, b + step, idesc, kk != 0);
   }
 }
 
-// D[128 x HD] (+)= A . B: A bf16 [128 x rows] in TMEM, B [rows x HD] in shared
-// memory (the same chunks, read with the columns as the MN side).
-template <int HD, int kRows>
-__device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a_tmem, uint32_t b, uint32_t idesc, bool accumulate) {
+// D[128 x HD] (+)= A . B: A bf16 [128 x 128] in TMEM, each kGroup columns of A
+// from a_tmem + kGroup * group on; B [128 x HD] in shared memory (the same
+// chunks, read with the columns as the MN side), b from cols_desc.  kGroup =
+// 128: A is packed.
+__device__ __forceinline__ uint64_t cols_desc(uint32_t addr) { return sdesc_mnmajor_sw128(addr, kTile * 128, 1024); }
+template <int HD, int kGroup>
+__device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, bool accumulate) {
 #pragma unroll
-  for (int kk = 0; kk < kRows / 16; ++kk) {
-    const uint64_t bd = sdesc_mnmajor_sw128(b + kk * 2048, kRows * 128, 1024);
-    mma_ts(d, a_tmem + kk * 8, bd, idesc, accumulate || kk != 0);
-  }
+  for (int kk = 0; kk < kTile / 16; ++kk)
+    mma_ts(d, a_tmem + kk * 16 / kGroup * kGroup + kk * 16 % kGroup / 2, b + kk * (2048 >> 4), idesc,
+           accumulate || kk != 0);
 }
 
 int packed_log2(int Hq, int Hkv);

@@ -21,15 +21,20 @@
 // kernel gets the summed delta.
 //
 // Both are one template.  Two tiles of 128 rows stay in shared memory (q and
-// do, or k and v); tiles of 64 rows of the other two stream through a ring.
+// do, or k and v); tiles of 128 rows of the other two stream through a ring.
 // Per streamed tile:
-//   S = A1 B1^T, P' = A2 B2^T  (128 x 64 each, TMEM, two buffers)
+//   S = A1 B1^T, P' = A2 B2^T  (128 x 128 each, TMEM)
 //   p and ds in registers -> bf16 over S and P' in TMEM
-//   acc += ds B1 and p f B1 (dq) or p B2 (dk, dv)
-// Eight warps own the elements, four to a buffer, so one buffer's exponentials
-// run under the other's products.  bf16 p and ds are the products' operands:
-// half a step of each term, of the same size as rounding the result.
+//   acc1 += p f B1 (dq) or p B2 (dv);  acc2 += ds B1 (dq, dk)
+// S, P' and the accumulators fill TMEM, so nothing is double-buffered; the
+// order acc1(i), S(i + 1), acc2(i), P'(i + 1) keeps the tensor cores on one pair
+// while the sixteen element warps (four to each 32 columns) work on the other.  128 columns per product: an operand from shared memory is fetched
+// once per instruction, and with 64 columns the fetch of the 128 resident rows
+// took twice the product's own time.
+// bf16 p and ds are the products' operands: half a step of each term, of the
+// same size as rounding the result.
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cstdint>
 #include <type_traits>
 
@@ -38,16 +43,28 @@
 namespace fl {
 namespace attn {
 
-constexpr int kBwdThreads = 320;
+constexpr int kGroups = 4;                  // groups of four element warps
+constexpr int kCols = kTile / kGroups;      // columns of a tile that one group owns
+constexpr int kBwdThreads = 64 + 128 * kGroups;
 constexpr int kTmemCols = 512;
-constexpr int kColP = 128, kColAcc = 256;   // TMEM: S buffers, P' buffers, accumulators
+constexpr int kColP = 128, kColAcc = 256;   // TMEM: S, P', the two accumulators
+
+// What the dk/dv kernel needs of 128 packed query rows, left by the dq kernel
+// and loaded with the tile: -lse log2(e), -delta, begin and end of each row,
+// then {max begin, min end} of each kCols rows inside the sequence.  Rows
+// past the sequence get a first entry of -inf, which makes p 0.
+struct __align__(16) RowInfo {
+  float nlse2[kTile], ndelta[kTile];
+  int lo[kTile], hi[kTile];
+  int max_lo[kGroups], min_hi[kGroups];
+};
+constexpr int kInfoBytes = sizeof(RowInfo);
 
 template <int HD>
 struct Bwd {
-  static constexpr int kStages = 3;
-  static constexpr int kRes = HD / 64 * kTile * 128;       // a resident tile
-  static constexpr int kStr = HD / 64 * kBwdTile * 128;    // a streamed tile
-  static constexpr int kSmem = 1024 + 2 * kRes + kStages * 2 * kStr + 4 * 4 * kBwdTile * 4 + 256;
+  static constexpr int kStages = 2;
+  static constexpr int kBytes = HD / 64 * kTile * 128;     // a tile of 128 rows
+  static constexpr int kSmem = 1024 + (2 + 2 * kStages) * kBytes + kStages * kInfoBytes + 256;
 };
 
 struct BwdArgs {
@@ -56,36 +73,34 @@ struct BwdArgs {
   const __nv_bfloat16* dout;  // strided
   int64_t do_batch, do_token, do_head;
   const float* lse;      // [B, Sq, Hq]
-  float* delta;          // [B, Sq, Hq]: written by the dq kernel, read by the other
-  Range* ranges;         // [B, q_tiles], tiles of kBwdTile packed rows: likewise
+  RowInfo* info;         // [B, Hkv * groups, q_tiles]: written by the dq kernel, read by the other
+  Range* ranges;         // [B, q_tiles]: likewise
   __nv_bfloat16* dq;     // [B, Sq, Hq, D]
   __nv_bfloat16* dk;     // [B, Sk, Hkv, D]
   __nv_bfloat16* dv;
   uint32_t* status;
-  int q_tiles;           // of kBwdTile packed rows
+  int q_tiles;           // of kTile packed rows
   int tiles;             // resident tiles per head
 };
 
 struct __align__(16) BwdBars {
   uint64_t a_full;
-  uint64_t b_full[3], b_empty[3];
-  uint64_t sp_full[2], ds_full[2], acc_done[2];
-  uint64_t all_done;
+  uint64_t b_full[2][2], b_empty[2][2];   // [B1, B2][stage]
+  uint64_t s_full, dp_full;               // S, P' written
+  uint64_t p_full, ds_full;               // p, ds written over them
+  uint64_t acc1_done, acc2_done, all_done;
   uint32_t tmem, abort_word;
   int first, last;
 };
 
-// Dot product of two rows of D bf16 values (D a multiple of 8, 16-byte aligned).
-__device__ __forceinline__ float row_dot(const __nv_bfloat16* x, const __nv_bfloat16* y, int D) {
+// Dot product of 8 bf16 columns.
+__device__ __forceinline__ float dot8(const uint4& a, const uint4& b) {
+  const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
   float sum = 0.f;
-  for (int d = 0; d < D; d += 8) {
-    const uint4 a = *reinterpret_cast<const uint4*>(x + d), b = *reinterpret_cast<const uint4*>(y + d);
-    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sum = fmaf(__uint_as_float(aw[i] << 16), __uint_as_float(bw[i] << 16), sum);
-      sum = fmaf(__uint_as_float(aw[i] & 0xFFFF0000u), __uint_as_float(bw[i] & 0xFFFF0000u), sum);
-    }
+  for (int i = 0; i < 4; ++i) {
+    sum = fmaf(__uint_as_float(aw[i] << 16), __uint_as_float(bw[i] << 16), sum);
+    sum = fmaf(__uint_as_float(aw[i] & 0xFFFF0000u), __uint_as_float(bw[i] & 0xFFFF0000u), sum);
   }
   return sum;
 }
@@ -101,12 +116,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* a1 = smem;
-  uint8_t* a2 = a1 + C::kRes;
-  uint8_t* bs = a2 + C::kRes;                              // kStages x (B1, B2)
-  float* info = reinterpret_cast<float*>(bs + C::kStages * 2 * C::kStr);  // [2 groups][2][4][64]
-  BwdBars* bars = reinterpret_cast<BwdBars*>(info + 4 * 4 * kBwdTile);
+  uint8_t* a2 = a1 + C::kBytes;
+  uint8_t* bs = a2 + C::kBytes;                            // [stage][B1, B2]
+  RowInfo* info = reinterpret_cast<RowInfo*>(bs + C::kStages * 2 * C::kBytes);   // [stage]
+  BwdBars* bars = reinterpret_cast<BwdBars*>(info + C::kStages);
   volatile uint32_t* abort_word = &bars->abort_word;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Broadcast so that the compiler knows a warp to be of one mind.
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const Shape& s = a.s;
   const int G = s.Hq / s.Hkv, pg = 1 << s.lgp;
 
@@ -118,20 +134,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int hg = static_cast<int>(blockIdx.x) % per % heads;
   const int b = static_cast<int>(blockIdx.x) % per / heads;
   const int kvh = kDq ? hg / s.groups : hg;
-  const int q_step = kBwdTile >> s.lgp;                    // tokens of a streamed query tile
-  const int row0 = kDq ? tile * (kTile >> s.lgp) : tile * kTile;
+  const int q_step = kTile >> s.lgp;                       // tokens of a query tile
+  const int row0 = kDq ? tile * q_step : tile * kTile;
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->a_full, 1);
-    for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(&bars->b_full[i], 1);
-      mbar_init(&bars->b_empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->sp_full[i], 1);
-      mbar_init(&bars->ds_full[i], 4);
-      mbar_init(&bars->acc_done[i], 1);
-    }
+    for (int i = 0; i < C::kStages; ++i)
+      for (int o = 0; o < 2; ++o) {
+        mbar_init(&bars->b_full[o][i], 1);
+        mbar_init(&bars->b_empty[o][i], 1);
+      }
+    mbar_init(&bars->s_full, 1);
+    mbar_init(&bars->dp_full, 1);
+    mbar_init(&bars->p_full, 4 * kGroups);
+    mbar_init(&bars->ds_full, 4 * kGroups);
+    mbar_init(&bars->acc1_done, 1);
+    mbar_init(&bars->acc2_done, 1);
     mbar_init(&bars->all_done, 1);
     bars->abort_word = 0;
     bars->first = kNone;
@@ -153,10 +171,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   Range mine{};
   int first = 0, n = 0, per_group = 0;
   if constexpr (kDq) {
-    mine = tile_range(s, b, row0, kTile >> s.lgp);
+    mine = tile_range(s, b, row0, q_step);
     if (mine.min_lo < mine.max_hi) {
-      first = mine.min_lo / kBwdTile;
-      n = (mine.max_hi + kBwdTile - 1) / kBwdTile - first;
+      first = mine.min_lo / kTile;
+      n = (mine.max_hi + kTile - 1) / kTile - first;
     }
   } else {
     int lo = kNone, hi = -1;
@@ -184,79 +202,105 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tma_prefetch_desc(&tm_b1);
       tma_prefetch_desc(&tm_b2);
       const int ah = kDq ? hg << s.lgp : kvh;
-      mbar_arrive_expect_tx(&bars->a_full, 2 * C::kRes);
+      mbar_arrive_expect_tx(&bars->a_full, 2 * C::kBytes);
       for (int c = 0; c < HD / 64; ++c) {
         tma_load_4d(a1 + c * kTile * 128, &tm_a1, 64 * c, ah, row0, b, &bars->a_full);
         tma_load_4d(a2 + c * kTile * 128, &tm_a2, 64 * c, ah, row0, b, &bars->a_full);
       }
-      int i = 0;
-      for (; i < n; ++i) {
+      int done[2] = {0, 0};                        // loads issued
+      bool ok = true;
+      for (int i = 0; i < n && ok; ++i) {
         const int st = i % C::kStages;
-        if (i >= C::kStages && !mbar_wait(&bars->b_empty[st], (i / C::kStages - 1) & 1, abort_word, a.status,
-                                          kStatusTimeoutEmpty))
-          break;
         int bh, br;
         if constexpr (kDq) {
           bh = kvh;
-          br = (first + i) * kBwdTile;
+          br = (first + i) * kTile;
         } else {
           bh = kvh * G + (i / per_group) * pg;
           br = (first + i % per_group) * q_step;
         }
-        uint8_t* b1 = bs + st * 2 * C::kStr;
-        mbar_arrive_expect_tx(&bars->b_full[st], 2 * C::kStr);
-        for (int c = 0; c < HD / 64; ++c) {
-          tma_load_4d(b1 + c * kBwdTile * 128, &tm_b1, 64 * c, bh, br, b, &bars->b_full[st]);
-          tma_load_4d(b1 + C::kStr + c * kBwdTile * 128, &tm_b2, 64 * c, bh, br, b, &bars->b_full[st]);
+        for (int o = 0; o < 2 && ok; ++o) {
+          if (i >= C::kStages && !mbar_wait_short(&bars->b_empty[o][st], (i / C::kStages - 1) & 1, abort_word, a.status,
+                                            kStatusTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          uint8_t* dst = bs + (st * 2 + o) * C::kBytes;
+          mbar_arrive_expect_tx(&bars->b_full[o][st], C::kBytes + (!kDq && o == 0 ? kInfoBytes : 0));
+          if (!kDq && o == 0)
+            bulk_load(info + st,
+                      a.info + (static_cast<int64_t>(b) * s.Hkv * s.groups + kvh * s.groups + i / per_group) *
+                                   a.q_tiles + first + i % per_group,
+                      kInfoBytes, &bars->b_full[o][st]);
+          for (int c = 0; c < HD / 64; ++c)
+            tma_load_4d(dst + c * kTile * 128, o ? &tm_b2 : &tm_b1, 64 * c, bh, br, b, &bars->b_full[o][st]);
+          ++done[o];
         }
       }
       // No copy may be in flight when the CTA leaves.
       uint32_t none = 0;
       mbar_wait(&bars->a_full, 0, &none, a.status, kStatusTimeoutDrain);
-      for (int j = max(i - C::kStages, 0); j < i; ++j)
-        mbar_wait(&bars->b_full[j % C::kStages], (j / C::kStages) & 1, &none, a.status, kStatusTimeoutDrain);
+      for (int o = 0; o < 2; ++o)
+        for (int i = max(done[o] - C::kStages, 0); i < done[o]; ++i)
+          mbar_wait(&bars->b_full[o][i % C::kStages], (i / C::kStages) & 1, &none, a.status, kStatusTimeoutDrain);
     }
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
-      const uint32_t id_s = idesc_bf16_f32(kTile, kBwdTile), id_acc = idesc_bf16_f32_bmn(kTile, HD);
-      bool ok = mbar_wait(&bars->a_full, 0, abort_word, a.status, kStatusTimeoutFull);
-      // S and P' of step i into buffer i & 1, once the products that read the
-      // buffer's p and ds are done.
-      auto scores = [&](int i) -> bool {
-        const int st = i % C::kStages;
-        if (i >= 2 && !mbar_wait(&bars->acc_done[i & 1], ((i >> 1) - 1) & 1, abort_word, a.status, kStatusTimeoutAccum))
-          return false;
-        if (!mbar_wait(&bars->b_full[st], (i / C::kStages) & 1, abort_word, a.status, kStatusTimeoutFull)) return false;
+    // The whole warp walks and one lane issues: operands stay uniform, and the
+    // issue takes few slots of the scheduler that the element warps share.
+    if (n > 0) {
+      const uint32_t id_s = idesc_bf16_f32(kTile, kTile), id_acc = idesc_bf16_f32_bmn(kTile, HD);
+      const uint32_t col_s = tmem, col_p = tmem + kColP;
+      const uint64_t d_a[2] = {sdesc_kmajor_sw128(smem_u32(a1)), sdesc_kmajor_sw128(smem_u32(a2))};
+      const uint64_t d_rows = sdesc_kmajor_sw128(smem_u32(bs)), d_cols = cols_desc(smem_u32(bs));
+      auto at = [&](int i, int o) { return static_cast<uint64_t>((i % C::kStages) * 2 + o) * (C::kBytes >> 4); };
+      auto wait = [&](uint64_t* bar, int phase, uint32_t bit) {
+        return mbar_wait_short_warp(bar, phase & 1, abort_word, a.status, bit);
+      };
+      // S (o = 0) or P' (o = 1) of step i.
+      auto scores = [&](int i, int o) -> bool {
+        if (!wait(&bars->b_full[o][i % C::kStages], i / C::kStages, kStatusTimeoutFull)) return false;
         tc_fence_after();
-        const uint32_t b1 = smem_u32(bs + st * 2 * C::kStr);
-        mma_rows<HD>(tmem + kBwdTile * (i & 1), smem_u32(a1), b1, kBwdTile, id_s);
-        mma_rows<HD>(tmem + kColP + kBwdTile * (i & 1), smem_u32(a2), b1 + C::kStr, kBwdTile, id_s);
-        tc_commit(&bars->sp_full[i & 1]);
+        if (elected()) {
+          mma_rows<HD>(o ? col_p : col_s, d_a[o], d_rows + at(i, o), id_s);
+          tc_commit(o ? &bars->dp_full : &bars->s_full);
+        }
+        __syncwarp();
         return true;
       };
-      ok = ok && scores(0);
+      bool ok = wait(&bars->a_full, 0, kStatusTimeoutFull) && scores(0, 0) && scores(0, 1);
       for (int i = 0; i < n && ok; ++i) {
-        if (i + 1 < n && !scores(i + 1)) break;
-        if (!mbar_wait(&bars->ds_full[i & 1], (i >> 1) & 1, abort_word, a.status, kStatusTimeoutFull)) break;
-        tc_fence_after();
         const int st = i % C::kStages;
-        const uint32_t b1 = smem_u32(bs + st * 2 * C::kStr);
-        mma_cols<HD, kBwdTile>(tmem + kColAcc, tmem + kBwdTile * (i & 1), kDq ? b1 : b1 + C::kStr, id_acc, i > 0);
-        mma_cols<HD, kBwdTile>(tmem + kColAcc + HD, tmem + kColP + kBwdTile * (i & 1), b1, id_acc, i > 0);
-        tc_commit(&bars->b_empty[st]);
-        tc_commit(&bars->acc_done[i & 1]);
+        if (!wait(&bars->p_full, i, kStatusTimeoutFull)) break;
+        tc_fence_after();
+        if (elected()) {
+          mma_cols<HD, kCols>(tmem + kColAcc, col_s, d_cols + at(i, kDq ? 0 : 1), id_acc, i > 0);
+          tc_commit(&bars->b_empty[1][st]);
+          tc_commit(&bars->acc1_done);
+        }
+        __syncwarp();
+        // S shares its columns with p, P' with ds: the products that read those have to be done.
+        if (i + 1 < n && !(wait(&bars->acc1_done, i, kStatusTimeoutAccum) && scores(i + 1, 0))) break;
+        if (!wait(&bars->ds_full, i, kStatusTimeoutFull)) break;
+        tc_fence_after();
+        if (elected()) {
+          mma_cols<HD, kCols>(tmem + kColAcc + HD, col_p, d_cols + at(i, 0), id_acc, i > 0);
+          tc_commit(&bars->b_empty[0][st]);
+          tc_commit(&bars->acc2_done);
+        }
+        __syncwarp();
+        if (i + 1 < n && !(wait(&bars->acc2_done, i, kStatusTimeoutAccum) && scores(i + 1, 1))) break;
       }
       // Completes after every product issued above, also after a wait that gave up.
-      tc_commit(&bars->all_done);
+      if (elected()) tc_commit(&bars->all_done);
       uint32_t none = 0;
       mbar_wait(&bars->all_done, 0, &none, a.status, kStatusTimeoutDrain);
+      __syncwarp();
     }
   } else {
-    const int group = (warp - 2) >> 2;             // the buffer (step parity) this warp serves
-    const int quarter = warp & 3, tid = (threadIdx.x - 64) & 127;
+    const int group = (warp - 2) >> 2;             // the columns this warp owns
+    const int quarter = warp & 3;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const int row = quarter * 32 + lane;           // TMEM lane: the element row this thread owns
-    float* my_info = info + group * 2 * 4 * kBwdTile;
     // dq: the row's token, head, range and statistics; else the row's key.
     int tok = 0, head = 0, lo = 0, hi = 0;
     float lse2 = INFINITY, d0 = 0.f;
@@ -270,208 +314,284 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         row_range(s, b, tok, lo, hi);
         const int64_t at = (static_cast<int64_t>(b) * s.Sq + tok) * s.Hq + head;
         lse2 = a.lse[at] * kLog2e;
-        d0 = row_dot(a.dout + b * a.do_batch + tok * a.do_token + head * a.do_head, a.out + at * s.D, s.D);
       }
-      // The ranges of this tile's two streamed tiles, for the dk/dv kernel.
-      if (hg == 0 && quarter == 0) {
-        const int t = 2 * tile + group;
-        const Range r = tile_range(s, b, t * q_step, q_step);
-        if (lane == 0 && t < a.q_tiles) a.ranges[static_cast<int64_t>(b) * a.q_tiles + t] = r;
+      // d0 = do . o: 16 lanes to a row, two rows of a warp at a time, handed to
+      // the rows' owners through shared memory.
+      float* dots = reinterpret_cast<float*>(info + 1);
+      const int ew = warp - 2, d = (lane & 15) * 8;
+      constexpr int kRounds = kTile / (8 * kGroups);
+      uint4 x[kRounds], y[kRounds];
+#pragma unroll
+      for (int i = 0; i < kRounds; ++i) {
+        const int rr = ew * 2 * kRounds + 2 * i + (lane >> 4);
+        const int64_t rt = row0 + (rr >> s.lgp), rh = (hg << s.lgp) + (rr & (pg - 1));
+        x[i] = y[i] = make_uint4(0, 0, 0, 0);
+        if (rt < s.Sq && d < s.D) {
+          x[i] = *reinterpret_cast<const uint4*>(a.dout + b * a.do_batch + rt * a.do_token + rh * a.do_head + d);
+          y[i] = *reinterpret_cast<const uint4*>(
+              a.out + ((static_cast<int64_t>(b) * s.Sq + rt) * s.Hq + rh) * s.D + d);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < kRounds; ++i) {
+        float sum = dot8(x[i], y[i]);
+#pragma unroll
+        for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if ((lane & 15) == 0) dots[ew * 2 * kRounds + 2 * i + (lane >> 4)] = sum;
+      }
+      named_barrier_sync(1, 128 * kGroups);
+      d0 = dots[row];
     }
     const float row_slope2 = kDq && kBias && s.slopes ? s.slopes[head] * kLog2e : 0.f;
     bool ok = true;
-    for (int i = group; i < n; i += 2) {
-      float* buf = my_info + ((i >> 1) & 1) * 4 * kBwdTile;
+    for (int i = 0; i < n; ++i) {
+      const int st = i % C::kStages;
+      const RowInfo& cols = info[st];              // dk, dv: of the step's columns
+      const int mine0 = group * kCols;             // the first of the group's columns
       bool whole;
       int col0, h_first = 0;                       // dq: first key; else first token and head
-      if constexpr (kDq) {
-        col0 = (first + i) * kBwdTile;
-        whole = mine.max_lo <= col0 && mine.min_hi >= col0 + kBwdTile;
-      } else {
-        const int t = first + i % per_group;
-        col0 = t * q_step;
-        h_first = kvh * G + (i / per_group) * pg;
-        const Range r = a.ranges[static_cast<int64_t>(b) * a.q_tiles + t];
-        whole = r.max_lo <= row0 && r.min_hi >= row0 + kTile;
-        // The columns' statistics and ranges, for all rows, through shared memory.
-        const int c = tid & (kBwdTile - 1), ct = col0 + (c >> s.lgp);
-        if (tid < kBwdTile) {
-          float x = -INFINITY, y = 0.f;            // a column past the sequence: p = 0
-          if (ct < s.Sq) {
-            const int64_t at = (static_cast<int64_t>(b) * s.Sq + ct) * s.Hq + h_first + (c & (pg - 1));
-            x = -a.lse[at] * kLog2e;
-            y = -a.delta[at];
-          }
-          buf[c] = x;
-          buf[kBwdTile + c] = y;
-        } else {
-          int l = 0, h = 0;
-          if (ct < s.Sq) row_range(s, b, ct, l, h);
-          buf[2 * kBwdTile + c] = __int_as_float(l);
-          buf[3 * kBwdTile + c] = __int_as_float(h);
-        }
-        named_barrier_sync(1 + group, 128);
-      }
-      if (ok && !mbar_wait_warp(&bars->sp_full[group], (i >> 1) & 1, abort_word, a.status, kStatusTimeoutAccum))
+      if (!kDq && !mbar_wait_short_warp(&bars->b_full[0][st], (i / C::kStages) & 1, abort_word, a.status,
+                                        kStatusTimeoutFull)) {
         ok = false;
-      if (!ok) {
-        if constexpr (kDq) break;
-        continue;                                  // the group's other warps count on the barrier
+        break;
+      }
+      if constexpr (kDq) {
+        col0 = (first + i) * kTile + mine0;
+        whole = mine.max_lo <= col0 && mine.min_hi >= col0 + kCols;
+      } else {
+        col0 = (first + i % per_group) * q_step + (mine0 >> s.lgp);
+        h_first = kvh * G + (i / per_group) * pg;
+        whole = cols.max_lo[group] <= row0 && cols.min_hi[group] >= row0 + kTile;
+      }
+      if (!mbar_wait_short_warp(&bars->s_full, i & 1, abort_word, a.status, kStatusTimeoutAccum)) {
+        ok = false;
+        break;
       }
       tc_fence_after();
-      const uint32_t at_s = tmem + kBwdTile * group + lanes, at_p = at_s + kColP;
-      uint32_t sv[kBwdTile], pv[kBwdTile];
-#pragma unroll
-      for (int c = 0; c < kBwdTile; c += 32) {
-        tmem_ld_32x32b_x32(at_s + c, reinterpret_cast<uint32_t(&)[32]>(sv[c]));
-        tmem_ld_32x32b_x32(at_p + c, reinterpret_cast<uint32_t(&)[32]>(pv[c]));
-      }
+      const uint32_t at_s = tmem + kCols * group + lanes, at_p = at_s + kColP;
+      uint32_t x[kCols], w[kCols / 2];             // scores, then p; packed operands
+      [[maybe_unused]] __half2 fac[kBias ? kCols / 2 : 1];
+      tmem_ld_32x32b_x32(at_s, x);
       tmem_wait_ld();
-      // Columns c .. c + 3 of the row: p (dq: p f) into sv, ds into pv.
-      auto four = [&](int c, auto masked) {
-        uint64_t nl[2], nd[2];                     // -lse2 and -delta of the columns
+      // Which of the columns c .. c + 3 the row does not see.
+      auto hidden = [&](int c, bool (&hide)[4]) {
+        if constexpr (kDq) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) hide[e] = c + e < lo - col0 || c + e >= hi - col0;
+        } else {
+          const int4 u = *reinterpret_cast<const int4*>(cols.lo + mine0 + c);
+          const int4 v = *reinterpret_cast<const int4*>(cols.hi + mine0 + c);
+          hide[0] = key < u.x || key >= v.x;
+          hide[1] = key < u.y || key >= v.y;
+          hide[2] = key < u.z || key >= v.z;
+          hide[3] = key < u.w || key >= v.w;
+        }
+      };
+      auto exponentials = [&](int c, auto masked) {
+        uint64_t nl[2];                            // -lse2 of the columns
         if constexpr (kDq) {
           nl[0] = nl[1] = pair(-lse2, -lse2);
-          nd[0] = nd[1] = pair(-d0, -d0);
         } else {
-          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(buf + c);
-          const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(buf + kBwdTile + c);
-          nl[0] = x.x, nl[1] = x.y;
-          nd[0] = y.x, nd[1] = y.y;
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(cols.nlse2 + mine0 + c);
+          nl[0] = v.x, nl[1] = v.y;
         }
-        bool hide[4] = {};
-        if constexpr (decltype(masked)::value) {
-          if constexpr (kDq) {
+        float p[4];
+        [[maybe_unused]] float f[4];
+        if constexpr (kBias) {
+          float l[4];
+          unpair(nl[0], l[0], l[1]);
+          unpair(nl[1], l[2], l[3]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) hide[e] = c + e < lo - col0 || c + e >= hi - col0;
-          } else {
-            const int4 u = *reinterpret_cast<const int4*>(buf + 2 * kBwdTile + c);
-            const int4 v = *reinterpret_cast<const int4*>(buf + 3 * kBwdTile + c);
-            hide[0] = key < u.x || key >= v.x;
-            hide[1] = key < u.y || key >= v.y;
-            hide[2] = key < u.z || key >= v.z;
-            hide[3] = key < u.w || key >= v.w;
+          for (int e = 0; e < 4; ++e) {
+            const int col = c + e;
+            const int at = kDq ? tok : col0 + (col >> s.lgp), k_at = kDq ? col0 + col : key;
+            const float slope2 = kDq ? row_slope2 : (s.slopes ? s.slopes[h_first + (col & (pg - 1))] * kLog2e : 0.f);
+            float th;
+            p[e] = ex2(score2(s, __uint_as_float(x[col]), slope2, at + s.Sk - s.Sq - k_at, th) + l[e]);
+            f[e] = 1.0f - th * th;
           }
-        }
+        } else {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int i = c + 2 * h;
-          float p[2];
-          [[maybe_unused]] float f[2];
-          if constexpr (kBias) {
-            float l[2];
-            unpair(nl[h], l[0], l[1]);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int col = i + e;
-              const int at = kDq ? tok : col0 + (col >> s.lgp), k_at = kDq ? col0 + col : key;
-              const float slope2 =
-                  kDq ? row_slope2 : (s.slopes ? s.slopes[h_first + (col & (pg - 1))] * kLog2e : 0.f);
-              float th;
-              p[e] = ex2(score2(s, __uint_as_float(sv[col]), slope2, at + s.Sk - s.Sq - k_at, th) + l[e]);
-              f[e] = 1.0f - th * th;
-            }
-          } else {
-            unpair(fma2(pair(sv[i], sv[i + 1]), sl2_2, nl[h]), p[0], p[1]);
-            p[0] = ex2(p[0]);
-            p[1] = ex2(p[1]);
-          }
-          if constexpr (decltype(masked)::value) {
-            if (hide[2 * h]) p[0] = 0.f;
-            if (hide[2 * h + 1]) p[1] = 0.f;
-          }
-          const uint64_t dp = pair(pv[i], pv[i + 1]);
-          uint64_t pp = pair(p[0], p[1]);
-          if constexpr (kDq) {
-            if constexpr (decltype(masked)::value) {
-              // 0 times whatever a hidden key's value makes of dp
-              float x, y;
-              unpair(mul2(pp, dp), x, y);
-              dsum2 = add2(dsum2, pair(hide[2 * h] ? 0.f : x, hide[2 * h + 1] ? 0.f : y));
+          for (int h = 0; h < 4; h += 2) {
+            unpair(fma2(pair(x[c + h], x[c + h + 1]), sl2_2, nl[h / 2]), p[h], p[h + 1]);
+            if (h == 0 && c % 8 == 0) {            // a quarter of the exponentials
+              ex2_pair(p[h], p[h + 1], p[h], p[h + 1]);
             } else {
-              dsum2 = fma2(pp, dp, dsum2);
+              p[h] = ex2(p[h]);
+              p[h + 1] = ex2(p[h + 1]);
             }
           }
-          uint64_t pf = pp;
-          if constexpr (kBias) pf = mul2(pp, pair(f[0], f[1]));
-          float ds[2];
-          unpair(mul2(pf, add2(dp, nd[h])), ds[0], ds[1]);
-          if constexpr (decltype(masked)::value) {
-            if (hide[2 * h]) ds[0] = 0.f;
-            if (hide[2 * h + 1]) ds[1] = 0.f;
-          }
-          float a0, a1;
-          unpair(kDq ? pf : pp, a0, a1);
-          sv[i / 2] = pack_bf16x2(a0, a1);
-          pv[i / 2] = pack_bf16x2(ds[0], ds[1]);
         }
+        if constexpr (decltype(masked)::value) {
+          bool hide[4];
+          hidden(c, hide);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (hide[e]) p[e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[c + e] = __float_as_uint(p[e]);
+        if constexpr (kBias) {
+          // f waits for dp in 16 bits: 2^-12 of a factor of ds, an eighth of ds's own rounding.
+          fac[c / 2] = __floats2half2_rn(f[0], f[1]);
+          fac[c / 2 + 1] = __floats2half2_rn(f[2], f[3]);
+          if constexpr (kDq) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[e] *= f[e];
+          }
+        }
+        w[c / 2] = pack_bf16x2(p[0], p[1]);
+        w[c / 2 + 1] = pack_bf16x2(p[2], p[3]);
       };
       if (whole) {
 #pragma unroll
-        for (int c = 0; c < kBwdTile; c += 4) four(c, std::false_type{});
+        for (int c = 0; c < kCols; c += 4) exponentials(c, std::false_type{});
       } else {
 #pragma unroll
-        for (int c = 0; c < kBwdTile; c += 4) four(c, std::true_type{});
+        for (int c = 0; c < kCols; c += 4) exponentials(c, std::true_type{});
       }
-      tmem_st_32x32b_x32(at_s, reinterpret_cast<uint32_t(&)[32]>(sv[0]));
-      tmem_st_32x32b_x32(at_p, reinterpret_cast<uint32_t(&)[32]>(pv[0]));
+      tmem_st_32x32b_x16(at_s, w);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->ds_full[group]);
+      if (lane == 0) mbar_arrive(&bars->p_full);
+
+      if (!mbar_wait_short_warp(&bars->dp_full, i & 1, abort_word, a.status, kStatusTimeoutAccum)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      // dp of the columns c .. c + 3 in y; ds into w.
+      auto gradients = [&](const uint32_t* y, int c, auto masked) {
+        uint64_t nd[2];                            // -delta of the columns
+        if constexpr (kDq) {
+          nd[0] = nd[1] = pair(-d0, -d0);
+        } else {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(cols.ndelta + mine0 + c);
+          nd[0] = v.x, nd[1] = v.y;
+        }
+        [[maybe_unused]] bool hide[4];
+        if constexpr (decltype(masked)::value) hidden(c, hide);
+#pragma unroll
+        for (int h = 0; h < 4; h += 2) {
+          const int col = c + h;
+          const uint64_t dp = pair(y[h], y[h + 1]), p = pair(x[col], x[col + 1]);
+          if constexpr (kDq) {
+            if constexpr (decltype(masked)::value) {
+              // p is 0 at a hidden key, but whatever its value makes of dp may not be finite
+              float d_0, d_1;
+              unpair(mul2(p, dp), d_0, d_1);
+              dsum2 = add2(dsum2, pair(hide[h] ? 0.f : d_0, hide[h + 1] ? 0.f : d_1));
+            } else {
+              dsum2 = fma2(p, dp, dsum2);
+            }
+          }
+          uint64_t pf = p;
+          if constexpr (kBias) {
+            const float2 f = __half22float2(fac[col / 2]);
+            pf = mul2(p, pair(f.x, f.y));
+          }
+          float ds[2];
+          unpair(mul2(pf, add2(dp, nd[h / 2])), ds[0], ds[1]);
+          if constexpr (decltype(masked)::value) {
+            if (hide[h]) ds[0] = 0.f;
+            if (hide[h + 1]) ds[1] = 0.f;
+          }
+          w[col / 2] = pack_bf16x2(ds[0], ds[1]);
+        }
+      };
+#pragma unroll
+      for (int c0 = 0; c0 < kCols; c0 += 16) {
+        uint32_t y[16];
+        tmem_ld_32x32b_x16(at_p + c0, y);
+        tmem_wait_ld();
+        if (whole) {
+#pragma unroll
+          for (int c = 0; c < 16; c += 4) gradients(y + c, c0 + c, std::false_type{});
+        } else {
+#pragma unroll
+          for (int c = 0; c < 16; c += 4) gradients(y + c, c0 + c, std::true_type{});
+        }
+      }
+      tmem_st_32x32b_x16(at_p, w);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->ds_full);
     }
     float fix = 0.f;
     if constexpr (kDq) {
-      // Each group summed delta over its half of the key tiles.
+      // Each group summed delta over its columns.
       float dsum, odd;
       unpair(dsum2, dsum, odd);
-      info[group * kTile + row] = dsum + odd;
-      named_barrier_sync(1, 256);
-      dsum = info[row] + info[kTile + row];
+      float* sums = reinterpret_cast<float*>(info);   // [kGroups][128]
+      static_assert(kGroups * kTile * sizeof(float) <= kInfoBytes, "the sums use the first row info's space");
+      sums[group * kTile + row] = dsum + odd;
+      named_barrier_sync(1, 128 * kGroups);
+      dsum = 0.f;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) dsum += sums[g * kTile + row];
       fix = d0 - dsum;
-      if (group == 0 && tok < s.Sq) a.delta[(static_cast<int64_t>(b) * s.Sq + tok) * s.Hq + head] = dsum;
+      RowInfo* o = a.info + (static_cast<int64_t>(b) * heads + hg) * a.q_tiles + tile;
+      if (group == 0) {
+        o->nlse2[row] = tok < s.Sq ? -lse2 : -INFINITY;
+        o->ndelta[row] = tok < s.Sq ? -dsum : 0.f;
+      } else if (group == 1) {
+        o->lo[row] = lo;
+        o->hi[row] = hi;
+      }
+      if (quarter == 0) {
+        const Range h = tile_range(s, b, row0 + ((group * kCols) >> s.lgp), max(kCols >> s.lgp, 1));
+        if (lane == 0) {
+          o->max_lo[group] = h.max_lo;
+          o->min_hi[group] = h.min_hi;
+          if (hg == 0 && group == 0) a.ranges[static_cast<int64_t>(b) * a.q_tiles + tile] = mine;
+        }
+      }
     }
-    if (n > 0 && !mbar_wait_warp(&bars->all_done, 0, abort_word, a.status, kStatusTimeoutAccum)) ok = false;
+    if (n > 0 && !mbar_wait_short_warp(&bars->all_done, 0, abort_word, a.status, kStatusTimeoutAccum)) ok = false;
     tc_fence_after();
     if (ok) {
-      // dq: each group stores half of the columns; else one stores dv, one dk.
+      // dq: each group stores a quarter of the columns; else two store the
+      // halves of dv, two those of dk.
       const bool live = kDq ? tok < s.Sq : key < s.Sk;
+      const bool second = kDq || group >= kGroups / 2;   // of the accumulators
       __nv_bfloat16* o;
       if constexpr (kDq)
         o = a.dq + ((static_cast<int64_t>(b) * s.Sq + tok) * s.Hq + head) * s.D;
       else
-        o = (group ? a.dk : a.dv) + ((static_cast<int64_t>(b) * s.Sk + key) * s.Hkv + kvh) * s.D;
-      const float by = kDq || group ? s.scale : 1.0f;
-      const int c_from = kDq ? group * (HD / 2) : 0, c_to = kDq ? c_from + HD / 2 : HD;
+        o = (second ? a.dk : a.dv) + ((static_cast<int64_t>(b) * s.Sk + key) * s.Hkv + kvh) * s.D;
+      const float by = second ? s.scale : 1.0f;
+      constexpr int kWidth = kDq ? HD / kGroups : HD / (kGroups / 2);
+      const int c_from = (kDq ? group : group & 1) * kWidth;
 #pragma unroll 1
-      for (int c = c_from; c < c_to; c += 32) {
-        uint32_t v[32];
+      for (int c = c_from; c < c_from + kWidth; c += 16) {
+        uint32_t v[16];
         if (n > 0) {
-          tmem_ld_32x32b_x32(tmem + kColAcc + (kDq || group ? HD : 0) + lanes + c, v);
+          tmem_ld_32x32b_x16(tmem + kColAcc + (second ? HD : 0) + lanes + c, v);
           if constexpr (kDq) {
-            uint32_t u[32];
-            tmem_ld_32x32b_x32(tmem + kColAcc + lanes + c, u);
+            uint32_t u[16];
+            tmem_ld_32x32b_x16(tmem + kColAcc + lanes + c, u);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
+            for (int e = 0; e < 16; ++e)
               v[e] = __float_as_uint(fmaf(fix, __uint_as_float(u[e]), __uint_as_float(v[e])));
           } else {
             tmem_wait_ld();
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = 0u;
+          for (int e = 0; e < 16; ++e) v[e] = 0u;
         }
         if (!live) continue;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 2; ++e)
           if (c + 8 * e < s.D) {
-            uint32_t w[4];
+            uint32_t u[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-              w[q] = pack_bf16x2(__uint_as_float(v[8 * e + 2 * q]) * by, __uint_as_float(v[8 * e + 2 * q + 1]) * by);
-            *reinterpret_cast<uint4*>(o + c + 8 * e) = make_uint4(w[0], w[1], w[2], w[3]);
+              u[q] = pack_bf16x2(__uint_as_float(v[8 * e + 2 * q]) * by, __uint_as_float(v[8 * e + 2 * q + 1]) * by);
+            *reinterpret_cast<uint4*>(o + c + 8 * e) = make_uint4(u[0], u[1], u[2], u[3]);
           }
       }
     }
@@ -495,9 +615,7 @@ int launch_bwd(const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& 
   return FL_OK;
 }
 
-size_t a256(size_t n) { return (n + 255) / 256 * 256; }
-
-int64_t q_tiles_of(int64_t Sq, int lgp) { return (Sq + (kBwdTile >> lgp) - 1) / (kBwdTile >> lgp); }
+int64_t q_tiles_of(int64_t Sq, int lgp) { return (Sq + (kTile >> lgp) - 1) / (kTile >> lgp); }
 
 }  // namespace attn
 }  // namespace fl
@@ -506,11 +624,12 @@ using namespace fl;
 
 extern "C" {
 
-// delta [B, Sq, Hq] fp32, then the ranges of the query tiles.
+// The query tiles' row statistics, then their ranges.
 size_t fl_attn_bwd_workspace_bytes(int64_t B, int64_t Sq, int Hq, int Hkv) {
   if (B <= 0 || Sq <= 0 || Hq < 1 || Hkv < 1 || Hq % Hkv) return 0;
-  return attn::a256(static_cast<size_t>(B) * Sq * Hq * sizeof(float)) +
-         static_cast<size_t>(B) * attn::q_tiles_of(Sq, attn::packed_log2(Hq, Hkv)) * sizeof(attn::Range);
+  const int lgp = attn::packed_log2(Hq, Hkv);
+  const size_t tiles = static_cast<size_t>(B) * attn::q_tiles_of(Sq, lgp);
+  return tiles * (Hq >> lgp) * sizeof(attn::RowInfo) + tiles * sizeof(attn::Range);
 }
 
 int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* strides,
@@ -544,53 +663,43 @@ int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, cons
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || !(a.status = status_word(dev)))
     return set_error(FL_ERR_CUDA, "fl_attn_bwd: status word unavailable");
-  const int64_t rows = B * Sq * Hq;
-  float* delta = static_cast<float*>(workspace);
-  auto* ranges = reinterpret_cast<attn::Range*>(static_cast<uint8_t*>(workspace) + attn::a256(rows * sizeof(float)));
+  a.q_tiles = static_cast<int>(attn::q_tiles_of(Sq, a.s.lgp));
+  a.info = static_cast<attn::RowInfo*>(workspace);
+  a.ranges = reinterpret_cast<attn::Range*>(a.info + B * (Hq >> a.s.lgp) * a.q_tiles);
   a.out = reinterpret_cast<const __nv_bfloat16*>(out);
   a.dout = reinterpret_cast<const __nv_bfloat16*>(dout);
   a.do_batch = strides[9];
   a.do_token = strides[10];
   a.do_head = strides[11];
   a.lse = lse;
-  a.delta = delta;
-  a.ranges = ranges;
   a.dq = reinterpret_cast<__nv_bfloat16*>(dq);
   a.dk = reinterpret_cast<__nv_bfloat16*>(dk);
   a.dv = reinterpret_cast<__nv_bfloat16*>(dv);
-  a.q_tiles = static_cast<int>(attn::q_tiles_of(Sq, a.s.lgp));
-  const int pg = 1 << a.s.lgp, q_rows = attn::kTile >> a.s.lgp, q_step = attn::kBwdTile >> a.s.lgp;
+  const int pg = 1 << a.s.lgp, q_step = attn::kTile >> a.s.lgp;
   const int64_t key_tiles = (Sk + attn::kTile - 1) / attn::kTile;
   if (key_tiles * B * Hkv > (int64_t(1) << 30)) return set_error(FL_ERR_ARG, "fl_attn_bwd: too many key tiles");
 
-  // Resident (128 rows) and streamed (64 rows) maps of each tensor.
-  CUtensorMap q_res, do_res, k_res, v_res, q_str, do_str, k_str, v_str;
+  CUtensorMap mq, mk, mv, mdo;
   const int b = (int)B, sq = (int)Sq, sk = (int)Sk;
-  auto rows_map = [&](CUtensorMap* m, const void* p, const int64_t* s, int tokens) {
-    return attn_map(m, p, s[0], s[1], s[2], b, sq, Hq, D, pg, tokens);
-  };
-  auto keys_map = [&](CUtensorMap* m, const void* p, const int64_t* s, int tokens) {
-    return attn_map(m, p, s[0], s[1], s[2], b, sk, Hkv, D, 1, tokens);
-  };
-  if ((rc = rows_map(&q_res, q, strides, q_rows)) || (rc = rows_map(&do_res, dout, strides + 9, q_rows)) ||
-      (rc = rows_map(&q_str, q, strides, q_step)) || (rc = rows_map(&do_str, dout, strides + 9, q_step)) ||
-      (rc = keys_map(&k_res, k, strides + 3, attn::kTile)) || (rc = keys_map(&v_res, v, strides + 6, attn::kTile)) ||
-      (rc = keys_map(&k_str, k, strides + 3, attn::kBwdTile)) || (rc = keys_map(&v_str, v, strides + 6, attn::kBwdTile)))
+  if ((rc = attn_map(&mq, q, strides[0], strides[1], strides[2], b, sq, Hq, D, pg, q_step)) ||
+      (rc = attn_map(&mk, k, strides[3], strides[4], strides[5], b, sk, Hkv, D, 1, attn::kTile)) ||
+      (rc = attn_map(&mv, v, strides[6], strides[7], strides[8], b, sk, Hkv, D, 1, attn::kTile)) ||
+      (rc = attn_map(&mdo, dout, strides[9], strides[10], strides[11], b, sq, Hq, D, pg, q_step)))
     return rc;
   const bool bias = softcap != 0.f || slopes;
   const int64_t q_grid = attn::fwd_ctas(b, sq, Hq, Hkv);
   a.tiles = static_cast<int>(q_grid / B / (Hq >> a.s.lgp));
-  rc = D <= 64 ? (bias ? attn::launch_bwd<64, true, true>(q_res, do_res, k_str, v_str, a, q_grid, st)
-                       : attn::launch_bwd<64, true, false>(q_res, do_res, k_str, v_str, a, q_grid, st))
-               : (bias ? attn::launch_bwd<128, true, true>(q_res, do_res, k_str, v_str, a, q_grid, st)
-                       : attn::launch_bwd<128, true, false>(q_res, do_res, k_str, v_str, a, q_grid, st));
+  rc = D <= 64 ? (bias ? attn::launch_bwd<64, true, true>(mq, mdo, mk, mv, a, q_grid, st)
+                       : attn::launch_bwd<64, true, false>(mq, mdo, mk, mv, a, q_grid, st))
+               : (bias ? attn::launch_bwd<128, true, true>(mq, mdo, mk, mv, a, q_grid, st)
+                       : attn::launch_bwd<128, true, false>(mq, mdo, mk, mv, a, q_grid, st));
   if (rc) return rc;
   a.tiles = static_cast<int>(key_tiles);
   const int64_t kv_grid = key_tiles * B * Hkv;
-  rc = D <= 64 ? (bias ? attn::launch_bwd<64, false, true>(k_res, v_res, q_str, do_str, a, kv_grid, st)
-                       : attn::launch_bwd<64, false, false>(k_res, v_res, q_str, do_str, a, kv_grid, st))
-               : (bias ? attn::launch_bwd<128, false, true>(k_res, v_res, q_str, do_str, a, kv_grid, st)
-                       : attn::launch_bwd<128, false, false>(k_res, v_res, q_str, do_str, a, kv_grid, st));
+  rc = D <= 64 ? (bias ? attn::launch_bwd<64, false, true>(mk, mv, mq, mdo, a, kv_grid, st)
+                       : attn::launch_bwd<64, false, false>(mk, mv, mq, mdo, a, kv_grid, st))
+               : (bias ? attn::launch_bwd<128, false, true>(mk, mv, mq, mdo, a, kv_grid, st)
+                       : attn::launch_bwd<128, false, false>(mk, mv, mq, mdo, a, kv_grid, st));
   if (rc) return rc;
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(FL_ERR_CUDA, "fl_attn_bwd: %s", cudaGetErrorString(e));

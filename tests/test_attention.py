@@ -8,6 +8,7 @@ distance), and moves p by a factor 1 + e.  So
   |out - o|  <= h |o| + (h + 2 e) sum p |v|
   |dv|:         h |dv| + (h + 2 e) sum p |do|
   |ds|:         (h + 4 e) |ds| + p (sum_d |do| (2 h + 2 e) sum p |v| + 2^-18 sum |do v|)
+                (under a cap 2^-11 |ds| more: its factor 1 - tanh^2 waits in fp16, half a step of that)
   |dq|:         h |dq| + scale sum |ds error| |k|, dk alike."""
 import pytest
 import torch
@@ -71,7 +72,7 @@ def _oracle(q, k, v, begin, end, scale, cap, slopes, do=None):
     ds = p * (dp - (do * o).sum(-1, keepdim=True))
     es = p * ((do.abs() * ((2 * HALF + 2 * e) * reach)).sum(-1, keepdim=True) + 2.0 ** -18 * (do.abs() @ v.abs().mT))
     if cap:
-        es = es + 2.0 ** -18 * ds.abs()
+        es = es + (2.0 ** -18 + 2.0 ** -11 * (1 - th * th)) * ds.abs()
         ds = ds * (1 - th * th)
     es = es + (HALF + 4 * e) * ds.abs()
     fold = lambda a: a.unflatten(1, (K, G)).sum(2)  # noqa: E731
