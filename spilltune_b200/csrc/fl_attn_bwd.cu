@@ -363,6 +363,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         h_first = kvh * G + (i / per_group) * pg;
         whole = cols.max_lo[group] <= row0 && cols.min_hi[group] >= row0 + kTile;
       }
+      [[maybe_unused]] uint64_t nl_of[kDq ? 1 : kCols / 2];   // dk, dv: -lse2 of the columns
+      if constexpr (!kDq && !kBias) {
+#pragma unroll
+        for (int c = 0; c < kCols; c += 4) {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(cols.nlse2 + mine0 + c);
+          nl_of[c / 2] = v.x, nl_of[c / 2 + 1] = v.y;
+        }
+      }
       if (!mbar_wait_short_warp(&bars->s_full, i & 1, abort_word, a.status, kStatusTimeoutAccum)) {
         ok = false;
         break;
@@ -391,9 +399,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         uint64_t nl[2];                            // -lse2 of the columns
         if constexpr (kDq) {
           nl[0] = nl[1] = pair(-lse2, -lse2);
-        } else {
+        } else if constexpr (kBias) {
           const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(cols.nlse2 + mine0 + c);
           nl[0] = v.x, nl[1] = v.y;
+        } else {
+          nl[0] = nl_of[c / 2], nl[1] = nl_of[c / 2 + 1];
         }
         float p[4];
         [[maybe_unused]] float f[4];
