@@ -340,7 +340,7 @@ int fl_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const i
                 int64_t Sk, int Hq, int Hkv, int D, const int32_t* begin, const int32_t* end, float scale,
                 float softcap, const float* slopes, uint16_t* out, float* lse, void* workspace,
                 size_t workspace_bytes, void* stream);
-size_t fl_attn_bwd_workspace_bytes(int64_t B, int64_t Sq, int Hq, int Hkv);
+size_t fl_attn_bwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D);
 int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* strides,
                 const uint16_t* out, const float* lse, int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D,
                 const int32_t* begin, const int32_t* end, float scale, float softcap, const float* slopes,

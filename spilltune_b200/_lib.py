@@ -56,7 +56,7 @@ SIGNATURES = {
     "fl_attn_fwd_workspace_bytes": ([_I64, _I64, _I64, _INT, _INT, _INT], _SZ),
     "fl_attn_fwd": ([_P, _P, _P, _P, _I64, _I64, _I64, _INT, _INT, _INT, _P, _P, _F, _F, _P, _P, _P, _P, _SZ, _P],
                     _INT),
-    "fl_attn_bwd_workspace_bytes": ([_I64, _I64, _INT, _INT], _SZ),
+    "fl_attn_bwd_workspace_bytes": ([_I64, _I64, _I64, _INT, _INT, _INT], _SZ),
     "fl_attn_bwd": ([_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _INT, _INT, _INT, _P, _P, _F, _F, _P, _P, _P, _P,
                      _P, _SZ, _P], _INT),
     "fl_grouped_workspace_bytes": ([_I64, _INT, _I64, _I64, _INT], _SZ),

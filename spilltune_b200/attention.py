@@ -85,16 +85,18 @@ def _view(x):
 
 def _check(q, k, v, begin, end, scale, softcap, slopes):
     _need_cuda(q, k, v, begin, end, slopes)
+    bf16 = torch.bfloat16
     for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4 or t.dtype != torch.bfloat16:
+        if t.dim() != 4 or t.dtype != bf16:
             raise ValueError(f"{name} must be bf16 [batch, tokens, heads, head size]")
     dev = q.device
-    for t in (k, v, begin, end, slopes):
-        if t is not None and t.device != dev:
-            raise ValueError("attention arguments must be on one device")
+    if k.device != dev or v.device != dev or begin.device != dev or end.device != dev or \
+            slopes is not None and slopes.device != dev:
+        raise ValueError("attention arguments must be on one device")
     B, Sq, Hq, D = q.shape
-    Sk, Hkv = k.shape[1], k.shape[2]
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+    ks = k.shape
+    Sk, Hkv = ks[1], ks[2]
+    if ks != v.shape or ks[0] != B or ks[3] != D:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
     if Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise ValueError(f"{Hq} query heads do not share {Hkv} key/value heads evenly")
@@ -111,15 +113,11 @@ def _check(q, k, v, begin, end, scale, softcap, slopes):
     softcap = float(softcap or 0.0)
     if not (softcap >= 0 and math.isfinite(softcap)):
         raise ValueError("softcap must be >= 0 and finite")
-    return B, Sq, Sk, Hq, Hkv, D, scale, softcap
+    return dev, B, Sq, Sk, Hq, Hkv, D, scale, softcap
 
 
-def _strides(*tensors):
-    return (ctypes.c_int64 * (3 * len(tensors)))(*(s for t in tensors for s in t.stride()[:3]))
-
-
-def _contiguous(t):
-    return None if t is None else t.contiguous()
+_Strides3 = ctypes.c_int64 * 9
+_Strides4 = ctypes.c_int64 * 12
 
 
 def fwd(q, k, v, begin, end, *, scale=None, softcap=0.0, slopes=None):
@@ -131,46 +129,52 @@ def fwd(q, k, v, begin, end, *, scale=None, softcap=0.0, slopes=None):
     query that sees none gets 0 and a log sum of -inf.
     scale: of q . k, default D ** -0.5.  softcap > 0: softcap * tanh(x / softcap).
     slopes: fp32 [Hq]; x -= slopes[h] * |i + Sk - Sq - j|."""
-    B, Sq, Sk, Hq, Hkv, D, scale, softcap = _check(q, k, v, begin, end, scale, softcap, slopes)
-    out = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=q.device)
-    lse = torch.empty((B, Sq, Hq), dtype=torch.float32, device=q.device)
+    dev, B, Sq, Sk, Hq, Hkv, D, scale, softcap = _check(q, k, v, begin, end, scale, softcap, slopes)
+    out = q.new_empty((B, Sq, Hq, D))
+    lse = q.new_empty((B, Sq, Hq), dtype=torch.float32)
     if out.numel() == 0:
         return out, lse
     q, k, v = _view(q), _view(k), _view(v)
-    begin, end, slopes = begin.contiguous(), end.contiguous(), _contiguous(slopes)
-    with on_device(q):
+    begin, end = begin.contiguous(), end.contiguous()
+    if slopes is not None:
+        slopes = slopes.contiguous()
+    with on_device(dev):
         n = _lib.load().fl_attn_fwd_workspace_bytes(B, Sq, Sk, Hq, Hkv, D)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        _lib.call("fl_attn_fwd", _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v), B, Sq, Sk, Hq, Hkv, D, _ptr(begin),
-                  _ptr(end), scale, softcap, _ptr(slopes), _ptr(out), _ptr(lse), _ptr(ws), n, stream_of(q))
+        ws = q.new_empty(n, dtype=torch.uint8) if n else None
+        _lib.call("fl_attn_fwd", _ptr(q), _ptr(k), _ptr(v),
+                  _Strides3(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), B, Sq, Sk, Hq, Hkv, D, _ptr(begin),
+                  _ptr(end), scale, softcap, _ptr(slopes), _ptr(out), _ptr(lse), _ptr(ws), n, stream_of(dev))
     return out, lse
 
 
 def bwd(dout, q, k, v, out, lse, begin, end, *, scale=None, softcap=0.0, slopes=None):
     """(dq, dk, dv) of fwd(): bf16, contiguous; dk and dv summed over the query
     heads that share them, in a fixed order.  out and lse: what fwd() returned."""
-    B, Sq, Sk, Hq, Hkv, D, scale, softcap = _check(q, k, v, begin, end, scale, softcap, slopes)
+    dev, B, Sq, Sk, Hq, Hkv, D, scale, softcap = _check(q, k, v, begin, end, scale, softcap, slopes)
     _need_cuda(dout, out, lse)
     if dout.shape != q.shape or out.shape != q.shape or dout.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
         raise ValueError("dout and out must be bf16 of q's shape")
     if lse.shape != (B, Sq, Hq) or lse.dtype != torch.float32:
         raise ValueError("lse must be fp32 [batch, query tokens, query heads]")
-    if any(t.device != q.device for t in (dout, out, lse)):
+    if dout.device != dev or out.device != dev or lse.device != dev:
         raise ValueError("attention arguments must be on one device")
-    dq = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=q.device)
-    dk = torch.empty((B, Sk, Hkv, D), dtype=torch.bfloat16, device=q.device)
-    dv = torch.empty_like(dk)
+    dq = q.new_empty((B, Sq, Hq, D))
+    dk = q.new_empty((B, Sk, Hkv, D))
+    dv = q.new_empty((B, Sk, Hkv, D))
     if dq.numel() + dk.numel() == 0:
         return dq, dk, dv
     q, k, v, dout = _view(q), _view(k), _view(v), _view(dout)
     out, lse = out.contiguous(), lse.contiguous()
-    begin, end, slopes = begin.contiguous(), end.contiguous(), _contiguous(slopes)
-    with on_device(q):
-        n = _lib.load().fl_attn_bwd_workspace_bytes(B, Sq, Hq, Hkv)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        _lib.call("fl_attn_bwd", _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _strides(q, k, v, dout), _ptr(out), _ptr(lse),
-                  B, Sq, Sk, Hq, Hkv, D, _ptr(begin), _ptr(end), scale, softcap, _ptr(slopes), _ptr(dq), _ptr(dk),
-                  _ptr(dv), _ptr(ws), n, stream_of(q))
+    begin, end = begin.contiguous(), end.contiguous()
+    if slopes is not None:
+        slopes = slopes.contiguous()
+    with on_device(dev):
+        n = _lib.load().fl_attn_bwd_workspace_bytes(B, Sq, Sk, Hq, Hkv, D)
+        ws = q.new_empty(n, dtype=torch.uint8) if n else None
+        _lib.call("fl_attn_bwd", _ptr(dout), _ptr(q), _ptr(k), _ptr(v),
+                  _Strides4(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *dout.stride()[:3]), _ptr(out),
+                  _ptr(lse), B, Sq, Sk, Hq, Hkv, D, _ptr(begin), _ptr(end), scale, softcap, _ptr(slopes), _ptr(dq),
+                  _ptr(dk), _ptr(dv), _ptr(ws), n, stream_of(dev))
     return dq, dk, dv
 
 

@@ -81,6 +81,8 @@ struct BwdArgs {
   uint32_t* status;
   int q_tiles;           // of kTile packed rows
   int tiles;             // resident tiles per head
+  int parts;             // dk, dv: CTAs that share a tile's walk
+  float* part;           // their sums [parts][dv, dk][B, Sk, Hkv, D] (parts > 1)
 };
 
 struct __align__(16) BwdBars {
@@ -128,11 +130,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
   // The heaviest tiles of a causal mask first: early keys, late queries.
   const int heads = kDq ? s.Hkv * s.groups : s.Hkv;
-  const int per = heads * s.B;
+  const int per = heads * s.B * a.parts;
   const int order = static_cast<int>(blockIdx.x) / per;
   const int tile = kDq ? a.tiles - 1 - order : order;
-  const int hg = static_cast<int>(blockIdx.x) % per % heads;
-  const int b = static_cast<int>(blockIdx.x) % per / heads;
+  int rest = static_cast<int>(blockIdx.x) % per;
+  const int hg = rest % heads;
+  rest /= heads;
+  const int b = rest % s.B, part = rest / s.B;
   const int kvh = kDq ? hg / s.groups : hg;
   const int q_step = kTile >> s.lgp;                       // tokens of a query tile
   const int row0 = kDq ? tile * q_step : tile * kTile;
@@ -169,7 +173,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   // query tiles `first` .. `first + per_group - 1` (those between that see none
   // of the keys add nothing).
   Range mine{};
-  int first = 0, n = 0, per_group = 0;
+  int first = 0, n = 0, per_group = 0, from = 0;   // from: this part's first step
   if constexpr (kDq) {
     mine = tile_range(s, b, row0, q_step);
     if (mine.min_lo < mine.max_hi) {
@@ -193,7 +197,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     first = bars->first;
     per_group = bars->last >= 0 ? bars->last - first + 1 : 0;
     n = per_group * s.groups;
+    if (a.parts > 1) {
+      from = static_cast<int>(static_cast<int64_t>(n) * part / a.parts);
+      n = static_cast<int>(static_cast<int64_t>(n) * (part + 1) / a.parts) - from;
+    }
   }
+  // Step i of this CTA: the head group and query tile (dk, dv).
+  auto group_of = [&](int i) { return (from + i) / per_group; };
+  auto q_tile_of = [&](int i) { return first + (from + i) % per_group; };
 
   if (warp == 0) {
     if (lane == 0 && n > 0) {
@@ -216,8 +227,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           bh = kvh;
           br = (first + i) * kTile;
         } else {
-          bh = kvh * G + (i / per_group) * pg;
-          br = (first + i % per_group) * q_step;
+          bh = kvh * G + group_of(i) * pg;
+          br = q_tile_of(i) * q_step;
         }
         for (int o = 0; o < 2 && ok; ++o) {
           if (i >= C::kStages && !mbar_wait_short(&bars->b_empty[o][st], (i / C::kStages - 1) & 1, abort_word, a.status,
@@ -229,8 +240,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           mbar_arrive_expect_tx(&bars->b_full[o][st], C::kBytes + (!kDq && o == 0 ? kInfoBytes : 0));
           if (!kDq && o == 0)
             bulk_load(info + st,
-                      a.info + (static_cast<int64_t>(b) * s.Hkv * s.groups + kvh * s.groups + i / per_group) *
-                                   a.q_tiles + first + i % per_group,
+                      a.info + (static_cast<int64_t>(b) * s.Hkv * s.groups + kvh * s.groups + group_of(i)) *
+                                   a.q_tiles + q_tile_of(i),
                       kInfoBytes, &bars->b_full[o][st]);
           for (int c = 0; c < HD / 64; ++c)
             tma_load_4d(dst + c * kTile * 128, o ? &tm_b2 : &tm_b1, 64 * c, bh, br, b, &bars->b_full[o][st]);
@@ -359,8 +370,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         col0 = (first + i) * kTile + mine0;
         whole = mine.max_lo <= col0 && mine.min_hi >= col0 + kCols;
       } else {
-        col0 = (first + i % per_group) * q_step + (mine0 >> s.lgp);
-        h_first = kvh * G + (i / per_group) * pg;
+        col0 = q_tile_of(i) * q_step + (mine0 >> s.lgp);
+        h_first = kvh * G + group_of(i) * pg;
         whole = cols.max_lo[group] <= row0 && cols.min_hi[group] >= row0 + kTile;
       }
       [[maybe_unused]] uint64_t nl_of[kDq ? 1 : kCols / 2];   // dk, dv: -lse2 of the columns
@@ -594,6 +605,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           for (int e = 0; e < 16; ++e) v[e] = 0u;
         }
         if (!live) continue;
+        if (!kDq && a.parts > 1) {
+          const int64_t rows = static_cast<int64_t>(s.B) * s.Sk * s.Hkv;
+          float* f = a.part + ((part * 2 + second) * rows + (static_cast<int64_t>(b) * s.Sk + key) * s.Hkv + kvh) * s.D + c;
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            if (c + e < s.D)
+              *reinterpret_cast<float4*>(f + e) =
+                  make_float4(__uint_as_float(v[e]) * by, __uint_as_float(v[e + 1]) * by,
+                              __uint_as_float(v[e + 2]) * by, __uint_as_float(v[e + 3]) * by);
+          continue;
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           if (c + 8 * e < s.D) {
@@ -616,6 +638,31 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   }
 }
 
+// dv and dk from the parts' sums, in the parts' order.  n4: groups of four
+// columns of one of the two.
+__global__ void __launch_bounds__(256) parts_kernel(const float4* __restrict__ part, int parts, int64_t n4,
+                                                    uint2* __restrict__ dv, uint2* __restrict__ dk) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < 2 * n4;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    float4 sum = part[i];
+    for (int p = 1; p < parts; ++p) {
+      const float4 x = part[2 * n4 * p + i];
+      sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+    }
+    (i < n4 ? dv[i] : dk[i - n4]) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
+  }
+}
+
+// CTAs that share one key tile's walk: none while the key tiles fill half the
+// SMs; else towards one CTA per SM, each keeping four steps of the longest
+// walk (a step is about 2 us, the reduction's launch another).
+int bwd_parts(int64_t key_ctas, int64_t steps) {
+  if (key_ctas > 74) return 1;
+  int64_t n = 148 / key_ctas;
+  if (n > steps / 4) n = steps / 4;
+  return n < 1 ? 1 : static_cast<int>(n);
+}
+
 template <int HD, bool kDq, bool kBias>
 int launch_bwd(const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1, const CUtensorMap& b2,
                const BwdArgs& a, int64_t grid, cudaStream_t stream) {
@@ -634,12 +681,22 @@ using namespace fl;
 
 extern "C" {
 
-// The query tiles' row statistics, then their ranges.
-size_t fl_attn_bwd_workspace_bytes(int64_t B, int64_t Sq, int Hq, int Hkv) {
-  if (B <= 0 || Sq <= 0 || Hq < 1 || Hkv < 1 || Hq % Hkv) return 0;
+// The query tiles' row statistics, then their ranges, then the parts' sums.
+static size_t attn_bwd_sizes(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D, int* parts, size_t* part_at) {
   const int lgp = attn::packed_log2(Hq, Hkv);
-  const size_t tiles = static_cast<size_t>(B) * attn::q_tiles_of(Sq, lgp);
-  return tiles * (Hq >> lgp) * sizeof(attn::RowInfo) + tiles * sizeof(attn::Range);
+  const int64_t q_tiles = attn::q_tiles_of(Sq, lgp), key_tiles = (Sk + attn::kTile - 1) / attn::kTile;
+  *parts = attn::bwd_parts(key_tiles * B * Hkv, q_tiles * ((Hq / Hkv) >> lgp));
+  *part_at = static_cast<size_t>(B) * q_tiles * ((Hq >> lgp) * sizeof(attn::RowInfo) + sizeof(attn::Range));
+  return *part_at + (*parts > 1 ? static_cast<size_t>(*parts) * 2 * B * Sk * Hkv * D * sizeof(float) : 0);
+}
+
+size_t fl_attn_bwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D) {
+  if (B <= 0 || Sq <= 0 || Sk <= 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || D < 8 || B > (1 << 16) || Sq > (1 << 30) ||
+      Sk > (1 << 30))
+    return 0;
+  int parts;
+  size_t part_at;
+  return attn_bwd_sizes(B, Sq, Sk, Hq, Hkv, D, &parts, &part_at);
 }
 
 int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, const uint16_t* v, const int64_t* strides,
@@ -665,8 +722,10 @@ int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, cons
       return set_error(FL_ERR_CUDA, "fl_attn_bwd: clearing dq failed");
     return FL_OK;
   }
-  if (!workspace || workspace_bytes < fl_attn_bwd_workspace_bytes(B, Sq, Hq, Hkv) ||
-      (reinterpret_cast<uintptr_t>(workspace) & 15u))
+  int parts;
+  size_t part_at;
+  const size_t need = attn_bwd_sizes(B, Sq, Sk, Hq, Hkv, D, &parts, &part_at);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u))
     return set_error(FL_ERR_ARG, "fl_attn_bwd: workspace missing, short or not 16-byte aligned");
   attn::BwdArgs a{};
   attn::fill_shape(a.s, (int)B, (int)Sq, (int)Sk, Hq, Hkv, D, begin, end, scale, softcap, slopes);
@@ -698,6 +757,7 @@ int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, cons
     return rc;
   const bool bias = softcap != 0.f || slopes;
   const int64_t q_grid = attn::fwd_ctas(b, sq, Hq, Hkv);
+  a.parts = 1;
   a.tiles = static_cast<int>(q_grid / B / (Hq >> a.s.lgp));
   rc = D <= 64 ? (bias ? attn::launch_bwd<64, true, true>(mq, mdo, mk, mv, a, q_grid, st)
                        : attn::launch_bwd<64, true, false>(mq, mdo, mk, mv, a, q_grid, st))
@@ -705,12 +765,20 @@ int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, cons
                        : attn::launch_bwd<128, true, false>(mq, mdo, mk, mv, a, q_grid, st));
   if (rc) return rc;
   a.tiles = static_cast<int>(key_tiles);
-  const int64_t kv_grid = key_tiles * B * Hkv;
+  a.parts = parts;
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + part_at);
+  const int64_t kv_grid = key_tiles * B * Hkv * parts;
   rc = D <= 64 ? (bias ? attn::launch_bwd<64, false, true>(mk, mv, mq, mdo, a, kv_grid, st)
                        : attn::launch_bwd<64, false, false>(mk, mv, mq, mdo, a, kv_grid, st))
                : (bias ? attn::launch_bwd<128, false, true>(mk, mv, mq, mdo, a, kv_grid, st)
                        : attn::launch_bwd<128, false, false>(mk, mv, mq, mdo, a, kv_grid, st));
   if (rc) return rc;
+  if (parts > 1) {
+    const int64_t n4 = B * Sk * Hkv * D / 4;
+    const int64_t blocks = (2 * n4 + 255) / 256;
+    attn::parts_kernel<<<static_cast<unsigned>(blocks < 2368 ? blocks : 2368), 256, 0, st>>>(
+        reinterpret_cast<const float4*>(a.part), parts, n4, reinterpret_cast<uint2*>(dv), reinterpret_cast<uint2*>(dk));
+  }
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(FL_ERR_CUDA, "fl_attn_bwd: %s", cudaGetErrorString(e));
   return FL_OK;

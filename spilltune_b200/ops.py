@@ -36,16 +36,18 @@ def _ptr(t):
 
 
 _SAME_DEVICE = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
-def on_device(t):
-    """Context in which t's device is the current one (none is entered when it is already)."""
-    return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def on_device(device):
+    """Context in which `device` is the current one (none is entered when it is already)."""
+    return _SAME_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
-def stream_of(t):
-    """The current stream of t's device."""
-    return torch.cuda.current_stream(t.device).cuda_stream
+def stream_of(device):
+    """Handle of the current stream of `device`.  The raw query is what torch's own generated
+    code calls; building a Stream object around it takes 2 us, a tenth of a small call."""
+    return _raw_stream(device.index) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
 
 
 def dequant(weight: PackedWeight, out=None):

@@ -90,76 +90,76 @@ def frequencies(dim, theta=10000.0, scaling=None):
 
 
 def _rows(x, what):
-    """x [..., heads, D] as (tensor, tokens, token stride, head stride): no copy
-    where the leading dimensions have one stride between tokens."""
-    if x.dim() < 3:
-        raise ValueError(f"{what} must be [..., heads, head size]")
+    """x [..., heads, D] as (tensor, token stride, head stride): no copy where
+    the leading dimensions have one stride between tokens."""
     if x.dtype != torch.bfloat16:
         raise ValueError(f"{what} must be bf16")
-    tokens = 1
-    for n in x.shape[:-2]:
-        tokens *= n
-    if x.dim() == 3 and (x.stride(-1) == 1 or x.shape[-1] == 1):
-        return x, tokens, x.stride(0), x.stride(1)
-    step, reach, even = None, 1, x.stride(-1) == 1
-    for n, s in zip(reversed(x.shape[:-2]), reversed(x.stride()[:-2])):
+    shape, stride = x.shape, x.stride()
+    if len(shape) == 3 and (stride[2] == 1 or shape[2] == 1):
+        return x, stride[0], stride[1]
+    step, reach, even = 0, 1, stride[-1] == 1
+    for n, s in zip(reversed(shape[:-2]), reversed(stride[:-2])):
         if n == 1:
             continue
-        if step is None:
+        if reach == 1:
             step = s
         even = even and s == step * reach
         reach *= n
     if not even:
         x = x.contiguous()
-        return x, tokens, x.shape[-2] * x.shape[-1], x.shape[-1]
-    return x, tokens, step or 0, x.stride(-2)
+        return x, shape[-2] * shape[-1], shape[-1]
+    return x, step, stride[-2]
 
 
 def _setup(q, k, positions, inv_freq, q_weight, k_weight, eps):
-    """Argument checks shared by both passes; returns the call's common values."""
+    """Argument checks of both passes and what they share: (tokens, key heads,
+    positions, position bytes, inv_freq, rotated columns, weights, weight bytes, eps)."""
     _need_cuda(q, k, positions, inv_freq, q_weight, k_weight)
-    dev = q.device
-    for t in (k, positions, inv_freq, q_weight, k_weight):
-        if t is not None and t.device != dev:
-            raise ValueError("rotary arguments must be on one device")
-    if q.dim() < 3:
+    dev, shape = q.device, q.shape
+    if len(shape) < 3:
         raise ValueError("q must be [..., heads, head size]")
-    D, lead = q.shape[-1], q.shape[:-2]
-    if k is not None and (k.dim() != q.dim() or k.shape[-1] != D or k.shape[:-2] != lead):
-        raise ValueError("q and k must agree in their leading dimensions and head size")
-    if positions.dtype not in _INTS:
+    D, lead = shape[-1], shape[:-2]
+    kh = 0
+    if k is not None:
+        ks = k.shape
+        if len(ks) != len(shape) or ks[-1] != D or ks[:-2] != lead:
+            raise ValueError("q and k must agree in their leading dimensions and head size")
+        kh = ks[-2]
+    pbytes = _INTS.get(positions.dtype)
+    if pbytes is None:
         raise ValueError("positions must be int32 or int64")
     if positions.shape != lead:
         try:
             positions = positions.expand(lead)
         except RuntimeError:
             raise ValueError(f"positions {tuple(positions.shape)} do not fit the tokens {tuple(lead)}") from None
-    positions = positions.contiguous()
     if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
         raise ValueError("inv_freq must be fp32 [rotated columns / 2]")
-    inv_freq = inv_freq.contiguous()
     rot = 2 * inv_freq.shape[0]
     if rot < 2 or rot > D:
         raise ValueError(f"{rot} rotated columns do not fit a head of {D}")
     if D > MAX_HEAD_DIM:
         raise ValueError(f"unsupported_capability: head size {D} > {MAX_HEAD_DIM}")
+    if (k is not None and k.device != dev) or positions.device != dev or inv_freq.device != dev:
+        raise ValueError("rotary arguments must be on one device")
     wbytes = 0
-    if (q_weight is None) != (k_weight is None) and k is not None:
-        raise ValueError("give both norm weights or neither")
-    if q_weight is not None:
+    if q_weight is not None or k_weight is not None:
+        if q_weight is None or (k_weight is None and k is not None):
+            raise ValueError("give both norm weights or neither")
         for w in (q_weight, k_weight):
-            if w is not None and (w.shape != (D,) or w.dtype not in _WEIGHTS or w.dtype != q_weight.dtype):
+            if w is None:
+                continue
+            if w.shape != (D,) or w.dtype not in _WEIGHTS or w.dtype != q_weight.dtype:
                 raise ValueError("norm weights must be bf16 or fp32 [head size], of one type")
+            if w.device != dev:
+                raise ValueError("rotary arguments must be on one device")
         if eps is None or not eps >= 0:
             raise ValueError("a norm needs eps >= 0")
         wbytes = _WEIGHTS[q_weight.dtype]
         q_weight = q_weight.contiguous()
         k_weight = None if k_weight is None else k_weight.contiguous()
-    return positions, inv_freq, rot, q_weight, k_weight, wbytes, float(eps or 0.0)
-
-
-def _out(shape, like):
-    return torch.empty(shape, dtype=torch.bfloat16, device=like.device)
+    return (math.prod(lead), kh, positions.contiguous(), pbytes, inv_freq.contiguous(), rot, q_weight, k_weight,
+            wbytes, float(eps or 0.0))
 
 
 def fwd(q, k, positions, inv_freq, *, interleaved=False, factor=1.0, q_weight=None, k_weight=None, eps=None):
@@ -170,19 +170,19 @@ def fwd(q, k, positions, inv_freq, *, interleaved=False, factor=1.0, q_weight=No
     positions: int32 or int64, broadcastable to the leading dimensions.
     interleaved: columns (2p, 2p + 1) pair up, not (p, p + rot / 2).
     factor: multiplies cosine and sine (see ``frequencies``)."""
-    positions, inv_freq, rot, q_weight, k_weight, wbytes, eps = _setup(q, k, positions, inv_freq, q_weight, k_weight,
-                                                                       eps)
-    qr, T, qt, qh = _rows(q, "q")
-    kr, _, kt, kh = _rows(k, "k") if k is not None else (None, T, 0, 0)
-    yq = _out(q.shape, q)
-    yk = _out(k.shape, k) if k is not None else None
-    Hk = 0 if k is None else k.shape[-2]
-    if q.shape[-2] + Hk == 0 or T == 0:
+    T, Hk, positions, pbytes, inv_freq, rot, q_weight, k_weight, wbytes, eps = _setup(q, k, positions, inv_freq,
+                                                                                      q_weight, k_weight, eps)
+    qr, qt, qh = _rows(q, "q")
+    kr, kt, kh = _rows(k, "k") if k is not None else (None, 0, 0)
+    yq = q.new_empty(q.shape)
+    yk = None if k is None else k.new_empty(k.shape)
+    if T == 0:
         return yq, yk
-    with on_device(q):
+    dev = q.device
+    with on_device(dev):
         _lib.call("fl_rotary_fwd", _ptr(qr), qt, qh, q.shape[-2], _ptr(kr), kt, kh, Hk, T, q.shape[-1],
-                  _ptr(positions), _INTS[positions.dtype], _ptr(inv_freq), rot, int(bool(interleaved)), float(factor),
-                  _ptr(q_weight), _ptr(k_weight), wbytes, eps, _ptr(yq), _ptr(yk), stream_of(q))
+                  _ptr(positions), pbytes, _ptr(inv_freq), rot, int(bool(interleaved)), factor, _ptr(q_weight),
+                  _ptr(k_weight), wbytes, eps, _ptr(yq), _ptr(yk), stream_of(dev))
     return yq, yk
 
 
@@ -192,41 +192,41 @@ def bwd(dq, dk, q, k, positions, inv_freq, *, interleaved=False, factor=1.0, q_w
     q and k are the forward's inputs, read only with a norm; dq and dk may be
     any views.  Weight gradients (fp32 [D], summed in a fixed order) are formed
     with weight_grads=True, else None."""
-    if k is None and dk is not None or k is not None and dk is None:
+    if (k is None) != (dk is None):
         raise ValueError("dk goes with k")
-    positions, inv_freq, rot, q_weight, k_weight, wbytes, eps = _setup(q, k, positions, inv_freq, q_weight, k_weight,
-                                                                       eps)
+    T, Hk, positions, pbytes, inv_freq, rot, q_weight, k_weight, wbytes, eps = _setup(q, k, positions, inv_freq,
+                                                                                      q_weight, k_weight, eps)
     _need_cuda(dq, dk)
     if dq.shape != q.shape or k is not None and dk.shape != k.shape:
         raise ValueError("dq and dk must have the shapes of q and k")
-    if dq.device != q.device or dk is not None and dk.device != q.device:
+    dev = q.device
+    if dq.device != dev or dk is not None and dk.device != dev:
         raise ValueError("rotary arguments must be on one device")
     if weight_grads and not wbytes:
         raise ValueError("weight gradients need the norm weights")
-    dqr, T, dqt, dqh = _rows(dq, "dq")
-    dkr, _, dkt, dkh = _rows(dk, "dk") if k is not None else (None, T, 0, 0)
+    dqr, dqt, dqh = _rows(dq, "dq")
+    dkr, dkt, dkh = _rows(dk, "dk") if k is not None else (None, 0, 0)
     qr, qt, qh, kr, kt, kh = None, 0, 0, None, 0, 0
     if wbytes:
-        qr, _, qt, qh = _rows(q, "q")
+        qr, qt, qh = _rows(q, "q")
         if k is not None:
-            kr, _, kt, kh = _rows(k, "k")
-    D, Hk = q.shape[-1], 0 if k is None else k.shape[-2]
-    gq = _out(q.shape, q)
-    gk = _out(k.shape, k) if k is not None else None
+            kr, kt, kh = _rows(k, "k")
+    D = q.shape[-1]
+    gq = q.new_empty(q.shape)
+    gk = None if k is None else k.new_empty(k.shape)
     gqw = gkw = ws = None
     nbytes = 0
     if weight_grads:
-        gqw = torch.zeros(D, dtype=torch.float32, device=q.device) if T == 0 else \
-            torch.empty(D, dtype=torch.float32, device=q.device)
-        gkw = None if k is None else torch.empty_like(gqw) if T else torch.zeros_like(gqw)
+        gqw = q.new_zeros(D, dtype=torch.float32) if T == 0 else q.new_empty(D, dtype=torch.float32)
+        gkw = None if k is None else gqw.new_zeros(D) if T == 0 else gqw.new_empty(D)
         nbytes = _lib.load().fl_rotary_bwd_workspace_bytes(D)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(nbytes, dtype=torch.uint8)
     if T:
-        with on_device(q):
+        with on_device(dev):
             _lib.call("fl_rotary_bwd", _ptr(dqr), dqt, dqh, _ptr(dkr), dkt, dkh, _ptr(qr), qt, qh, q.shape[-2],
-                      _ptr(kr), kt, kh, Hk, T, D, _ptr(positions), _INTS[positions.dtype], _ptr(inv_freq), rot,
-                      int(bool(interleaved)), float(factor), _ptr(q_weight), _ptr(k_weight), wbytes, eps, _ptr(gq),
-                      _ptr(gk), _ptr(gqw), _ptr(gkw), _ptr(ws), nbytes, stream_of(q))
+                      _ptr(kr), kt, kh, Hk, T, D, _ptr(positions), pbytes, _ptr(inv_freq), rot,
+                      int(bool(interleaved)), factor, _ptr(q_weight), _ptr(k_weight), wbytes, eps, _ptr(gq), _ptr(gk),
+                      _ptr(gqw), _ptr(gkw), _ptr(ws), nbytes, stream_of(dev))
     return gq, gk, gqw, gkw
 
 
