@@ -344,33 +344,39 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
 }
 
 // Joins the splits of a row: weights 2^(lse_s - max) over their sum, splits in
-// order.  16 lanes to a row, 8 columns to a lane.
-__global__ void join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse, int splits,
-                            int64_t rows, int D, __nv_bfloat16* __restrict__ out, float* __restrict__ lse) {
+// order.  16 lanes to a row, 8 columns to a lane; the lanes share the log sums.
+__global__ void __launch_bounds__(128) join_kernel(const float* __restrict__ part_o,
+                                                   const float* __restrict__ part_lse, int splits, int64_t rows, int D,
+                                                   __nv_bfloat16* __restrict__ out, float* __restrict__ lse) {
   const int64_t row = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
-  const int d = (threadIdx.x & 15) * 8;
+  const int sub = threadIdx.x & 15, d = sub * 8;
+  griddep_wait();
+  const int64_t at = row < rows ? row : rows - 1;
+  float top = -INFINITY, sum = 0.f;
+  for (int i = sub; i < splits; i += 16) top = fmaxf(top, part_lse[i * rows + at]);
+#pragma unroll
+  for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float base = top == -INFINITY ? 0.f : top;
+  for (int i = sub; i < splits; i += 16) sum += ex2((part_lse[i * rows + at] - base) * kLog2e);
+#pragma unroll
+  for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (row >= rows) return;
-  float top = -INFINITY;
-  for (int i = 0; i < splits; ++i) top = fmaxf(top, part_lse[i * rows + row]);
-  float sum = 0.f, o[8] = {};
-  if (top != -INFINITY) {
+  float o[8] = {};
+  if (d < D) {
+#pragma unroll 4
     for (int i = 0; i < splits; ++i) {
-      const float w = ex2((part_lse[i * rows + row] - top) * kLog2e);
-      sum += w;
-      if (d < D && w != 0.f) {
-        const float4* p = reinterpret_cast<const float4*>(part_o + (i * rows + row) * D + d);
-        const float4 x = p[0], y = p[1];
-        o[0] += w * x.x, o[1] += w * x.y, o[2] += w * x.z, o[3] += w * x.w;
-        o[4] += w * y.x, o[5] += w * y.y, o[6] += w * y.z, o[7] += w * y.w;
-      }
+      const float4* p = reinterpret_cast<const float4*>(part_o + (i * rows + row) * D + d);
+      const float4 x = p[0], y = p[1];
+      const float w = ex2((part_lse[i * rows + row] - base) * kLog2e);
+      o[0] += w * x.x, o[1] += w * x.y, o[2] += w * x.z, o[3] += w * x.w;
+      o[4] += w * y.x, o[5] += w * y.y, o[6] += w * y.z, o[7] += w * y.w;
     }
-  }
-  const float inv = sum > 0.f ? 1.0f / sum : sum == 0.f ? 0.f : sum;
-  if (d < D)
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     *reinterpret_cast<uint4*>(out + row * D + d) =
         make_uint4(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
                    pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
-  if (d == 0) lse[row] = sum == 0.f ? -INFINITY : top + log2f(sum) * kLn2;
+  }
+  if (sub == 0) lse[row] = sum == 0.f ? -INFINITY : top + log2f(sum) * kLn2;
 }
 
 // Splits of the key tiles: none while the row tiles fill half the SMs; else
@@ -543,9 +549,21 @@ int fl_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const i
                : (bias ? attn::launch_fwd<128, true>(mq, mk, mv, a, grid, st)
                        : attn::launch_fwd<128, false>(mq, mk, mv, a, grid, st));
   if (rc) return rc;
-  if (a.splits > 1)
-    attn::join_kernel<<<static_cast<unsigned>((rows * 16 + 127) / 128), 128, 0, st>>>(a.part_o, a.part_lse, a.splits,
-                                                                                     rows, D, a.out, lse);
+  if (a.splits > 1) {
+    // A programmatic dependent: its launch overlaps the attention kernel, whose results it waits for.
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>((rows * 16 + 127) / 128));
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t le = cudaLaunchKernelEx(&cfg, attn::join_kernel, static_cast<const float*>(a.part_o),
+                                              static_cast<const float*>(a.part_lse), a.splits, rows, D, a.out, lse);
+    if (le != cudaSuccess) return set_error(FL_ERR_CUDA, "fl_attn_fwd: %s", cudaGetErrorString(le));
+  }
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(FL_ERR_CUDA, "fl_attn_fwd: %s", cudaGetErrorString(e));
   return FL_OK;

@@ -89,34 +89,6 @@ __device__ __forceinline__ float rcp(float x) {
   return y;
 }
 
-// Two FP32 values to a 64-bit register: one instruction works on both.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-  return d;
-}
-__device__ __forceinline__ void unpair(uint64_t d, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(d));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
-  return static_cast<uint64_t>(hi) << 32 | lo;
-}
-
 // 2^x of two values without the special-function unit, whose 16 results a
 // cycle and SM bound the exponentials: x = i + f with i the nearest integer
 // (by adding 1.5 * 2^23), 2^f on [-1/2, 1/2] by the polynomial of degree 5 with

@@ -54,6 +54,7 @@ struct Args {
   const float* inv;
   float factor, eps;
   int tokens;                      // tokens per block
+  unsigned heads_magic;            // ceil(2^32 / heads), 0 for one head: row / heads for a block's rows
   int lanes_log2;                  // lanes per head (vector form)
   float* dw_part;                  // [gridDim.x][2][D]
 };
@@ -73,77 +74,149 @@ __device__ __forceinline__ float weight_at(const Args& a, int which, int d) {
   return a.w16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(w)[d]) : static_cast<const float*>(w)[d];
 }
 
-__device__ __forceinline__ void unpack8(const uint4& v, float* f) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-  }
-}
-__device__ __forceinline__ uint4 pack8(const float* f) {
-  return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                    pack_bf16x2(f[6], f[7]));
-}
-
 // Streamed once: keep the lines out of L1.
 __device__ __forceinline__ uint4 load_stream(const __nv_bfloat16* p) {
   return __ldcs(reinterpret_cast<const uint4*>(p));
 }
 
+// Eight columns as four pairs of FP32 values; one instruction works on a pair.
+struct V8 {
+  uint64_t p[4];
+};
+__device__ __forceinline__ V8 unpack(const uint4& v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  V8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.p[i] = pair(w[i] << 16, w[i] & 0xFFFF0000u);
+  return r;
+}
+__device__ __forceinline__ uint4 pack(const V8& v) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float lo, hi;
+    unpair(v.p[i], lo, hi);
+    w[i] = pack_bf16x2(lo, hi);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ V8 mul(const V8& a, const V8& b) {
+  V8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.p[i] = mul2(a.p[i], b.p[i]);
+  return r;
+}
+__device__ __forceinline__ void scale(V8& a, float s) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a.p[i] = mul2(a.p[i], pair(s, s));
+}
+__device__ __forceinline__ float dot(const V8& a0, const V8& b0, const V8& a1, const V8& b1) {
+  uint64_t s = mul2(a0.p[0], b0.p[0]), t = mul2(a1.p[0], b1.p[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    s = fma2(a0.p[i], b0.p[i], s);
+    t = fma2(a1.p[i], b1.p[i], t);
+  }
+  float lo, hi;
+  unpair(add2(s, t), lo, hi);
+  return lo + hi;
+}
+constexpr uint64_t kSigns = 0x8000000080000000ull;
+
+// Turns the pairs of two vectors in place; kBack: by the negative angles.
+// cs[i * stride] = {cos, cos, sin, sin} of the pairs 2i and 2i + 1.
+template <bool kInter, bool kBack>
+__device__ __forceinline__ void turn(V8& a, V8& b, const float4* cs, int stride) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(cs + i * stride);
+    const uint64_t c = v.x, s = kBack ? v.y ^ kSigns : v.y, n = kBack ? v.y : v.y ^ kSigns;
+    if constexpr (!kInter) {
+      const uint64_t x = a.p[i];
+      a.p[i] = fma2(c, x, mul2(n, b.p[i]));
+      b.p[i] = fma2(c, b.p[i], mul2(s, x));
+    } else {
+      float c0, c1, s0, s1, n0, n1;
+      unpair(c, c0, c1);
+      unpair(s, s0, s1);
+      unpair(n, n0, n1);
+      V8& x = i < 2 ? a : b;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        uint64_t& y = x.p[2 * (i & 1) + e];
+        float lo, hi;
+        unpair(y, lo, hi);
+        y = fma2(e ? pair(c1, c1) : pair(c0, c0), y, mul2(e ? pair(n1, s1) : pair(n0, s0), pair(hi, lo)));
+      }
+    }
+  }
+}
+
 template <bool kNorm, bool kInter, bool kBwd, bool kDw>
-__global__ void __launch_bounds__(kThreads) vec_kernel(const Args a) {
-  __shared__ float4 cs4[kMaxTokens * kMaxDim / 4];   // (cos, sin) of [token][rot / 2]
-  __shared__ float ws[kNorm ? 2 * kMaxDim : 1];
-  float2* cs = reinterpret_cast<float2*>(cs4);
+__global__ void __launch_bounds__(kThreads, kNorm && kBwd ? 2 : 3) vec_kernel(const Args a) {
+  constexpr int kItems = kNorm && kBwd ? kChunk / 2 : kChunk;  // rows loaded before the first is used
+  // (cos, cos, sin, sin) of [token][i][slot], weights of [side][i][slot]: the
+  // lanes of a head read neighbouring words.
+  __shared__ float4 cs4[kMaxTokens * kMaxDim / 4];
+  __shared__ float4 w4[kNorm ? 2 * kMaxDim / 4 : 1];
   const int L = 1 << a.lanes_log2, D = a.D, half = a.rot >> 1;
   const int slots = D >> 4, turned = a.rot >> 4;
   const int slot = threadIdx.x & (L - 1);
   const bool live_slot = slot < slots;
-  // Columns of the thread's two vectors.
-  const int c0 = kInter ? 16 * slot : (slot < turned ? 8 * slot : a.rot + 16 * (slot - turned));
-  const int c1 = kInter ? c0 + 8 : (slot < turned ? c0 + half : c0 + 8);
-  float accq[kDw ? 16 : 1], acck[kDw ? 16 : 1];
+  // Columns of a slot's two vectors.
+  auto first_col = [&](int sl) { return kInter ? 16 * sl : (sl < turned ? 8 * sl : a.rot + 16 * (sl - turned)); };
+  auto second_col = [&](int sl) { return first_col(sl) + (kInter || sl >= turned ? 8 : half); };
+  const int c0 = first_col(slot), c1 = second_col(slot);
+  uint64_t accq[kDw ? 8 : 1], acck[kDw ? 8 : 1];
   if constexpr (kDw) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) accq[i] = acck[i] = 0.f;
+    for (int i = 0; i < 8; ++i) accq[i] = acck[i] = 0;
   }
   if constexpr (kNorm) {
     for (int i = threadIdx.x; i < 2 * D; i += kThreads) {
-      const int which = i >= D;
-      if (which == 0 || a.heads > a.heads_q) ws[i] = weight_at(a, which, i - which * D);
+      const int which = i >= D, j = i - which * D, e = j & 15, sl = j >> 4;
+      const int col = e < 8 ? first_col(sl) + e : second_col(sl) + e - 8;
+      if (which == 0 || a.heads > a.heads_q)
+        reinterpret_cast<float*>(w4 + (which * 4 + (e >> 2)) * slots + sl)[e & 3] = weight_at(a, which, col);
     }
   }
-  const int n_rows = a.tokens * a.heads;           // (token, head) rows of a full block
   const int step = kThreads >> a.lanes_log2;       // rows a pass of the block covers
   const int row0 = threadIdx.x >> a.lanes_log2;
   const float inv_d = 1.0f / static_cast<float>(D);
+  const Side q = a.side[0], k = a.side[1];
 
   for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens; t0 < a.T;
        t0 += static_cast<int64_t>(gridDim.x) * a.tokens) {
+    const int n_tokens = static_cast<int>(a.T - t0 < a.tokens ? a.T - t0 : a.tokens);
+    const int n_rows = n_tokens * a.heads;         // (token, head) rows of the block
     bool first = true;
-    // Uniform trip count: every lane takes part in the shuffles of each row.
-    for (int rb = 0; rb < n_rows; rb += kChunk * step) {
-      uint4 xa[kChunk], xb[kChunk], da[kBwd ? kChunk : 1], db[kBwd ? kChunk : 1];
+    const __nv_bfloat16 *qx = q.x + t0 * q.x_tok, *kx = k.x + t0 * k.x_tok;
+    const __nv_bfloat16 *qd = q.dy + t0 * q.dy_tok, *kd = k.dy + t0 * k.dy_tok;
+    __nv_bfloat16 *qo = q.out + t0 * (a.heads_q * D), *ko = k.out + t0 * ((a.heads - a.heads_q) * D);
+    // Uniform trip counts: every lane takes part in the shuffles of each row.
+    for (int rb = 0; rb < n_rows; rb += kItems * step) {
+      uint4 xa[kItems], xb[kItems], da[kBwd ? kItems : 1], db[kBwd ? kItems : 1];
+      int tok[kItems], head[kItems];
 #pragma unroll
-      for (int u = 0; u < kChunk; ++u) {
+      for (int u = 0; u < kItems; ++u) {
+        if (rb + u * step >= n_rows) continue;
         const int row = rb + u * step + row0;
-        const int tl = row / a.heads;
-        int h = row - tl * a.heads;
-        const int64_t t = t0 + tl;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        xa[u] = xb[u] = zero;
-        if constexpr (kBwd) da[u] = db[u] = zero;
-        if (live_slot && row < n_rows && t < a.T) {
-          const Side& s = a.side[h >= a.heads_q];
-          if (h >= a.heads_q) h -= a.heads_q;
+        tok[u] = a.heads_magic ? __umulhi(row, a.heads_magic) : row;   // row / heads
+        head[u] = row - tok[u] * a.heads;
+        xa[u] = xb[u] = make_uint4(0, 0, 0, 0);
+        if constexpr (kBwd) da[u] = db[u] = make_uint4(0, 0, 0, 0);
+        if (live_slot && row < n_rows) {
+          const bool is_k = head[u] >= a.heads_q;
+          const int h = is_k ? head[u] - a.heads_q : head[u];
           if constexpr (!kBwd || kNorm) {
-            const __nv_bfloat16* p = s.x + t * s.x_tok + h * s.x_head;
+            const __nv_bfloat16* p = (is_k ? kx : qx) + (tok[u] * static_cast<int>(is_k ? k.x_tok : q.x_tok) +
+                                                         h * static_cast<int>(is_k ? k.x_head : q.x_head));
             xa[u] = load_stream(p + c0);
             xb[u] = load_stream(p + c1);
           }
           if constexpr (kBwd) {
-            const __nv_bfloat16* p = s.dy + t * s.dy_tok + h * s.dy_head;
+            const __nv_bfloat16* p = (is_k ? kd : qd) + (tok[u] * static_cast<int>(is_k ? k.dy_tok : q.dy_tok) +
+                                                         h * static_cast<int>(is_k ? k.dy_head : q.dy_head));
             da[u] = load_stream(p + c0);
             db[u] = load_stream(p + c1);
           }
@@ -152,130 +225,89 @@ __global__ void __launch_bounds__(kThreads) vec_kernel(const Args a) {
       if (first) {  // the block's angles, formed while the first loads are in flight
         first = false;
         __syncthreads();
-        for (int i = threadIdx.x; i < a.tokens * half; i += kThreads) {
-          const int tl = i / half;
-          if (t0 + tl < a.T) cs[i] = cos_sin(a, t0 + tl, i - tl * half);
+        for (int i = threadIdx.x; i < n_tokens * half; i += kThreads) {
+          const int tl = i / half, p = i - tl * half;
+          const float2 cs = cos_sin(a, t0 + tl, p);
+          float* o = reinterpret_cast<float*>(cs4 + (tl * 4 + ((p & 7) >> 1)) * turned + (p >> 3)) + (p & 1);
+          o[0] = cs.x;
+          o[2] = cs.y;
         }
         __syncthreads();
       }
 #pragma unroll
-      for (int u = 0; u < kChunk; ++u) {
-        const int row = rb + u * step + row0;
-        const int tl = row / a.heads;
-        int h = row - tl * a.heads;
-        const int64_t t = t0 + tl;
-        const bool live = live_slot && row < n_rows && t < a.T;
-        const int which = h >= a.heads_q;
-        float x0[8], x1[8], y0[8], y1[8], c[8], sn[8];
-        unpack8(xa[u], x0);
-        unpack8(xb[u], x1);
-        if (live && slot < turned) {
-          const float4* q = cs4 + ((tl * half) >> 1) + slot * 4;
+      for (int u = 0; u < kItems; ++u) {
+        if (rb + u * step >= n_rows) break;
+        const bool live = live_slot && rb + u * step + row0 < n_rows;
+        const bool is_k = head[u] >= a.heads_q;
+        const float4* cs = cs4 + tok[u] * 4 * turned + slot;
+        const bool turns = live && slot < turned;
+        V8 w0, w1, y0, y1;
+        if constexpr (kNorm) {
+          const float4* w = w4 + (is_k ? 4 * slots : 0) + (live ? slot : 0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float4 v = q[i];
-            c[2 * i] = v.x;
-            sn[2 * i] = v.y;
-            c[2 * i + 1] = v.z;
-            sn[2 * i + 1] = v.w;
+          for (int i = 0; i < 2; ++i) {
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(w + i * slots);
+            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(w + (2 + i) * slots);
+            w0.p[2 * i] = v.x, w0.p[2 * i + 1] = v.y;
+            w1.p[2 * i] = x.x, w1.p[2 * i + 1] = x.y;
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) c[i] = 1.f, sn[i] = 0.f;
         }
-        const float* w = ws + which * D;
         if constexpr (!kBwd) {
+          y0 = unpack(xa[u]);
+          y1 = unpack(xb[u]);
           if constexpr (kNorm) {
-            float ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) ss += x0[i] * x0[i] + x1[i] * x1[i];
+            float ss = dot(y0, y0, y1, y1);
             for (int o = L >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             const float r = rsqrtf(ss * inv_d + a.eps);
-            if (live) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                x0[i] *= r * w[c0 + i];
-                x1[i] *= r * w[c1 + i];
-              }
-            }
+            y0 = mul(y0, w0);
+            y1 = mul(y1, w1);
+            scale(y0, r);
+            scale(y1, r);
           }
-          if constexpr (kInter) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              y0[2 * i] = c[i] * x0[2 * i] - sn[i] * x0[2 * i + 1];
-              y0[2 * i + 1] = c[i] * x0[2 * i + 1] + sn[i] * x0[2 * i];
-              y1[2 * i] = c[4 + i] * x1[2 * i] - sn[4 + i] * x1[2 * i + 1];
-              y1[2 * i + 1] = c[4 + i] * x1[2 * i + 1] + sn[4 + i] * x1[2 * i];
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              y0[i] = c[i] * x0[i] - sn[i] * x1[i];
-              y1[i] = c[i] * x1[i] + sn[i] * x0[i];
-            }
-          }
+          if (turns) turn<kInter, false>(y0, y1, cs, turned);
         } else {
-          float d0[8], d1[8];
-          unpack8(da[u], d0);
-          unpack8(db[u], d1);
-          if constexpr (kInter) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              y0[2 * i] = c[i] * d0[2 * i] + sn[i] * d0[2 * i + 1];
-              y0[2 * i + 1] = c[i] * d0[2 * i + 1] - sn[i] * d0[2 * i];
-              y1[2 * i] = c[4 + i] * d1[2 * i] + sn[4 + i] * d1[2 * i + 1];
-              y1[2 * i + 1] = c[4 + i] * d1[2 * i + 1] - sn[4 + i] * d1[2 * i];
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              y0[i] = c[i] * d0[i] + sn[i] * d1[i];
-              y1[i] = c[i] * d1[i] - sn[i] * d0[i];
-            }
-          }
+          y0 = unpack(da[u]);
+          y1 = unpack(db[u]);
+          if (turns) turn<kInter, true>(y0, y1, cs, turned);
           if constexpr (kNorm) {
-            float ss = 0.f, gx = 0.f, g0[8], g1[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              ss += x0[i] * x0[i] + x1[i] * x1[i];
-              g0[i] = live ? y0[i] * w[c0 + i] : 0.f;
-              g1[i] = live ? y1[i] * w[c1 + i] : 0.f;
-              gx += g0[i] * x0[i] + g1[i] * x1[i];
-            }
+            const V8 x0 = unpack(xa[u]), x1 = unpack(xb[u]);
+            const V8 g0 = mul(y0, w0), g1 = mul(y1, w1);
+            float ss = dot(x0, x0, x1, x1), gx = dot(g0, x0, g1, x1);
             for (int o = L >> 1; o; o >>= 1) {
               ss += __shfl_xor_sync(0xffffffffu, ss, o);
               gx += __shfl_xor_sync(0xffffffffu, gx, o);
             }
             const float r = rsqrtf(ss * inv_d + a.eps);
-            const float m = gx * r * r * inv_d;   // mean(g w xh) r
+            const float m = -gx * r * r * inv_d;   // -mean(g w xh) r
             if constexpr (kDw) {
               if (live) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  const float e0 = y0[i] * (x0[i] * r), e1 = y1[i] * (x1[i] * r);
-                  if (which) {
-                    acck[i] += e0;
-                    acck[8 + i] += e1;
+                for (int i = 0; i < 4; ++i) {
+                  const uint64_t e0 = mul2(x0.p[i], pair(r, r)), e1 = mul2(x1.p[i], pair(r, r));
+                  if (is_k) {
+                    acck[i] = fma2(y0.p[i], e0, acck[i]);
+                    acck[4 + i] = fma2(y1.p[i], e1, acck[4 + i]);
                   } else {
-                    accq[i] += e0;
-                    accq[8 + i] += e1;
+                    accq[i] = fma2(y0.p[i], e0, accq[i]);
+                    accq[4 + i] = fma2(y1.p[i], e1, accq[4 + i]);
                   }
                 }
               }
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              y0[i] = r * (g0[i] - x0[i] * m);
-              y1[i] = r * (g1[i] - x1[i] * m);
+            for (int i = 0; i < 4; ++i) {
+              y0.p[i] = fma2(x0.p[i], pair(m, m), g0.p[i]);
+              y1.p[i] = fma2(x1.p[i], pair(m, m), g1.p[i]);
             }
+            scale(y0, r);
+            scale(y1, r);
           }
         }
         if (live) {
-          const int heads = which ? a.heads - a.heads_q : a.heads_q;
-          if (which) h -= a.heads_q;
-          __nv_bfloat16* o = a.side[which].out + (t * heads + h) * D;
-          __stcs(reinterpret_cast<uint4*>(o + c0), pack8(y0));
-          __stcs(reinterpret_cast<uint4*>(o + c1), pack8(y1));
+          const int heads = is_k ? a.heads - a.heads_q : a.heads_q, h = is_k ? head[u] - a.heads_q : head[u];
+          __nv_bfloat16* o = (is_k ? ko : qo) + (tok[u] * heads + h) * D;
+          __stcs(reinterpret_cast<uint4*>(o + c0), pack(y0));
+          __stcs(reinterpret_cast<uint4*>(o + c1), pack(y1));
         }
       }
     }
@@ -288,96 +320,104 @@ __global__ void __launch_bounds__(kThreads) vec_kernel(const Args a) {
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) red[threadIdx.x * 16 + i] = which ? acck[i] : accq[i];
+      for (int i = 0; i < 8; ++i)
+        reinterpret_cast<uint64_t*>(red)[threadIdx.x * 8 + i] = which ? acck[i] : accq[i];
       __syncthreads();
       for (int i = threadIdx.x; i < slots * 16; i += kThreads) {
         const int sl = i >> 4, e = i & 15;
         float sum = 0.f;
         for (int r = 0; r < step; ++r) sum += red[((r << a.lanes_log2) + sl) * 16 + e];
-        const int b0 = kInter ? 16 * sl : (sl < turned ? 8 * sl : a.rot + 16 * (sl - turned));
-        const int b1 = kInter ? b0 + 8 : (sl < turned ? b0 + half : b0 + 8);
-        a.dw_part[(static_cast<int64_t>(blockIdx.x) * 2 + which) * D + (e < 8 ? b0 + e : b1 + e - 8)] = sum;
+        a.dw_part[(static_cast<int64_t>(blockIdx.x) * 2 + which) * D +
+                  (e < 8 ? first_col(sl) + e : second_col(sl) + e - 8)] = sum;
       }
     }
   }
 }
 
-// Scalar form: a warp per (token, head) row, lane l holding columns l, l + 32, ...
+// Scalar form: a block per few tokens, a warp per (token, head) row, lane l holding columns l, l + 32, ...
 template <bool kNorm, bool kInter, bool kBwd, bool kDw>
 __global__ void __launch_bounds__(kThreads) scalar_kernel(const Args a) {
   constexpr int kPer = kMaxDim / 32;
-  __shared__ float red[kDw ? (kThreads / 32) * kMaxDim : 1];
+  constexpr int kWarps = kThreads / 32;
+  __shared__ float red[kDw ? kWarps * kMaxDim : 1];
+  __shared__ float2 angles[kMaxTokens * kMaxDim / 2];   // (cos, sin) of [token][rot / 2]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int D = a.D, half = a.rot >> 1;
-  const int64_t rows = a.T * a.heads;
   float accq[kDw ? kPer : 1], acck[kDw ? kPer : 1];
   if constexpr (kDw) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) accq[i] = acck[i] = 0.f;
   }
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + warp; row < rows;
-       row += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
-    const int64_t t = row / a.heads;
-    int h = static_cast<int>(row - t * a.heads);
-    const int which = h >= a.heads_q;
-    const Side& s = a.side[which];
-    if (which) h -= a.heads_q;
-    const __nv_bfloat16* x = s.x + t * s.x_tok + h * s.x_head;
-    const __nv_bfloat16* dy = kBwd ? s.dy + t * s.dy_tok + h * s.dy_head : nullptr;
-    __nv_bfloat16* out = s.out + (t * (which ? a.heads - a.heads_q : a.heads_q) + h) * D;
-    float r = 1.f;
-    if constexpr (kNorm) {
-      float ss = 0.f;
-      for (int d = lane; d < D; d += 32) {
-        const float v = __bfloat162float(x[d]);
-        ss += v * v;
+  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens; t0 < a.T;
+       t0 += static_cast<int64_t>(gridDim.x) * a.tokens) {
+    const int n_tokens = static_cast<int>(a.T - t0 < a.tokens ? a.T - t0 : a.tokens);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_tokens * half; i += kThreads) angles[i] = cos_sin(a, t0 + i / half, i % half);
+    __syncthreads();
+    for (int row = warp; row < n_tokens * a.heads; row += kWarps) {
+      const int tl = row / a.heads;
+      const int64_t t = t0 + tl;
+      int h = row - tl * a.heads;
+      const int which = h >= a.heads_q;
+      const Side& s = a.side[which];
+      if (which) h -= a.heads_q;
+      const __nv_bfloat16* x = s.x + t * s.x_tok + h * s.x_head;
+      const __nv_bfloat16* dy = kBwd ? s.dy + t * s.dy_tok + h * s.dy_head : nullptr;
+      __nv_bfloat16* out = s.out + (t * (which ? a.heads - a.heads_q : a.heads_q) + h) * D;
+      float r = 1.f;
+      if constexpr (kNorm) {
+        float ss = 0.f;
+        for (int d = lane; d < D; d += 32) {
+          const float v = __bfloat162float(x[d]);
+          ss += v * v;
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        r = rsqrtf(ss / static_cast<float>(D) + a.eps);
       }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      r = rsqrtf(ss / static_cast<float>(D) + a.eps);
-    }
-    float y[kPer], gx = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int d = lane + 32 * i;
-      y[i] = 0.f;
-      if (d >= D) continue;
-      const __nv_bfloat16* in = kBwd ? dy : x;
-      float v = __bfloat162float(in[d]);
-      if constexpr (kNorm && !kBwd) v *= r * weight_at(a, which, d);
-      if (d < a.rot) {
-        const bool left = kInter ? (d & 1) == 0 : d < half;
-        const int mate = kInter ? d ^ 1 : (left ? d + half : d - half);
-        float m = __bfloat162float(in[mate]);
-        if constexpr (kNorm && !kBwd) m *= r * weight_at(a, which, mate);
-        const float2 cs = cos_sin(a, t, kInter ? d >> 1 : (left ? d : mate));
-        // forward: left -s, right +s; the transposed rotation: left +s, right -s
-        v = cs.x * v + ((left == kBwd) ? cs.y : -cs.y) * m;
-      }
-      y[i] = v;
-      if constexpr (kNorm && kBwd) gx += v * weight_at(a, which, d) * __bfloat162float(x[d]);
-    }
-    if constexpr (kNorm && kBwd) {
-#pragma unroll
-      for (int o = 16; o; o >>= 1) gx += __shfl_xor_sync(0xffffffffu, gx, o);
-      const float m = gx * r * r / static_cast<float>(D);
+      float y[kPer], gx = 0.f;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int d = lane + 32 * i;
+        y[i] = 0.f;
         if (d >= D) continue;
-        const float xv = __bfloat162float(x[d]);
-        if constexpr (kDw) {
-          if (which)
-            acck[i] += y[i] * (xv * r);
-          else
-            accq[i] += y[i] * (xv * r);
+        const __nv_bfloat16* in = kBwd ? dy : x;
+        float v = __bfloat162float(in[d]);
+        if constexpr (kNorm && !kBwd) v *= r * weight_at(a, which, d);
+        if (d < a.rot) {
+          const bool left = kInter ? (d & 1) == 0 : d < half;
+          const int mate = kInter ? d ^ 1 : (left ? d + half : d - half);
+          float m = __bfloat162float(in[mate]);
+          if constexpr (kNorm && !kBwd) m *= r * weight_at(a, which, mate);
+          const float2 cs = angles[tl * half + (kInter ? d >> 1 : (left ? d : mate))];
+          // forward: left -s, right +s; the transposed rotation: left +s, right -s
+          v = cs.x * v + ((left == kBwd) ? cs.y : -cs.y) * m;
         }
-        y[i] = r * (y[i] * weight_at(a, which, d) - xv * m);
+        y[i] = v;
+        if constexpr (kNorm && kBwd) gx += v * weight_at(a, which, d) * __bfloat162float(x[d]);
       }
-    }
+      if constexpr (kNorm && kBwd) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (lane + 32 * i < D) out[lane + 32 * i] = __float2bfloat16_rn(y[i]);
+        for (int o = 16; o; o >>= 1) gx += __shfl_xor_sync(0xffffffffu, gx, o);
+        const float m = gx * r * r / static_cast<float>(D);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int d = lane + 32 * i;
+          if (d >= D) continue;
+          const float xv = __bfloat162float(x[d]);
+          if constexpr (kDw) {
+            if (which)
+              acck[i] += y[i] * (xv * r);
+            else
+              accq[i] += y[i] * (xv * r);
+          }
+          y[i] = r * (y[i] * weight_at(a, which, d) - xv * m);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (lane + 32 * i < D) out[lane + 32 * i] = __float2bfloat16_rn(y[i]);
+    }
   }
   if constexpr (kDw) {
     for (int which = 0; which < 2; ++which) {
@@ -387,7 +427,7 @@ __global__ void __launch_bounds__(kThreads) scalar_kernel(const Args a) {
       __syncthreads();
       for (int d = threadIdx.x; d < D; d += kThreads) {
         float sum = 0.f;
-        for (int w = 0; w < kThreads / 32; ++w) sum += red[w * kMaxDim + d];
+        for (int w = 0; w < kWarps; ++w) sum += red[w * kMaxDim + d];
         a.dw_part[(static_cast<int64_t>(blockIdx.x) * 2 + which) * D + d] = sum;
       }
     }
@@ -421,8 +461,10 @@ Kernel pick(bool vec, bool inter) {
   return inter ? scalar_kernel<kNorm, true, kBwd, kDw> : scalar_kernel<kNorm, false, kBwd, kDw>;
 }
 
-bool rows_aligned(const void* p, int64_t tok, int64_t head) {
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && tok % 8 == 0 && head % 8 == 0;
+// 16-byte rows, offsets within a block in 32 bits.
+bool rows_fit(const void* p, int64_t tok, int64_t head, int heads) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && tok % 8 == 0 && head % 8 == 0 && tok >= 0 && head >= 0 &&
+         tok * kMaxTokens + head * heads < (int64_t(1) << 31);
 }
 
 int sm_count() {
@@ -434,12 +476,12 @@ int sm_count() {
 }
 
 int launch(Args& a, bool norm, bool inter, bool bwd, float* dqw, float* dkw, cudaStream_t stream) {
-  bool vec = a.D % 16 == 0 && a.rot % 16 == 0;
+  bool vec = a.D % 16 == 0 && a.rot % 16 == 0 && a.heads <= 4096;
   for (int i = 0; i < (a.heads > a.heads_q ? 2 : 1); ++i) {
     const Side& s = a.side[i];
     vec = vec && (reinterpret_cast<uintptr_t>(s.out) & 15u) == 0;
-    if (!bwd || norm) vec = vec && rows_aligned(s.x, s.x_tok, s.x_head);
-    if (bwd) vec = vec && rows_aligned(s.dy, s.dy_tok, s.dy_head);
+    if (!bwd || norm) vec = vec && rows_fit(s.x, s.x_tok, s.x_head, a.heads);
+    if (bwd) vec = vec && rows_fit(s.dy, s.dy_tok, s.dy_head, a.heads);
   }
   const bool dw = dqw || dkw;
   const Kernel kernel = !bwd ? (norm ? pick<true, false, false>(vec, inter) : pick<false, false, false>(vec, inter))
@@ -450,16 +492,27 @@ int launch(Args& a, bool norm, bool inter, bool bwd, float* dqw, float* dkw, cud
   if (vec) {
     a.lanes_log2 = 0;
     while ((16 << a.lanes_log2) < a.D) ++a.lanes_log2;
-    // About kChunk rows to a thread, so that a block's angles serve many rows;
-    // fewer tokens to a block while the blocks would not cover the GPU twice.
-    int64_t tokens = (static_cast<int64_t>(kChunk) * (kThreads >> a.lanes_log2) + a.heads / 2) / a.heads;
-    tokens = tokens < 1 ? 1 : tokens > kMaxTokens ? kMaxTokens : tokens;
+    // Tokens of a block: up to two loads' worth of rows, the count that leaves
+    // the fewest of a pass's rows idle (36 heads of 128: 4 tokens in 160 rows
+    // measured 41 us where 128 + 32 of 256 took 54); fewer while the blocks
+    // would not cover the GPU twice.
+    const int64_t pass = kThreads >> a.lanes_log2;
+    int64_t tokens = 1;
+    auto use = [&](int64_t n) { return static_cast<double>(n * a.heads) / ((n * a.heads + pass - 1) / pass * pass); };
+    for (int64_t n = 2; n <= kMaxTokens && n * a.heads <= 2 * kChunk * pass; ++n)
+      if (use(n) > use(tokens) + 0.01) tokens = n;
+    while (tokens > 1 && (a.T + tokens - 1) / tokens < 2 * sm_count()) --tokens;
+    a.tokens = static_cast<int>(tokens);
+    // exact while row * heads < 2^32
+    a.heads_magic = static_cast<unsigned>(((uint64_t(1) << 32) + a.heads - 1) / a.heads);
+    grid = (a.T + tokens - 1) / tokens;
+  } else {
+    // Two rows to a warp at least, so that a block's angles serve them.
+    int64_t tokens = (2 * (kThreads / 32) + a.heads - 1) / a.heads;
+    if (tokens > kMaxTokens) tokens = kMaxTokens;
     while (tokens > 1 && (a.T + tokens - 1) / tokens < 2 * sm_count()) --tokens;
     a.tokens = static_cast<int>(tokens);
     grid = (a.T + tokens - 1) / tokens;
-  } else {
-    grid = (a.T * a.heads + kThreads / 32 - 1) / (kThreads / 32);
-    if (grid > (1 << 20)) grid = 1 << 20;
   }
   if (dw && grid > kGradBlocks) grid = kGradBlocks;
   if (grid > 0x7fffffff) grid = 0x7fffffff;
