@@ -40,35 +40,30 @@ def row_ranges(batch, length, *, documents=None, prefix=None, window=None, lengt
         raise ValueError("batch and length must not be negative")
     if window is not None and (not causal or window < 1):
         raise ValueError("a window needs a causal mask and a size >= 1")
-    for t in (documents, prefix, lengths):
-        if t is not None and device is None:
-            device = t.device
+    given = [t for t in (documents, prefix, lengths) if t is not None]
+    if device is None and given:
+        device = given[0].device
+    for name, t, shape in (("documents", documents, (batch, length)), ("prefix", prefix, (batch,)),
+                           ("lengths", lengths, (batch,))):
+        if t is not None and tuple(t.shape) != shape:
+            raise ValueError(f"{name} must be {list(shape)}")
     at = torch.arange(length, device=device, dtype=torch.int64).expand(batch, length)
-    begin = torch.zeros_like(at)
-    stop = torch.full_like(at, length)
-    if documents is not None:
-        if documents.shape != (batch, length):
-            raise ValueError("documents must be [batch, length]")
+    begin, stop = torch.zeros_like(at), torch.full_like(at, length)
+    if documents is not None and length:
+        documents = documents.to(at.device)
         change = documents[:, 1:] != documents[:, :-1]
-        edge = torch.cat((torch.ones_like(documents[:, :1], dtype=torch.bool), change), 1) if length else change
-        begin = torch.where(edge, at, torch.zeros_like(at)).cummax(1).values if length else begin
-        tail = torch.cat((change, torch.ones_like(documents[:, :1], dtype=torch.bool)), 1) if length else change
-        stop = torch.where(tail, at + 1, torch.full_like(at, length)).flip(1).cummin(1).values.flip(1) \
-            if length else stop
+        edge = torch.ones_like(documents[:, :1], dtype=torch.bool)
+        begin = at.masked_fill(~torch.cat((edge, change), 1), 0).cummax(1).values
+        stop = (at + 1).masked_fill(~torch.cat((change, edge), 1), length).flip(1).cummin(1).values.flip(1)
     end = torch.minimum(at + 1, stop) if causal else stop
     if prefix is not None:
-        if prefix.shape != (batch,):
-            raise ValueError("prefix must be [batch]")
-        end = torch.maximum(end, torch.minimum(prefix.to(torch.int64)[:, None], stop))
+        end = torch.maximum(end, torch.minimum(prefix.to(at)[:, None], stop))
     if window is not None:
         begin = torch.maximum(begin, at + 1 - window)
     if lengths is not None:
-        if lengths.shape != (batch,):
-            raise ValueError("lengths must be [batch]")
-        live = lengths.to(torch.int64)[:, None]
-        end = torch.where(at < live, torch.minimum(end, live), torch.zeros_like(end))
-    end = torch.maximum(end, torch.zeros_like(end))
-    return begin.to(torch.int32).contiguous(), end.to(torch.int32).contiguous()
+        live = lengths.to(at)[:, None]
+        end = torch.minimum(end, live).masked_fill(at >= live, 0)
+    return begin.to(torch.int32).contiguous(), end.clamp_min(0).to(torch.int32).contiguous()
 
 
 def _view(x):

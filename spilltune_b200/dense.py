@@ -18,15 +18,25 @@ is a plain frozen tensor, so the reference's ``StreamingBlockFunction``
 tensors, drives this functional unchanged: forward under a ``forward`` borrow,
 recompute + ``torch.autograd.grad`` under a ``backward`` borrow.
 
+Between the projections the functional follows the reference op by op (eager
+torch) by default.  With ``attention=FusedAttention(...)`` the norm of each head,
+the rotation and the attention run as the fused operators of
+``spilltune_b200.rotary`` and ``spilltune_b200.attention`` instead, reading q, k
+and v in place in the fused projection's output: no [S, S] mask or scores, no
+repeated key/value heads.
+
 ``PackedBlockReloader`` is the matching ``weight_reloader`` (its ``borrow(phase)``
 is what recompute.py:137-144 calls) over a ``PackedSlotSession``.
 """
 from contextlib import contextmanager
+from dataclasses import dataclass
+from typing import Optional
 
 import torch
 import torch.nn.functional as F
 
-from . import codec, ops
+from . import attention as fused_attention
+from . import codec, ops, rotary
 
 _LUTS = {}
 
@@ -61,14 +71,48 @@ def rms(hidden, weight, eps):
     return weight * (value * torch.rsqrt(value.square().mean(-1, keepdim=True) + eps)).to(hidden.dtype)
 
 
+@dataclass(frozen=True)
+class FusedAttention:
+    """How a block's fused attention sees its tokens: shared by all layers of a
+    batch, as the mask and the cos/sin tables of the eager form are.
+
+    begin, end: int32 [batch, tokens], the keys each token sees
+        (``attention.row_ranges``).
+    softcap, slopes, scale: as ``attention.attend``.
+    interleaved, factor: as ``rotary.rotate``.
+    The block's ``position_embeddings`` are then ``(positions, inv_freq)``
+    (``rotary.frequencies``) and its ``attention_mask`` None."""
+    begin: torch.Tensor
+    end: torch.Tensor
+    softcap: float = 0.0
+    slopes: Optional[torch.Tensor] = None
+    scale: Optional[float] = None
+    interleaved: bool = False
+    factor: float = 1.0
+
+    def __call__(self, q, k, v, positions, inv_freq, q_weight=None, k_weight=None, eps=None):
+        """Attended values [batch, tokens, heads, D] of projected q, k, v."""
+        turn = dict(interleaved=self.interleaved, factor=self.factor)
+        if q_weight is not None:
+            q, k = rotary.norm_rotate(q, k, q_weight, k_weight, positions, inv_freq, eps=eps, **turn)
+        else:
+            q, k = rotary.rotate(q, k, positions, inv_freq, **turn)
+        return fused_attention.attend(q, k, v, self.begin, self.end, scale=self.scale, softcap=self.softcap,
+                                      slopes=self.slopes)
+
+
 def block_forward(hidden_states, position_embeddings, attention_mask, linear, weights, *, heads, kv_heads,
-                  head_dim, eps, qk_norm=False, feed_forward=None, fused=None):
+                  head_dim, eps, qk_norm=False, feed_forward=None, fused=None, attention=None):
     """The dense block's math (adapters/dense.py:120-153) with the projections
     supplied by ``linear(x, path)``: RMSNorm, GQA attention with full RoPE and
     an additive mask (softmax in FP32), residuals, SwiGLU MLP.  The op order
     follows the reference so BF16 roundings match.  ``fused(x, paths)``, when
     given, computes projections that share their input (q, k, v; gate, up)
-    together and returns their outputs in order."""
+    together and returns their outputs in order.  ``attention``: a
+    ``FusedAttention`` in place of the eager norms of heads, rotation and
+    attention (see there for the positions and the mask)."""
+    if attention is not None and attention_mask is not None:
+        raise ValueError("fused attention takes row ranges, not an attention mask")
     if fused is None:
         fused = lambda x, paths: [linear(x, p) for p in paths]  # noqa: E731
     residual = hidden_states
@@ -77,6 +121,11 @@ def block_forward(hidden_states, position_embeddings, attention_mask, linear, we
     q, k, v = fused(x, ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj"))
     q = q.view(shape)
     k = k.view(shape)
+    if attention is not None:
+        norms = (weights["self_attn.q_norm.weight"], weights["self_attn.k_norm.weight"], eps) if qk_norm else ()
+        attended = attention(q, k, v.view(shape), *position_embeddings, *norms)
+        attended = attended.reshape(*x.shape[:-1], heads * head_dim)
+        return _after_attention(attended, residual, linear, fused, weights, eps, feed_forward)
     v = v.view(shape).transpose(1, 2)
     if qk_norm:
         q = rms(q, weights["self_attn.q_norm.weight"], eps)
@@ -98,6 +147,11 @@ def block_forward(hidden_states, position_embeddings, attention_mask, linear, we
     scores = (q @ k.transpose(-2, -1)) * head_dim ** -0.5
     probabilities = torch.softmax(scores + attention_mask, dim=-1, dtype=torch.float32).to(q.dtype)
     attended = (probabilities @ v).transpose(1, 2).contiguous().reshape(*x.shape[:-1], heads * head_dim)
+    return _after_attention(attended, residual, linear, fused, weights, eps, feed_forward)
+
+
+def _after_attention(attended, residual, linear, fused, weights, eps, feed_forward):
+    """The block from the output projection on."""
     x = residual + linear(attended, "self_attn.o_proj")
     residual = x
     x = rms(x, weights["post_attention_layernorm.weight"], eps)
@@ -109,7 +163,7 @@ def block_forward(hidden_states, position_embeddings, attention_mask, linear, we
 
 def packed_dense_block(hidden_states, position_embeddings, attention_mask, *, heads, kv_heads, head_dim, eps,
                        lora_q, lora_v, lora_o, qk_norm=False, feed_forward=None, codec_name=codec.INT4_SYM,
-                       lora_k=None, lora_gate=None, lora_up=None, lora_down=None, **weights):
+                       lora_k=None, lora_gate=None, lora_up=None, lora_down=None, attention=None, **weights):
     """Drop-in for the reference's ``dense_block`` functional over packed parts.
 
     ``lora_q``/``lora_v``/``lora_o`` are the block's ``LoRAProjection`` objects
@@ -119,7 +173,10 @@ def packed_dense_block(hidden_states, position_embeddings, attention_mask, *, he
     seven.  Each is a keyword argument of its own, so ``StreamingBlockFunction``'s
     binding check (recompute.py:180-203) sees every bound projection.  Each
     projection runs as one fused call; unadapted projections run the plain
-    frozen F.linear (rank 0)."""
+    frozen F.linear (rank 0).  ``attention``: a ``FusedAttention`` runs the norms
+    of heads, the rotation and the attention as fused operators too; then
+    ``position_embeddings`` is ``(positions, inv_freq)`` and ``attention_mask``
+    None."""
     adapters = {"self_attn.q_proj": lora_q, "self_attn.k_proj": lora_k, "self_attn.v_proj": lora_v,
                 "self_attn.o_proj": lora_o, "mlp.gate_proj": lora_gate, "mlp.up_proj": lora_up,
                 "mlp.down_proj": lora_down}
@@ -153,7 +210,7 @@ def packed_dense_block(hidden_states, position_embeddings, attention_mask, *, he
 
     return block_forward(hidden_states, position_embeddings, attention_mask, linear, weights, heads=heads,
                          kv_heads=kv_heads, head_dim=head_dim, eps=eps, qk_norm=qk_norm, feed_forward=feed_forward,
-                         fused=fused)
+                         fused=fused, attention=attention)
 
 
 class PackedBlockReloader:

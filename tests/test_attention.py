@@ -160,3 +160,268 @@ def test_backward(cuda_lib, B, Sq, Sk, H, K, D, mask, cap, slopes):
     want = _oracle(q, k, v, begin, end, D ** -0.5, cap, sl, do)
     for name in got:
         _within(name, got[name], want[name])
+
+
+@pytest.mark.gpu
+def test_strided_views_are_read_in_place(cuda_lib):
+    """Views of one projection's output, heads before tokens, and rows that have to be copied."""
+    B, S, H, K, D = 2, 140, 4, 2, 64
+    q, k, v, do = _inputs(B, S, S, H, K, D, 3)
+    begin, end = (t.cuda() for t in _ranges("causal", B, S, S, 0))
+    want = _both(q, k, v, begin, end, do)
+    x = torch.cat([t.flatten(2) for t in (q, k, v)], -1)
+    a, b, c = x.split([H * D, K * D, K * D], -1)
+    views = (a.unflatten(-1, (H, D)), b.unflatten(-1, (K, D)), c.unflatten(-1, (K, D)))
+    heads_first = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    odd = [torch.nn.functional.pad(t, (1, 2))[..., 1:D + 1] for t in (q, k, v)]
+    for q2, k2, v2 in (views, heads_first, odd):
+        got = _both(q2, k2, v2, begin, end, do.transpose(1, 2).contiguous().transpose(1, 2))
+        assert all(torch.equal(got[n], want[n]) for n in want)
+    one = torch.ones((), dtype=torch.bfloat16, device="cuda").expand(do.shape)
+    assert all(torch.equal(x, y) for x, y in zip(_both(q, k, v, begin, end, one).values(),
+                                                 _both(q, k, v, begin, end, one.contiguous()).values()))
+    cols = torch.stack((begin, end), -1)
+    got = _both(q, k, v, cols[..., 0], cols[..., 1], do)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.gpu
+def test_values_out_of_sight(cuda_lib):
+    """Keys that no row sees: infinities and NaN in their k and v leave forward and backward alone, as far as
+    they lie in 128-key tiles that no row of the 128-row tile sees.  Scores of hidden keys inside a seen tile may
+    be anything (NaN keys with finite values)."""
+    B, S, H, K, D = 1, 512, 2, 2, 64
+    q, k, v, do = _inputs(B, S, S, H, K, D, 4)
+    begin = torch.full((B, S), 128, dtype=torch.int32, device="cuda")
+    end = torch.full((B, S), 300, dtype=torch.int32, device="cuda")
+    want = _both(q, k, v, begin, end, do)
+    bad_k, bad_v = k.clone(), v.clone()
+    bad_k[:, :128], bad_k[:, 384:] = float("nan"), float("inf")
+    bad_v[:, :128], bad_v[:, 384:] = float("inf"), float("nan")
+    got = _both(q, bad_k, bad_v, begin, end, do)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    from spilltune_b200 import attention
+    bad_k[:, 300:384] = float("nan")
+    out, lse = attention.fwd(q, bad_k, bad_v, begin, end)
+    assert torch.equal(out, want["out"]) and torch.equal(lse, want["lse"])
+
+
+@pytest.mark.gpu
+def test_empty_rows_and_rows_behind_the_last(cuda_lib):
+    """Rows that see nothing: zero output and gradient, log sum -inf; empty inputs."""
+    from spilltune_b200 import attention
+    B, S, H, K, D = 2, 200, 4, 2, 64
+    q, k, v, do = _inputs(B, S, S, H, K, D, 5)
+    begin, end = attention.row_ranges(B, S, lengths=torch.tensor([130, 0]), device="cuda")
+    got = _both(q, k, v, begin.cuda(), end.cuda(), do)
+    for b, live in ((0, 130), (1, 0)):
+        assert not bool(got["out"][b, live:].any()) and bool((got["lse"][b, live:] == -torch.inf).all())
+        for n in ("dq", "dk", "dv"):
+            assert not bool(got[n][b, live:].any()), n
+    short = _both(q[:1, :130], k[:1, :130], v[:1, :130], begin[:1, :130].cuda(), end[:1, :130].cuda(), do[:1, :130])
+    assert torch.equal(short["out"], got["out"][:1, :130])
+    none = torch.zeros(B, 0, dtype=torch.int32, device="cuda")
+    out, lse = attention.fwd(q[:, :0], k, v, none, none)
+    assert out.shape == (B, 0, H, D) and lse.shape == (B, 0, H)
+    grads = attention.bwd(do[:, :0], q[:, :0], k, v, out, lse, none, none)
+    assert grads[0].shape == (B, 0, H, D) and not bool(grads[1].any()) and not bool(grads[2].any())
+    zero = torch.zeros(B, S, dtype=torch.int32, device="cuda")
+    out, lse = attention.fwd(q, k[:, :0], v[:, :0], zero, zero + 5)
+    assert not bool(out.any()) and bool((lse == -torch.inf).all())
+    assert not bool(attention.bwd(do, q, k[:, :0], v[:, :0], out, lse, zero, zero)[0].any())
+
+
+@pytest.mark.gpu
+def test_equal_bits_other_stream_and_captured_passes(cuda_lib):
+    """Twice the same bits; on a side stream; forward and backward in one graph, replayed on new inputs, with a
+    second graph of the same shapes replayed between."""
+    from spilltune_b200 import attention
+    B, S, H, K, D = 2, 260, 14, 2, 64
+    q, k, v, do = _inputs(B, S, S, H, K, D, 6)
+    begin, end = (t.cuda() for t in _ranges("causal", B, S, S, 0))
+    want = _both(q, k, v, begin, end, do)
+    again = _both(q, k, v, begin, end, do)
+    assert all(torch.equal(again[n], want[n]) for n in want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = _both(q, k, v, begin, end, do)
+    side.synchronize()
+    assert all(torch.equal(other[n], want[n]) for n in want)
+
+    def captured(q):
+        out, lse = attention.fwd(q, k, v, begin, end)
+        return (out, *attention.bwd(do, q, k, v, out, lse, begin, end))
+
+    static = [q.clone(), q.clone()]
+    graphs, results = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for graph, x in zip(graphs, static):
+        with torch.cuda.graph(graph):
+            results.append(captured(x))
+    static[0].copy_(q.flip(1))
+    graphs[0].replay()
+    graphs[1].replay()
+    torch.cuda.synchronize()
+    flipped = captured(q.flip(1).contiguous())
+    assert all(torch.equal(x, y) for x, y in zip(results[0], flipped))
+    assert all(torch.equal(x, want[n]) for x, n in zip(results[1], ("out", "dq", "dk", "dv")))
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once(cuda_lib):
+    """Two streams, each with its own call under way (a split forward and a split backward among them)."""
+    cases = []
+    for seed, (B, Sq, Sk, H, K) in enumerate(((1, 3, 3000, 8, 2), (1, 600, 600, 14, 2))):
+        q, k, v, do = _inputs(B, Sq, Sk, H, K, 64, seed)
+        begin, end = (t.cuda() for t in _ranges("causal", B, Sq, Sk, 0))
+        cases.append(((q, k, v, begin, end, do), _both(q, k, v, begin, end, do)))
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[] for _ in cases]
+    from spilltune_b200 import attention
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for s, ((q, k, v, begin, end, do), _), g in zip(streams, cases, got):
+            with torch.cuda.stream(s):
+                out, lse = attention.fwd(q, k, v, begin, end)
+                g.append((out, lse, *attention.bwd(do, q, k, v, out, lse, begin, end)))
+    torch.cuda.synchronize()
+    for (_, want), g in zip(cases, got):
+        for r in g:
+            assert all(torch.equal(x, want[n]) for x, n in zip(r, ("out", "lse", "dq", "dk", "dv")))
+
+
+@pytest.mark.gpu
+def test_autograd_and_differences(cuda_lib):
+    """attend()'s gradients: bwd()'s bits, and a directional derivative against a central difference of the
+    64-bit formula (tied to the kernel by test_backward; every element is off by at most its bound there)."""
+    from spilltune_b200 import attention
+    B, S, H, K, D = 1, 90, 4, 2, 64
+    q, k, v, do = _inputs(B, S, S, H, K, D, 8)
+    begin, end = (t.cuda() for t in _ranges("documents", B, S, S, 2))
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = attention.attend(*leaves, begin, end, softcap=30.0)
+    grads = torch.autograd.grad(out, leaves, do)
+    want = _both(q, k, v, begin, end, do, cap=30.0)
+    assert all(torch.equal(g, want[n]) for g, n in zip(grads, ("dq", "dk", "dv")))
+    bounds = _oracle(q, k, v, begin, end, D ** -0.5, 30.0, None, do)
+    g = torch.Generator().manual_seed(9)
+    step = [torch.randn(t.shape, generator=g, dtype=torch.float64).cuda() for t in leaves]
+
+    def at(e):
+        moved = [t.detach().double() + e * s for t, s in zip(leaves, step)]
+        return float((_oracle(*moved, begin, end, D ** -0.5, 30.0, None)["out"][0] * do.double()).sum())
+
+    expect = (at(1e-4) - at(-1e-4)) / 2e-4
+    got = float(sum((x.double() * s).sum() for x, s in zip(grads, step)))
+    room = float(sum((bounds[n][1] * s.abs()).sum() for n, s in zip(("dq", "dk", "dv"), step)))
+    assert abs(got - expect) <= room + 1e-5 * abs(expect)
+
+
+@pytest.mark.gpu
+def test_long_rows_and_large_scores(cuda_lib):
+    """Scores that grow along the row (the running maximum moves with every tile) and peak above 2^8 of the
+    first tile's."""
+    B, S, H, K, D = 1, 1500, 2, 1, 128
+    q, k, v, do = _inputs(B, S, S, H, K, D, 10, qscale=1.0)
+    k = (k.float() * torch.linspace(0.1, 12.0, S, device="cuda")[None, :, None, None]).to(torch.bfloat16)
+    begin, end = (t.cuda() for t in _ranges("all", B, S, S, 0))
+    got = _both(q, k, v, begin, end, do)
+    want = _oracle(q, k, v, begin, end, D ** -0.5, 0.0, None, do)
+    for n in got:
+        _within(n, got[n], want[n])
+
+
+def test_row_ranges():
+    from spilltune_b200.attention import row_ranges
+    begin, end = row_ranges(1, 4)
+    assert begin.tolist() == [[0, 0, 0, 0]] and end.tolist() == [[1, 2, 3, 4]]
+    assert row_ranges(1, 3, causal=False)[1].tolist() == [[3, 3, 3]]
+    docs = torch.tensor([[5, 5, 7, 7, 7, 5]])
+    begin, end = row_ranges(1, 6, documents=docs)
+    assert begin.tolist() == [[0, 0, 2, 2, 2, 5]] and end.tolist() == [[1, 2, 3, 4, 5, 6]]
+    begin, end = row_ranges(1, 6, documents=docs, causal=False)
+    assert end.tolist() == [[2, 2, 5, 5, 5, 6]]
+    begin, end = row_ranges(1, 6, documents=docs, prefix=torch.tensor([4]))
+    assert begin.tolist() == [[0, 0, 2, 2, 2, 5]] and end.tolist() == [[2, 2, 4, 4, 5, 6]]
+    begin, end = row_ranges(2, 5, window=2, lengths=torch.tensor([3, 5]))
+    assert begin.tolist() == [[0, 0, 1, 2, 3]] * 2 and end.tolist() == [[1, 2, 3, 0, 0], [1, 2, 3, 4, 5]]
+    assert all(x.dtype == torch.int32 and x.shape == (2, 0) for x in row_ranges(2, 0, documents=torch.zeros(2, 0)))
+    for bad in (dict(window=0), dict(window=3, causal=False), dict(documents=docs[:, :3]),
+                dict(prefix=torch.zeros(2)), dict(lengths=torch.zeros(2, 1))):
+        with pytest.raises(ValueError):
+            row_ranges(1, 6, **bad)
+    with pytest.raises(ValueError):
+        row_ranges(1, -1)
+
+
+def test_no_cpu_fallback():
+    from spilltune_b200 import attention
+    x = torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16)
+    r = torch.zeros(1, 4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        attention.attend(x, x, x, r, r)
+
+
+def test_c_entry_refusals():
+    """Bad arguments are refused before any launch (no GPU needed)."""
+    import ctypes
+
+    from spilltune_b200 import _lib, build
+    build.build()
+    lib = _lib.load()
+    p = 4096  # never read: each call is refused first
+    good = [64 * 4 * 2, 64 * 2, 64] * 4
+
+    def fwd(B=1, Sq=4, Sk=4, Hq=2, Hkv=2, D=64, scale=1.0, cap=0.0, strides=good, q=p, begin=p, out=p, ws=None, n=0):
+        s = (ctypes.c_int64 * 12)(*strides) if strides else None
+        return lib.fl_attn_fwd(q, p, p, s, B, Sq, Sk, Hq, Hkv, D, begin, p, scale, cap, None, out, p, ws, n, None)
+
+    def bwd(B=1, Sq=4, Sk=4, Hq=2, Hkv=2, D=64, scale=1.0, cap=0.0, strides=good, q=p, begin=p, out=p, ws=p, n=1 << 20):
+        s = (ctypes.c_int64 * 12)(*strides) if strides else None
+        return lib.fl_attn_bwd(p, q, p, p, s, out, p, B, Sq, Sk, Hq, Hkv, D, begin, p, scale, cap, None, p, p, p, ws, n,
+                               None)
+
+    bad = [dict(B=-1), dict(Sq=-1), dict(Sk=-2), dict(Hq=0), dict(Hkv=0), dict(Hq=3), dict(D=4), dict(D=68),
+           dict(D=136), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(cap=-1.0),
+           dict(cap=float("nan")), dict(strides=None), dict(strides=[12] + good[1:], B=2), dict(q=None),
+           dict(q=p + 8), dict(begin=None), dict(out=None), dict(out=p + 2),
+           dict(strides=[good[0], 0, 64] + good[3:]), dict(strides=[good[0], good[1], 36] + good[3:]),
+           dict(B=1 << 20), dict(Sq=1 << 31), dict(Hq=1 << 13, Hkv=1 << 13)]
+    for call in (fwd, bwd):
+        for b in bad:
+            assert call(**b) == _lib.FL_ERR_ARG, (call.__name__, b)
+    assert bwd(ws=None) == _lib.FL_ERR_ARG and bwd(n=16) == _lib.FL_ERR_ARG and bwd(ws=p + 4) == _lib.FL_ERR_ARG
+    long = dict(Sq=1, Sk=4096)
+    assert lib.fl_attn_fwd_workspace_bytes(1, 1, 4096, 2, 2, 64) > 0
+    assert fwd(**long) == _lib.FL_ERR_ARG and fwd(**long, ws=p, n=64) == _lib.FL_ERR_ARG
+    assert fwd(B=0) == _lib.FL_OK and fwd(Sq=0) == _lib.FL_OK and bwd(B=0) == _lib.FL_OK
+    assert lib.fl_attn_fwd_workspace_bytes(0, 1, 1, 1, 1, 64) == 0
+    assert lib.fl_attn_bwd_workspace_bytes(1, 1, 1, 3, 2, 64) == 0
+
+
+@pytest.mark.gpu
+def test_refusals(cuda_lib):
+    from spilltune_b200 import attention
+    q, k, v, do = _inputs(1, 8, 8, 4, 2, 64, 1)
+    r = torch.zeros(1, 8, dtype=torch.int32, device="cuda")
+    out, lse = attention.fwd(q, k, v, r, r + 8)
+    bad = [(lambda: attention.fwd(q.float(), k, v, r, r), "bf16"),
+           (lambda: attention.fwd(q[0], k, v, r, r), "bf16 \\[batch"),
+           (lambda: attention.fwd(q, k[..., :32], v, r, r), "do not fit"),
+           (lambda: attention.fwd(q, k, v[:, :4], r, r), "do not fit"),
+           (lambda: attention.fwd(q[:, :, :3], k, v, r, r), "share"),
+           (lambda: attention.fwd(q, k, v, r.long(), r), "begin"),
+           (lambda: attention.fwd(q, k, v, r, r[:, :4]), "end"),
+           (lambda: attention.fwd(q, k, v, r, r, scale=0.0), "scale"),
+           (lambda: attention.fwd(q, k, v, r, r, softcap=-1.0), "softcap"),
+           (lambda: attention.fwd(q, k, v, r, r, slopes=torch.ones(2, device="cuda")), "slopes"),
+           (lambda: attention.attend(q, k, v, r, r, slopes=torch.ones(4, device="cuda", requires_grad=True)),
+            "no gradient"),
+           (lambda: attention.bwd(do[:, :4], q, k, v, out, lse, r, r), "q's shape"),
+           (lambda: attention.bwd(do, q, k, v, out, lse.double(), r, r), "lse"),
+           (lambda: attention.fwd(*(torch.zeros(1, 8, 2, 136, dtype=torch.bfloat16, device="cuda"),) * 3, r, r),
+            "unsupported_capability")]
+    for call, match in bad:
+        with pytest.raises(ValueError, match=match):
+            call()
