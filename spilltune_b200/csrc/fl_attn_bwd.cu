@@ -64,7 +64,7 @@ template <int HD>
 struct Bwd {
   static constexpr int kStages = 2;
   static constexpr int kBytes = HD / 64 * kTile * 128;     // a tile of 128 rows
-  static constexpr int kSmem = 1024 + (2 + 2 * kStages) * kBytes + kStages * kInfoBytes + 256;
+  static constexpr int kSmem = 1024 + (2 + 2 * kStages) * kBytes + kStages * kInfoBytes + 512;
 };
 
 struct BwdArgs {
@@ -81,18 +81,32 @@ struct BwdArgs {
   uint32_t* status;
   int q_tiles;           // of kTile packed rows
   int tiles;             // resident tiles per head
-  int parts;             // dk, dv: CTAs that share a tile's walk
+  int64_t items;         // pieces of work: tiles, heads, sequences, parts
+  int* taken;            // items of dk and dv beyond the CTAs' first: 0 again after the dq kernel
+  int parts;             // dk, dv: items that share a tile's walk
   float* part;           // their sums [parts][dv, dk][B, Sk, Hkv, D] (parts > 1)
 };
 
+// One piece of work: a resident tile and the steps to walk.
+struct Item {
+  int tile, hg, b, part;   // tile < 0: no more work
+  int first;               // dq: first key tile; else first query tile of each head group
+  int per_group, from, n;  // dk, dv: query tiles of a group, first step; steps
+  Range seen;              // dq: of the tile's rows
+};
+
 struct __align__(16) BwdBars {
-  uint64_t a_full;
+  uint64_t item_full[2], item_empty[2];
+  uint64_t a_full, a_empty;
   uint64_t b_full[2][2], b_empty[2][2];   // [B1, B2][stage]
   uint64_t s_full, dp_full;               // S, P' written
   uint64_t p_full, ds_full;               // p, ds written over them
-  uint64_t acc1_done, acc2_done, all_done;
+  uint64_t acc1_done, acc2_done;
+  uint64_t acc_full, acc_empty;           // accumulators summed, read
+  uint64_t met;                           // dq: the element warps among themselves
+  uint64_t drained;
+  Item item[2];
   uint32_t tmem, abort_word;
-  int first, last;
 };
 
 // Dot product of 8 bf16 columns.
@@ -128,21 +142,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const Shape& s = a.s;
   const int G = s.Hq / s.Hkv, pg = 1 << s.lgp;
 
-  // The heaviest tiles of a causal mask first: early keys, late queries.
   const int heads = kDq ? s.Hkv * s.groups : s.Hkv;
-  const int per = heads * s.B * a.parts;
-  const int order = static_cast<int>(blockIdx.x) / per;
-  const int tile = kDq ? a.tiles - 1 - order : order;
-  int rest = static_cast<int>(blockIdx.x) % per;
-  const int hg = rest % heads;
-  rest /= heads;
-  const int b = rest % s.B, part = rest / s.B;
-  const int kvh = kDq ? hg / s.groups : hg;
   const int q_step = kTile >> s.lgp;                       // tokens of a query tile
-  const int row0 = kDq ? tile * q_step : tile * kTile;
+  static_assert(sizeof(BwdBars) <= 512, "the barriers' space");
 
   if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->item_full[i], 1);
+      mbar_init(&bars->item_empty[i], 1 + 4 * kGroups);
+    }
     mbar_init(&bars->a_full, 1);
+    mbar_init(&bars->a_empty, 1);
     for (int i = 0; i < C::kStages; ++i)
       for (int o = 0; o < 2; ++o) {
         mbar_init(&bars->b_full[o][i], 1);
@@ -154,11 +164,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_init(&bars->ds_full, 4 * kGroups);
     mbar_init(&bars->acc1_done, 1);
     mbar_init(&bars->acc2_done, 1);
-    mbar_init(&bars->all_done, 1);
+    mbar_init(&bars->acc_full, 1);
+    mbar_init(&bars->acc_empty, 4 * kGroups);
+    mbar_init(&bars->met, 4 * kGroups);
+    mbar_init(&bars->drained, 1);
     bars->abort_word = 0;
-    bars->first = kNone;
-    bars->last = -1;
     fence_barrier_init();
+    if (kDq && blockIdx.x == 0) *a.taken = 0;
   }
   if (warp == 1) {
     tmem_alloc(&bars->tmem, kTmemCols);
@@ -168,463 +180,560 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
-
-  // What to walk: `n` steps; dq: key tiles from `first`; else the head groups'
-  // query tiles `first` .. `first + per_group - 1` (those between that see none
-  // of the keys add nothing).
-  Range mine{};
-  int first = 0, n = 0, per_group = 0, from = 0;   // from: this part's first step
-  if constexpr (kDq) {
-    mine = tile_range(s, b, row0, q_step);
-    if (mine.min_lo < mine.max_hi) {
-      first = mine.min_lo / kTile;
-      n = (mine.max_hi + kTile - 1) / kTile - first;
-    }
-  } else {
-    int lo = kNone, hi = -1;
-    for (int i = threadIdx.x; i < a.q_tiles; i += kBwdThreads) {
-      const Range r = a.ranges[static_cast<int64_t>(b) * a.q_tiles + i];
-      if (r.min_lo < row0 + kTile && r.max_hi > row0) {
-        lo = min(lo, i);
-        hi = i;
+  // The head group and query tile of an item's step (dk, dv).
+  struct Walk {
+    int group, tile;
+    __device__ explicit Walk(const Item& it)
+        : group(it.n ? it.from / it.per_group : 0), tile(it.n ? it.first + it.from % it.per_group : 0) {}
+    __device__ void step(const Item& it) {
+      if (++tile == it.first + it.per_group) {
+        tile = it.first;
+        ++group;
       }
     }
-    if (hi >= 0) {
-      atomicMin(&bars->first, lo);
-      atomicMax(&bars->last, hi);
-    }
-    __syncthreads();
-    first = bars->first;
-    per_group = bars->last >= 0 ? bars->last - first + 1 : 0;
-    n = per_group * s.groups;
-    if (a.parts > 1) {
-      from = static_cast<int>(static_cast<int64_t>(n) * part / a.parts);
-      n = static_cast<int>(static_cast<int64_t>(n) * (part + 1) / a.parts) - from;
-    }
-  }
-  // Step i of this CTA: the head group and query tile (dk, dv).
-  auto group_of = [&](int i) { return (from + i) / per_group; };
-  auto q_tile_of = [&](int i) { return first + (from + i) % per_group; };
+  };
+  auto wait = [&](uint64_t* bar, int phase, uint32_t bit) {
+    return mbar_wait_short_warp(bar, phase & 1, abort_word, a.status, bit);
+  };
 
   if (warp == 0) {
-    if (lane == 0 && n > 0) {
+    // ------------------------------------------------------ work and loads
+    if (lane == 0) {
       tma_prefetch_desc(&tm_a1);
       tma_prefetch_desc(&tm_a2);
       tma_prefetch_desc(&tm_b1);
       tma_prefetch_desc(&tm_b2);
-      const int ah = kDq ? hg << s.lgp : kvh;
-      mbar_arrive_expect_tx(&bars->a_full, 2 * C::kBytes);
-      for (int c = 0; c < HD / 64; ++c) {
-        tma_load_4d(a1 + c * kTile * 128, &tm_a1, 64 * c, ah, row0, b, &bars->a_full);
-        tma_load_4d(a2 + c * kTile * 128, &tm_a2, 64 * c, ah, row0, b, &bars->a_full);
+    }
+    int loads_a = 0, loads_b[2] = {0, 0}, k = 0, g = 0;
+    // Heaviest tiles of a causal mask first (early keys, late queries): dq's
+    // many short items dealt out back and forth, so that every CTA gets as many
+    // early as late; those of dk and dv to whichever CTA is free.
+    auto dealt = [&](int turn) {
+      int64_t deal = blockIdx.x;
+      if constexpr (kDq) {
+        deal = static_cast<int64_t>(turn) * gridDim.x + (turn & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      } else if (turn > 0) {
+        int taken = 0;
+        if (lane == 0) taken = atomicAdd(a.taken, 1);
+        deal = static_cast<int64_t>(gridDim.x) + __shfl_sync(0xffffffffu, taken, 0);
       }
-      int done[2] = {0, 0};                        // loads issued
-      bool ok = true;
-      for (int i = 0; i < n && ok; ++i) {
-        const int st = i % C::kStages;
-        int bh, br;
+      Item it{};
+      it.tile = -1;
+      if (deal < a.items) {
+        const int per = heads * s.B * a.parts, w = static_cast<int>(deal);
+        it.tile = kDq ? a.tiles - 1 - w / per : w / per;
+        it.hg = w % per % heads;
+        it.b = w % per / heads % s.B;
+        it.part = w % per / heads / s.B;
+      }
+      return it;
+    };
+    for (int turn = 0;; ++turn) {
+      Item it = dealt(turn);
+      if (it.tile >= 0) {
         if constexpr (kDq) {
-          bh = kvh;
-          br = (first + i) * kTile;
+          it.seen = tile_range(s, it.b, it.tile * q_step, q_step);
+          if (it.seen.min_lo < it.seen.max_hi) {
+            it.first = it.seen.min_lo / kTile;
+            it.n = (it.seen.max_hi + kTile - 1) / kTile - it.first;
+          }
         } else {
-          bh = kvh * G + group_of(i) * pg;
-          br = q_tile_of(i) * q_step;
+          // The query tiles from the first to the last that see any of the keys
+          // (those between that see none add nothing).
+          int lo = kNone, hi = -1;
+          for (int i = lane; i < a.q_tiles; i += 32) {
+            const Range r = a.ranges[static_cast<int64_t>(it.b) * a.q_tiles + i];
+            if (r.min_lo < (it.tile + 1) * kTile && r.max_hi > it.tile * kTile) {
+              lo = min(lo, i);
+              hi = i;
+            }
+          }
+          lo = __reduce_min_sync(0xffffffffu, lo);
+          hi = __reduce_max_sync(0xffffffffu, hi);
+          it.first = lo;
+          it.per_group = hi >= 0 ? hi - lo + 1 : 0;
+          const int n = it.per_group * s.groups;
+          it.from = static_cast<int>(static_cast<int64_t>(n) * it.part / a.parts);
+          it.n = static_cast<int>(static_cast<int64_t>(n) * (it.part + 1) / a.parts) - it.from;
         }
+      }
+      if (turn >= 2 && !wait(&bars->item_empty[turn & 1], (turn >> 1) - 1, kStatusTimeoutEmpty)) break;
+      if (lane == 0) {
+        bars->item[turn & 1] = it;
+        mbar_arrive(&bars->item_full[turn & 1]);
+      }
+      __syncwarp();
+      if (it.tile < 0) break;
+      if (it.n == 0) continue;
+      if (k > 0 && !wait(&bars->a_empty, k - 1, kStatusTimeoutEmpty)) break;
+      const int kvh = kDq ? it.hg / s.groups : it.hg;
+      const int ah = kDq ? it.hg << s.lgp : kvh, ar = it.tile * (kDq ? q_step : kTile);
+      if (elected()) {
+        mbar_arrive_expect_tx(&bars->a_full, 2 * C::kBytes);
+        for (int c = 0; c < HD / 64; ++c) {
+          tma_load_4d(a1 + c * kTile * 128, &tm_a1, 64 * c, ah, ar, it.b, &bars->a_full);
+          tma_load_4d(a2 + c * kTile * 128, &tm_a2, 64 * c, ah, ar, it.b, &bars->a_full);
+        }
+      }
+      __syncwarp();
+      loads_a = ++k;
+      bool ok = true;
+      Walk at(it);
+      for (int i = 0; i < it.n && ok; ++i, ++g, at.step(it)) {
+        const int st = g % C::kStages;
+        const int bh = kDq ? kvh : kvh * G + at.group * pg;
+        const int br = kDq ? (it.first + i) * kTile : at.tile * q_step;
         for (int o = 0; o < 2 && ok; ++o) {
-          if (i >= C::kStages && !mbar_wait_short(&bars->b_empty[o][st], (i / C::kStages - 1) & 1, abort_word, a.status,
-                                            kStatusTimeoutEmpty)) {
+          if (g >= C::kStages && !wait(&bars->b_empty[o][st], g / C::kStages - 1, kStatusTimeoutEmpty)) {
             ok = false;
             break;
           }
-          uint8_t* dst = bs + (st * 2 + o) * C::kBytes;
-          mbar_arrive_expect_tx(&bars->b_full[o][st], C::kBytes + (!kDq && o == 0 ? kInfoBytes : 0));
-          if (!kDq && o == 0)
-            bulk_load(info + st,
-                      a.info + (static_cast<int64_t>(b) * s.Hkv * s.groups + kvh * s.groups + group_of(i)) *
-                                   a.q_tiles + q_tile_of(i),
-                      kInfoBytes, &bars->b_full[o][st]);
-          for (int c = 0; c < HD / 64; ++c)
-            tma_load_4d(dst + c * kTile * 128, o ? &tm_b2 : &tm_b1, 64 * c, bh, br, b, &bars->b_full[o][st]);
-          ++done[o];
+          if (elected()) {
+            uint8_t* dst = bs + (st * 2 + o) * C::kBytes;
+            mbar_arrive_expect_tx(&bars->b_full[o][st], C::kBytes + (!kDq && o == 0 ? kInfoBytes : 0));
+            if (!kDq && o == 0)
+              bulk_load(info + st,
+                        a.info + (static_cast<int64_t>(it.b) * s.Hkv * s.groups + kvh * s.groups + at.group) *
+                                     a.q_tiles + at.tile,
+                        kInfoBytes, &bars->b_full[o][st]);
+            for (int c = 0; c < HD / 64; ++c)
+              tma_load_4d(dst + c * kTile * 128, o ? &tm_b2 : &tm_b1, 64 * c, bh, br, it.b, &bars->b_full[o][st]);
+          }
+          __syncwarp();
+          ++loads_b[o];
         }
       }
-      // No copy may be in flight when the CTA leaves.
-      uint32_t none = 0;
-      mbar_wait(&bars->a_full, 0, &none, a.status, kStatusTimeoutDrain);
-      for (int o = 0; o < 2; ++o)
-        for (int i = max(done[o] - C::kStages, 0); i < done[o]; ++i)
-          mbar_wait(&bars->b_full[o][i % C::kStages], (i / C::kStages) & 1, &none, a.status, kStatusTimeoutDrain);
+      if (!ok) break;
     }
+    // No copy may be in flight when the CTA leaves.
+    uint32_t none = 0;
+    if (loads_a) mbar_wait(&bars->a_full, (loads_a - 1) & 1, &none, a.status, kStatusTimeoutDrain);
+    for (int o = 0; o < 2; ++o)
+      for (int i = max(loads_b[o] - C::kStages, 0); i < loads_b[o]; ++i)
+        mbar_wait(&bars->b_full[o][i % C::kStages], (i / C::kStages) & 1, &none, a.status, kStatusTimeoutDrain);
+    __syncwarp();
   } else if (warp == 1) {
+    // ------------------------------------------------------------- products
     // The whole warp walks and one lane issues: operands stay uniform, and the
     // issue takes few slots of the scheduler that the element warps share.
-    if (n > 0) {
-      const uint32_t id_s = idesc_bf16_f32(kTile, kTile), id_acc = idesc_bf16_f32_bmn(kTile, HD);
-      const uint32_t col_s = tmem, col_p = tmem + kColP;
-      const uint64_t d_a[2] = {sdesc_kmajor_sw128(smem_u32(a1)), sdesc_kmajor_sw128(smem_u32(a2))};
-      const uint64_t d_rows = sdesc_kmajor_sw128(smem_u32(bs)), d_cols = cols_desc(smem_u32(bs));
-      auto at = [&](int i, int o) { return static_cast<uint64_t>((i % C::kStages) * 2 + o) * (C::kBytes >> 4); };
-      auto wait = [&](uint64_t* bar, int phase, uint32_t bit) {
-        return mbar_wait_short_warp(bar, phase & 1, abort_word, a.status, bit);
-      };
-      // S (o = 0) or P' (o = 1) of step i.
-      auto scores = [&](int i, int o) -> bool {
-        if (!wait(&bars->b_full[o][i % C::kStages], i / C::kStages, kStatusTimeoutFull)) return false;
-        tc_fence_after();
-        if (elected()) {
-          mma_rows<HD>(o ? col_p : col_s, d_a[o], d_rows + at(i, o), id_s);
-          tc_commit(o ? &bars->dp_full : &bars->s_full);
-        }
-        __syncwarp();
-        return true;
-      };
-      bool ok = wait(&bars->a_full, 0, kStatusTimeoutFull) && scores(0, 0) && scores(0, 1);
+    const uint32_t id_s = idesc_bf16_f32(kTile, kTile), id_acc = idesc_bf16_f32_bmn(kTile, HD);
+    const uint32_t col_s = tmem, col_p = tmem + kColP;
+    const uint64_t d_a[2] = {sdesc_kmajor_sw128(smem_u32(a1)), sdesc_kmajor_sw128(smem_u32(a2))};
+    const uint64_t d_rows = sdesc_kmajor_sw128(smem_u32(bs)), d_cols = cols_desc(smem_u32(bs));
+    auto at = [&](int g, int o) { return static_cast<uint64_t>((g % C::kStages) * 2 + o) * (C::kBytes >> 4); };
+    int g0 = 0, k = 0;       // steps and items with steps before this one
+    bool issued = false;
+    // S (o = 0) or P' (o = 1) of step g, once the products that read the p or
+    // ds in its columns are done; the item's last P' frees the resident tiles.
+    auto scores = [&](int g, int o, bool last) -> bool {
+      if (g > 0 && !wait(o ? &bars->acc2_done : &bars->acc1_done, g - 1, kStatusTimeoutAccum)) return false;
+      if (!wait(&bars->b_full[o][g % C::kStages], g / C::kStages, kStatusTimeoutFull)) return false;
+      tc_fence_after();
+      if (elected()) {
+        mma_rows<HD>(o ? col_p : col_s, d_a[o], d_rows + at(g, o), id_s);
+        tc_commit(o ? &bars->dp_full : &bars->s_full);
+        if (o && last) tc_commit(&bars->a_empty);
+      }
+      __syncwarp();
+      issued = true;
+      return true;
+    };
+    bool ok = true;
+    for (int turn = 0; ok; ++turn) {
+      if (!wait(&bars->item_full[turn & 1], turn >> 1, kStatusTimeoutFull)) break;
+      const int n = bars->item[turn & 1].tile < 0 ? -1 : bars->item[turn & 1].n;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->item_empty[turn & 1]);
+      if (n < 0) break;
+      if (n == 0) continue;
+      ok = wait(&bars->a_full, k, kStatusTimeoutFull) && scores(g0, 0, false) && scores(g0, 1, n == 1);
       for (int i = 0; i < n && ok; ++i) {
-        const int st = i % C::kStages;
-        if (!wait(&bars->p_full, i, kStatusTimeoutFull)) break;
+        const int g = g0 + i, st = g % C::kStages;
+        if (!wait(&bars->p_full, g, kStatusTimeoutFull) ||
+            (i == 0 && k > 0 && !wait(&bars->acc_empty, k - 1, kStatusTimeoutAccum))) {
+          ok = false;
+          break;
+        }
         tc_fence_after();
         if (elected()) {
-          mma_cols<HD, kCols>(tmem + kColAcc, col_s, d_cols + at(i, kDq ? 0 : 1), id_acc, i > 0);
+          mma_cols<HD, kCols>(tmem + kColAcc, col_s, d_cols + at(g, kDq ? 0 : 1), id_acc, i > 0);
           tc_commit(&bars->b_empty[1][st]);
           tc_commit(&bars->acc1_done);
         }
         __syncwarp();
-        // S shares its columns with p, P' with ds: the products that read those have to be done.
-        if (i + 1 < n && !(wait(&bars->acc1_done, i, kStatusTimeoutAccum) && scores(i + 1, 0))) break;
-        if (!wait(&bars->ds_full, i, kStatusTimeoutFull)) break;
+        if (i + 1 < n && !scores(g + 1, 0, false)) ok = false;
+        if (!ok || !wait(&bars->ds_full, g, kStatusTimeoutFull)) {
+          ok = false;
+          break;
+        }
         tc_fence_after();
         if (elected()) {
-          mma_cols<HD, kCols>(tmem + kColAcc + HD, col_p, d_cols + at(i, 0), id_acc, i > 0);
+          mma_cols<HD, kCols>(tmem + kColAcc + HD, col_p, d_cols + at(g, 0), id_acc, i > 0);
           tc_commit(&bars->b_empty[0][st]);
           tc_commit(&bars->acc2_done);
+          if (i + 1 == n) tc_commit(&bars->acc_full);
         }
         __syncwarp();
-        if (i + 1 < n && !(wait(&bars->acc2_done, i, kStatusTimeoutAccum) && scores(i + 1, 1))) break;
+        if (i + 1 < n && !scores(g + 1, 1, i + 2 == n)) ok = false;
       }
-      // Completes after every product issued above, also after a wait that gave up.
-      if (elected()) tc_commit(&bars->all_done);
+      g0 += n;
+      ++k;
+    }
+    // Every product issued has to be done before the CTA leaves, also after a wait that gave up.
+    if (issued) {
+      if (elected()) tc_commit(&bars->drained);
       uint32_t none = 0;
-      mbar_wait(&bars->all_done, 0, &none, a.status, kStatusTimeoutDrain);
+      mbar_wait(&bars->drained, 0, &none, a.status, kStatusTimeoutDrain);
       __syncwarp();
     }
   } else {
+    // ------------------------------------------------------------- elements
     const int group = (warp - 2) >> 2;             // the columns this warp owns
     const int quarter = warp & 3;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const int row = quarter * 32 + lane;           // TMEM lane: the element row this thread owns
-    // dq: the row's token, head, range and statistics; else the row's key.
-    int tok = 0, head = 0, lo = 0, hi = 0;
-    float lse2 = INFINITY, d0 = 0.f;
-    uint64_t dsum2 = 0;                            // (0, 0)
     const uint64_t sl2_2 = pair(s.sl2, s.sl2);
-    const int key = row0 + row;
-    if constexpr (kDq) {
-      tok = row0 + (row >> s.lgp);
-      head = (hg << s.lgp) + (row & (pg - 1));
-      if (tok < s.Sq) {
-        row_range(s, b, tok, lo, hi);
-        const int64_t at = (static_cast<int64_t>(b) * s.Sq + tok) * s.Hq + head;
-        lse2 = a.lse[at] * kLog2e;
-      }
-      // d0 = do . o: 16 lanes to a row, two rows of a warp at a time, handed to
-      // the rows' owners through shared memory.
-      float* dots = reinterpret_cast<float*>(info + 1);
-      const int ew = warp - 2, d = (lane & 15) * 8;
-      constexpr int kRounds = kTile / (8 * kGroups);
-      uint4 x[kRounds], y[kRounds];
-#pragma unroll
-      for (int i = 0; i < kRounds; ++i) {
-        const int rr = ew * 2 * kRounds + 2 * i + (lane >> 4);
-        const int64_t rt = row0 + (rr >> s.lgp), rh = (hg << s.lgp) + (rr & (pg - 1));
-        x[i] = y[i] = make_uint4(0, 0, 0, 0);
-        if (rt < s.Sq && d < s.D) {
-          x[i] = *reinterpret_cast<const uint4*>(a.dout + b * a.do_batch + rt * a.do_token + rh * a.do_head + d);
-          y[i] = *reinterpret_cast<const uint4*>(
-              a.out + ((static_cast<int64_t>(b) * s.Sq + rt) * s.Hq + rh) * s.D + d);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kRounds; ++i) {
-        float sum = dot8(x[i], y[i]);
-#pragma unroll
-        for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if ((lane & 15) == 0) dots[ew * 2 * kRounds + 2 * i + (lane >> 4)] = sum;
-      }
-      named_barrier_sync(1, 128 * kGroups);
-      d0 = dots[row];
-    }
-    const float row_slope2 = kDq && kBias && s.slopes ? s.slopes[head] * kLog2e : 0.f;
-    bool ok = true;
-    for (int i = 0; i < n; ++i) {
-      const int st = i % C::kStages;
-      const RowInfo& cols = info[st];              // dk, dv: of the step's columns
-      const int mine0 = group * kCols;             // the first of the group's columns
-      bool whole;
-      int col0, h_first = 0;                       // dq: first key; else first token and head
-      if (!kDq && !mbar_wait_short_warp(&bars->b_full[0][st], (i / C::kStages) & 1, abort_word, a.status,
-                                        kStatusTimeoutFull)) {
-        ok = false;
-        break;
-      }
-      if constexpr (kDq) {
-        col0 = (first + i) * kTile + mine0;
-        whole = mine.max_lo <= col0 && mine.min_hi >= col0 + kCols;
-      } else {
-        col0 = q_tile_of(i) * q_step + (mine0 >> s.lgp);
-        h_first = kvh * G + group_of(i) * pg;
-        whole = cols.max_lo[group] <= row0 && cols.min_hi[group] >= row0 + kTile;
-      }
-      [[maybe_unused]] uint64_t nl_of[kDq ? 1 : kCols / 2];   // dk, dv: -lse2 of the columns
-      if constexpr (!kDq && !kBias) {
-#pragma unroll
-        for (int c = 0; c < kCols; c += 4) {
-          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(cols.nlse2 + mine0 + c);
-          nl_of[c / 2] = v.x, nl_of[c / 2 + 1] = v.y;
-        }
-      }
-      if (!mbar_wait_short_warp(&bars->s_full, i & 1, abort_word, a.status, kStatusTimeoutAccum)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      const uint32_t at_s = tmem + kCols * group + lanes, at_p = at_s + kColP;
-      uint32_t x[kCols], w[kCols / 2];             // scores, then p; packed operands
-      [[maybe_unused]] __half2 fac[kBias ? kCols / 2 : 1];
-      tmem_ld_32x32b_x32(at_s, x);
-      tmem_wait_ld();
-      // Which of the columns c .. c + 3 the row does not see.
-      auto hidden = [&](int c, bool (&hide)[4]) {
-        if constexpr (kDq) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) hide[e] = c + e < lo - col0 || c + e >= hi - col0;
-        } else {
-          const int4 u = *reinterpret_cast<const int4*>(cols.lo + mine0 + c);
-          const int4 v = *reinterpret_cast<const int4*>(cols.hi + mine0 + c);
-          hide[0] = key < u.x || key >= v.x;
-          hide[1] = key < u.y || key >= v.y;
-          hide[2] = key < u.z || key >= v.z;
-          hide[3] = key < u.w || key >= v.w;
-        }
-      };
-      auto exponentials = [&](int c, auto masked) {
-        uint64_t nl[2];                            // -lse2 of the columns
-        if constexpr (kDq) {
-          nl[0] = nl[1] = pair(-lse2, -lse2);
-        } else if constexpr (kBias) {
-          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(cols.nlse2 + mine0 + c);
-          nl[0] = v.x, nl[1] = v.y;
-        } else {
-          nl[0] = nl_of[c / 2], nl[1] = nl_of[c / 2 + 1];
-        }
-        float p[4];
-        [[maybe_unused]] float f[4];
-        if constexpr (kBias) {
-          float l[4];
-          unpair(nl[0], l[0], l[1]);
-          unpair(nl[1], l[2], l[3]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int col = c + e;
-            const int at = kDq ? tok : col0 + (col >> s.lgp), k_at = kDq ? col0 + col : key;
-            const float slope2 = kDq ? row_slope2 : (s.slopes ? s.slopes[h_first + (col & (pg - 1))] * kLog2e : 0.f);
-            float th;
-            p[e] = ex2(score2(s, __uint_as_float(x[col]), slope2, at + s.Sk - s.Sq - k_at, th) + l[e]);
-            f[e] = 1.0f - th * th;
-          }
-        } else {
-#pragma unroll
-          for (int h = 0; h < 4; h += 2) {
-            unpair(fma2(pair(x[c + h], x[c + h + 1]), sl2_2, nl[h / 2]), p[h], p[h + 1]);
-            if (h == 0 && c % 8 == 0) {            // a quarter of the exponentials
-              ex2_pair(p[h], p[h + 1], p[h], p[h + 1]);
-            } else {
-              p[h] = ex2(p[h]);
-              p[h + 1] = ex2(p[h + 1]);
-            }
-          }
-        }
-        if constexpr (decltype(masked)::value) {
-          bool hide[4];
-          hidden(c, hide);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (hide[e]) p[e] = 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[c + e] = __float_as_uint(p[e]);
-        if constexpr (kBias) {
-          // f waits for dp in 16 bits: 2^-12 of a factor of ds, an eighth of ds's own rounding.
-          fac[c / 2] = __floats2half2_rn(f[0], f[1]);
-          fac[c / 2 + 1] = __floats2half2_rn(f[2], f[3]);
-          if constexpr (kDq) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p[e] *= f[e];
-          }
-        }
-        w[c / 2] = pack_bf16x2(p[0], p[1]);
-        w[c / 2 + 1] = pack_bf16x2(p[2], p[3]);
-      };
-      if (whole) {
-#pragma unroll
-        for (int c = 0; c < kCols; c += 4) exponentials(c, std::false_type{});
-      } else {
-#pragma unroll
-        for (int c = 0; c < kCols; c += 4) exponentials(c, std::true_type{});
-      }
-      tmem_st_32x32b_x16(at_s, w);
-      tmem_wait_st();
-      tc_fence_before();
+    const int mine0 = group * kCols;               // the first of the group's columns
+    int g0 = 0, k = 0, meetings = 0;
+    // A barrier of the element warps that gives up as every other wait does.
+    auto meet = [&]() -> bool {
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->p_full);
-
-      if (!mbar_wait_short_warp(&bars->dp_full, i & 1, abort_word, a.status, kStatusTimeoutAccum)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      // dp of the columns c .. c + 3 in y; ds into w.
-      auto gradients = [&](const uint32_t* y, int c, auto masked) {
-        uint64_t nd[2];                            // -delta of the columns
-        if constexpr (kDq) {
-          nd[0] = nd[1] = pair(-d0, -d0);
-        } else {
-          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(cols.ndelta + mine0 + c);
-          nd[0] = v.x, nd[1] = v.y;
-        }
-        [[maybe_unused]] bool hide[4];
-        if constexpr (decltype(masked)::value) hidden(c, hide);
+      if (lane == 0) mbar_arrive(&bars->met);
+      return wait(&bars->met, meetings++, kStatusTimeoutAccum);
+    };
+    for (int turn = 0;; ++turn) {
+      if (!wait(&bars->item_full[turn & 1], turn >> 1, kStatusTimeoutFull)) break;
+      const Item it = bars->item[turn & 1];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->item_empty[turn & 1]);
+      if (it.tile < 0) break;
+      const int kvh = kDq ? it.hg / s.groups : it.hg, b = it.b;
+      const int row0 = it.tile * (kDq ? q_step : kTile);
+      // dq: the row's token, head, range and statistics; else the row's key.
+      int tok = 0, head = 0, lo = 0, hi = 0;
+      float lse2 = INFINITY, d0 = 0.f;
+      uint64_t dsum2 = 0;                          // (0, 0)
+      const int key = row0 + row;
+      if constexpr (kDq) {
+        tok = row0 + (row >> s.lgp);
+        head = (it.hg << s.lgp) + (row & (pg - 1));
+        // Every load first, from the last row where there is none: one latency, not four.
+        const int last = s.Sq - 1;
+        const int64_t at = static_cast<int64_t>(b) * s.Sq + min(tok, last);
+        const int begin = s.begin[at], end = s.end[at];
+        const float lse = a.lse[at * s.Hq + head];
+        // d0 = do . o: 16 lanes to a row, two rows of a warp at a time, handed to
+        // the rows' owners through shared memory.
+        float* dots = reinterpret_cast<float*>(info + 1) + (turn & 1) * kTile;
+        const bool in_row = (lane & 15) * 8 < s.D;
+        const int d = in_row ? (lane & 15) * 8 : 0;
+        constexpr int kRounds = kTile / (8 * kGroups);
+        uint4 x[kRounds], y[kRounds];
 #pragma unroll
-        for (int h = 0; h < 4; h += 2) {
-          const int col = c + h;
-          const uint64_t dp = pair(y[h], y[h + 1]), p = pair(x[col], x[col + 1]);
+        for (int i = 0; i < kRounds; ++i) {
+          const int rr = ((warp - 2) * kRounds + i) * 2 + (lane >> 4);
+          const int rt = min(row0 + (rr >> s.lgp), last), rh = (it.hg << s.lgp) + (rr & (pg - 1));
+          x[i] = *reinterpret_cast<const uint4*>(a.dout + b * a.do_batch + rt * a.do_token + rh * a.do_head + d);
+          y[i] = *reinterpret_cast<const uint4*>(a.out + ((static_cast<int64_t>(b) * s.Sq + rt) * s.Hq + rh) * s.D + d);
+        }
+        if (tok < s.Sq) {
+          lo = max(begin, 0);
+          hi = min(end, s.Sk);
+          if (lo >= hi) lo = hi = 0;
+          lse2 = lse * kLog2e;
+        }
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i) {
+          float sum = in_row ? dot8(x[i], y[i]) : 0.f;
+#pragma unroll
+          for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          if ((lane & 15) == 0) dots[((warp - 2) * kRounds + i) * 2 + (lane >> 4)] = sum;
+        }
+        if (!meet()) break;
+        d0 = dots[row];
+      }
+      const float row_slope2 = kDq && kBias && s.slopes ? s.slopes[head] * kLog2e : 0.f;
+      bool ok = true;
+      Walk at(it);
+      for (int i = 0; i < it.n; ++i, at.step(it)) {
+        const int g = g0 + i, st = g % C::kStages;
+        const RowInfo& cols = info[st];              // dk, dv: of the step's columns
+        bool whole;
+        int col0, h_first = 0;                       // dq: first key; else first token and head
+        if (!kDq && !wait(&bars->b_full[0][st], g / C::kStages, kStatusTimeoutFull)) {
+          ok = false;
+          break;
+        }
+        if constexpr (kDq) {
+          col0 = (it.first + i) * kTile + mine0;
+          whole = it.seen.max_lo <= col0 && it.seen.min_hi >= col0 + kCols;
+        } else {
+          col0 = at.tile * q_step + (mine0 >> s.lgp);
+          h_first = kvh * G + at.group * pg;
+          whole = cols.max_lo[group] <= row0 && cols.min_hi[group] >= row0 + kTile;
+        }
+        [[maybe_unused]] uint64_t nl_of[kDq ? 1 : kCols / 2];   // dk, dv: -lse2 of the columns
+        if constexpr (!kDq && !kBias) {
+#pragma unroll
+          for (int c = 0; c < kCols; c += 4) {
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(cols.nlse2 + mine0 + c);
+            nl_of[c / 2] = v.x, nl_of[c / 2 + 1] = v.y;
+          }
+        }
+        if (!wait(&bars->s_full, g, kStatusTimeoutAccum)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t at_s = tmem + kCols * group + lanes, at_p = at_s + kColP;
+        uint32_t x[kCols], w[kCols / 2];             // scores, then p; packed operands
+        [[maybe_unused]] __half2 fac[kBias ? kCols / 2 : 1];
+        tmem_ld_32x32b_x32(at_s, x);
+        tmem_wait_ld();
+        // Which of the columns c .. c + 3 the row does not see.
+        auto hidden = [&](int c, bool (&hide)[4]) {
           if constexpr (kDq) {
-            if constexpr (decltype(masked)::value) {
-              // p is 0 at a hidden key, but whatever its value makes of dp may not be finite
-              float d_0, d_1;
-              unpair(mul2(p, dp), d_0, d_1);
-              dsum2 = add2(dsum2, pair(hide[h] ? 0.f : d_0, hide[h + 1] ? 0.f : d_1));
-            } else {
-              dsum2 = fma2(p, dp, dsum2);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hide[e] = c + e < lo - col0 || c + e >= hi - col0;
+          } else {
+            const int4 u = *reinterpret_cast<const int4*>(cols.lo + mine0 + c);
+            const int4 v = *reinterpret_cast<const int4*>(cols.hi + mine0 + c);
+            hide[0] = key < u.x || key >= v.x;
+            hide[1] = key < u.y || key >= v.y;
+            hide[2] = key < u.z || key >= v.z;
+            hide[3] = key < u.w || key >= v.w;
+          }
+        };
+        auto exponentials = [&](int c, auto masked) {
+          uint64_t nl[2];                            // -lse2 of the columns
+          if constexpr (kDq) {
+            nl[0] = nl[1] = pair(-lse2, -lse2);
+          } else if constexpr (kBias) {
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(cols.nlse2 + mine0 + c);
+            nl[0] = v.x, nl[1] = v.y;
+          } else {
+            nl[0] = nl_of[c / 2], nl[1] = nl_of[c / 2 + 1];
+          }
+          float p[4];
+          [[maybe_unused]] float f[4];
+          if constexpr (kBias) {
+            float l[4];
+            unpair(nl[0], l[0], l[1]);
+            unpair(nl[1], l[2], l[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int col = c + e;
+              const int at = kDq ? tok : col0 + (col >> s.lgp), k_at = kDq ? col0 + col : key;
+              const float slope2 = kDq ? row_slope2 : (s.slopes ? s.slopes[h_first + (col & (pg - 1))] * kLog2e : 0.f);
+              float th;
+              p[e] = ex2(score2(s, __uint_as_float(x[col]), slope2, at + s.Sk - s.Sq - k_at, th) + l[e]);
+              f[e] = 1.0f - th * th;
+            }
+          } else {
+#pragma unroll
+            for (int h = 0; h < 4; h += 2) {
+              unpair(fma2(pair(x[c + h], x[c + h + 1]), sl2_2, nl[h / 2]), p[h], p[h + 1]);
+              if (h == 0 && c % 8 == 0) {            // a quarter of the exponentials
+                ex2_pair(p[h], p[h + 1], p[h], p[h + 1]);
+              } else {
+                p[h] = ex2(p[h]);
+                p[h + 1] = ex2(p[h + 1]);
+              }
             }
           }
-          uint64_t pf = p;
-          if constexpr (kBias) {
-            const float2 f = __half22float2(fac[col / 2]);
-            pf = mul2(p, pair(f.x, f.y));
-          }
-          float ds[2];
-          unpair(mul2(pf, add2(dp, nd[h / 2])), ds[0], ds[1]);
           if constexpr (decltype(masked)::value) {
-            if (hide[h]) ds[0] = 0.f;
-            if (hide[h + 1]) ds[1] = 0.f;
-          }
-          w[col / 2] = pack_bf16x2(ds[0], ds[1]);
-        }
-      };
+            bool hide[4];
+            hidden(c, hide);
 #pragma unroll
-      for (int c0 = 0; c0 < kCols; c0 += 16) {
-        uint32_t y[16];
-        tmem_ld_32x32b_x16(at_p + c0, y);
-        tmem_wait_ld();
+            for (int e = 0; e < 4; ++e)
+              if (hide[e]) p[e] = 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[c + e] = __float_as_uint(p[e]);
+          if constexpr (kBias) {
+            // f waits for dp in 16 bits: 2^-12 of a factor of ds, an eighth of ds's own rounding.
+            fac[c / 2] = __floats2half2_rn(f[0], f[1]);
+            fac[c / 2 + 1] = __floats2half2_rn(f[2], f[3]);
+            if constexpr (kDq) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) p[e] *= f[e];
+            }
+          }
+          w[c / 2] = pack_bf16x2(p[0], p[1]);
+          w[c / 2 + 1] = pack_bf16x2(p[2], p[3]);
+        };
         if (whole) {
 #pragma unroll
-          for (int c = 0; c < 16; c += 4) gradients(y + c, c0 + c, std::false_type{});
+          for (int c = 0; c < kCols; c += 4) exponentials(c, std::false_type{});
         } else {
 #pragma unroll
-          for (int c = 0; c < 16; c += 4) gradients(y + c, c0 + c, std::true_type{});
+          for (int c = 0; c < kCols; c += 4) exponentials(c, std::true_type{});
         }
-      }
-      tmem_st_32x32b_x16(at_p, w);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->ds_full);
-    }
-    float fix = 0.f;
-    if constexpr (kDq) {
-      // Each group summed delta over its columns.
-      float dsum, odd;
-      unpair(dsum2, dsum, odd);
-      float* sums = reinterpret_cast<float*>(info);   // [kGroups][128]
-      static_assert(kGroups * kTile * sizeof(float) <= kInfoBytes, "the sums use the first row info's space");
-      sums[group * kTile + row] = dsum + odd;
-      named_barrier_sync(1, 128 * kGroups);
-      dsum = 0.f;
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) dsum += sums[g * kTile + row];
-      fix = d0 - dsum;
-      RowInfo* o = a.info + (static_cast<int64_t>(b) * heads + hg) * a.q_tiles + tile;
-      if (group == 0) {
-        o->nlse2[row] = tok < s.Sq ? -lse2 : -INFINITY;
-        o->ndelta[row] = tok < s.Sq ? -dsum : 0.f;
-      } else if (group == 1) {
-        o->lo[row] = lo;
-        o->hi[row] = hi;
-      }
-      if (quarter == 0) {
-        const Range h = tile_range(s, b, row0 + ((group * kCols) >> s.lgp), max(kCols >> s.lgp, 1));
-        if (lane == 0) {
-          o->max_lo[group] = h.max_lo;
-          o->min_hi[group] = h.min_hi;
-          if (hg == 0 && group == 0) a.ranges[static_cast<int64_t>(b) * a.q_tiles + tile] = mine;
+        tmem_st_32x32b_x16(at_s, w);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->p_full);
+
+        if (!wait(&bars->dp_full, g, kStatusTimeoutAccum)) {
+          ok = false;
+          break;
         }
-      }
-    }
-    if (n > 0 && !mbar_wait_short_warp(&bars->all_done, 0, abort_word, a.status, kStatusTimeoutAccum)) ok = false;
-    tc_fence_after();
-    if (ok) {
-      // dq: each group stores a quarter of the columns; else two store the
-      // halves of dv, two those of dk.
-      const bool live = kDq ? tok < s.Sq : key < s.Sk;
-      const bool second = kDq || group >= kGroups / 2;   // of the accumulators
-      __nv_bfloat16* o;
-      if constexpr (kDq)
-        o = a.dq + ((static_cast<int64_t>(b) * s.Sq + tok) * s.Hq + head) * s.D;
-      else
-        o = (second ? a.dk : a.dv) + ((static_cast<int64_t>(b) * s.Sk + key) * s.Hkv + kvh) * s.D;
-      const float by = second ? s.scale : 1.0f;
-      constexpr int kWidth = kDq ? HD / kGroups : HD / (kGroups / 2);
-      const int c_from = (kDq ? group : group & 1) * kWidth;
-#pragma unroll 1
-      for (int c = c_from; c < c_from + kWidth; c += 16) {
-        uint32_t v[16];
-        if (n > 0) {
-          tmem_ld_32x32b_x16(tmem + kColAcc + (second ? HD : 0) + lanes + c, v);
+        tc_fence_after();
+        // dp of the columns c .. c + 3 in y; ds into w.
+        auto gradients = [&](const uint32_t* y, int c, auto masked) {
+          uint64_t nd[2];                            // -delta of the columns
           if constexpr (kDq) {
-            uint32_t u[16];
-            tmem_ld_32x32b_x16(tmem + kColAcc + lanes + c, u);
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              v[e] = __float_as_uint(fmaf(fix, __uint_as_float(u[e]), __uint_as_float(v[e])));
+            nd[0] = nd[1] = pair(-d0, -d0);
           } else {
-            tmem_wait_ld();
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(cols.ndelta + mine0 + c);
+            nd[0] = v.x, nd[1] = v.y;
           }
-        } else {
+          [[maybe_unused]] bool hide[4];
+          if constexpr (decltype(masked)::value) hidden(c, hide);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] = 0u;
-        }
-        if (!live) continue;
-        if (!kDq && a.parts > 1) {
-          const int64_t rows = static_cast<int64_t>(s.B) * s.Sk * s.Hkv;
-          float* f = a.part + ((part * 2 + second) * rows + (static_cast<int64_t>(b) * s.Sk + key) * s.Hkv + kvh) * s.D + c;
-#pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            if (c + e < s.D)
-              *reinterpret_cast<float4*>(f + e) =
-                  make_float4(__uint_as_float(v[e]) * by, __uint_as_float(v[e + 1]) * by,
-                              __uint_as_float(v[e + 2]) * by, __uint_as_float(v[e + 3]) * by);
-          continue;
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (c + 8 * e < s.D) {
-            uint32_t u[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              u[q] = pack_bf16x2(__uint_as_float(v[8 * e + 2 * q]) * by, __uint_as_float(v[8 * e + 2 * q + 1]) * by);
-            *reinterpret_cast<uint4*>(o + c + 8 * e) = make_uint4(u[0], u[1], u[2], u[3]);
+          for (int h = 0; h < 4; h += 2) {
+            const int col = c + h;
+            const uint64_t dp = pair(y[h], y[h + 1]), p = pair(x[col], x[col + 1]);
+            if constexpr (kDq) {
+              if constexpr (decltype(masked)::value) {
+                // p is 0 at a hidden key, but whatever its value makes of dp may not be finite
+                float d_0, d_1;
+                unpair(mul2(p, dp), d_0, d_1);
+                dsum2 = add2(dsum2, pair(hide[h] ? 0.f : d_0, hide[h + 1] ? 0.f : d_1));
+              } else {
+                dsum2 = fma2(p, dp, dsum2);
+              }
+            }
+            uint64_t pf = p;
+            if constexpr (kBias) {
+              const float2 f = __half22float2(fac[col / 2]);
+              pf = mul2(p, pair(f.x, f.y));
+            }
+            float ds[2];
+            unpair(mul2(pf, add2(dp, nd[h / 2])), ds[0], ds[1]);
+            if constexpr (decltype(masked)::value) {
+              if (hide[h]) ds[0] = 0.f;
+              if (hide[h + 1]) ds[1] = 0.f;
+            }
+            w[col / 2] = pack_bf16x2(ds[0], ds[1]);
           }
+        };
+#pragma unroll
+        for (int c0 = 0; c0 < kCols; c0 += 16) {
+          uint32_t y[16];
+          tmem_ld_32x32b_x16(at_p + c0, y);
+          tmem_wait_ld();
+          if (whole) {
+#pragma unroll
+            for (int c = 0; c < 16; c += 4) gradients(y + c, c0 + c, std::false_type{});
+          } else {
+#pragma unroll
+            for (int c = 0; c < 16; c += 4) gradients(y + c, c0 + c, std::true_type{});
+          }
+        }
+        tmem_st_32x32b_x16(at_p, w);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->ds_full);
+      }
+      g0 += it.n;
+      float fix = 0.f;
+      if constexpr (kDq) {
+        // Each group summed delta over its columns.
+        float dsum, odd;
+        unpair(dsum2, dsum, odd);
+        float* sums = reinterpret_cast<float*>(info);   // [kGroups][128]
+        static_assert(kGroups * kTile * sizeof(float) <= kInfoBytes, "the sums use the first row info's space");
+        sums[group * kTile + row] = dsum + odd;
+        if (!ok || !meet()) break;
+        dsum = 0.f;
+#pragma unroll
+        for (int q = 0; q < kGroups; ++q) dsum += sums[q * kTile + row];
+        fix = d0 - dsum;
+        RowInfo* o = a.info + (static_cast<int64_t>(b) * heads + it.hg) * a.q_tiles + it.tile;
+        if (group == 0) {
+          o->nlse2[row] = tok < s.Sq ? -lse2 : -INFINITY;
+          o->ndelta[row] = tok < s.Sq ? -dsum : 0.f;
+        } else if (group == 1) {
+          o->lo[row] = lo;
+          o->hi[row] = hi;
+        }
+        if (quarter == 0) {
+          const Range h = tile_range(s, b, row0 + (mine0 >> s.lgp), max(kCols >> s.lgp, 1));
+          if (lane == 0) {
+            o->max_lo[group] = h.max_lo;
+            o->min_hi[group] = h.min_hi;
+            if (it.hg == 0 && group == 0) a.ranges[static_cast<int64_t>(b) * a.q_tiles + it.tile] = it.seen;
+          }
+        }
+      }
+      if (it.n > 0) {
+        ok = ok && wait(&bars->acc_full, k, kStatusTimeoutAccum);
+        ++k;
+      }
+      tc_fence_after();
+      if (ok) {
+        // dq: each group stores a quarter of the columns; else two store the
+        // halves of dv, two those of dk.
+        const bool live = kDq ? tok < s.Sq : key < s.Sk;
+        const bool second = kDq || group >= kGroups / 2;   // of the accumulators
+        __nv_bfloat16* o;
+        if constexpr (kDq)
+          o = a.dq + ((static_cast<int64_t>(b) * s.Sq + tok) * s.Hq + head) * s.D;
+        else
+          o = (second ? a.dk : a.dv) + ((static_cast<int64_t>(b) * s.Sk + key) * s.Hkv + kvh) * s.D;
+        const float by = second ? s.scale : 1.0f;
+        constexpr int kWidth = kDq ? HD / kGroups : HD / (kGroups / 2);
+        const int c_from = (kDq ? group : group & 1) * kWidth;
+#pragma unroll 1
+        for (int c = c_from; c < c_from + kWidth; c += 16) {
+          uint32_t v[16];
+          if (it.n > 0) {
+            tmem_ld_32x32b_x16(tmem + kColAcc + (second ? HD : 0) + lanes + c, v);
+            if constexpr (kDq) {
+              uint32_t u[16];
+              tmem_ld_32x32b_x16(tmem + kColAcc + lanes + c, u);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                v[e] = __float_as_uint(fmaf(fix, __uint_as_float(u[e]), __uint_as_float(v[e])));
+            } else {
+              tmem_wait_ld();
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = 0u;
+          }
+          if (!live) continue;
+          if (!kDq && a.parts > 1) {
+            const int64_t rows = static_cast<int64_t>(s.B) * s.Sk * s.Hkv;
+            float* f = a.part + ((it.part * 2 + second) * rows + (static_cast<int64_t>(b) * s.Sk + key) * s.Hkv + kvh) * s.D + c;
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              if (c + e < s.D)
+                *reinterpret_cast<float4*>(f + e) =
+                    make_float4(__uint_as_float(v[e]) * by, __uint_as_float(v[e + 1]) * by,
+                                __uint_as_float(v[e + 2]) * by, __uint_as_float(v[e + 3]) * by);
+            continue;
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (c + 8 * e < s.D) {
+              uint32_t u[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                u[q] = pack_bf16x2(__uint_as_float(v[8 * e + 2 * q]) * by, __uint_as_float(v[8 * e + 2 * q + 1]) * by);
+              *reinterpret_cast<uint4*>(o + c + 8 * e) = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+        }
+      }
+      if (!ok) break;
+      if (it.n > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->acc_empty);
       }
     }
   }
@@ -663,11 +772,20 @@ int bwd_parts(int64_t key_ctas, int64_t steps) {
   return n < 1 ? 1 : static_cast<int>(n);
 }
 
+int device_sms() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;
+  return n;
+}
+
 template <int HD, bool kDq, bool kBias>
 int launch_bwd(const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1, const CUtensorMap& b2,
-               const BwdArgs& a, int64_t grid, cudaStream_t stream) {
+               const BwdArgs& a, cudaStream_t stream) {
   int rc = allow_smem(reinterpret_cast<const void*>(&bwd_kernel<HD, kDq, kBias>), Bwd<HD>::kSmem);
   if (rc) return rc;
+  const int64_t grid = a.items < device_sms() ? a.items : device_sms();
   bwd_kernel<HD, kDq, kBias><<<static_cast<unsigned>(grid), kBwdThreads, Bwd<HD>::kSmem, stream>>>(a1, a2, b1, b2, a);
   return FL_OK;
 }
@@ -681,12 +799,13 @@ using namespace fl;
 
 extern "C" {
 
-// The query tiles' row statistics, then their ranges, then the parts' sums.
+// The query tiles' row statistics, then their ranges, the count of items taken,
+// and the parts' sums.
 static size_t attn_bwd_sizes(int64_t B, int64_t Sq, int64_t Sk, int Hq, int Hkv, int D, int* parts, size_t* part_at) {
   const int lgp = attn::packed_log2(Hq, Hkv);
   const int64_t q_tiles = attn::q_tiles_of(Sq, lgp), key_tiles = (Sk + attn::kTile - 1) / attn::kTile;
   *parts = attn::bwd_parts(key_tiles * B * Hkv, q_tiles * ((Hq / Hkv) >> lgp));
-  *part_at = static_cast<size_t>(B) * q_tiles * ((Hq >> lgp) * sizeof(attn::RowInfo) + sizeof(attn::Range));
+  *part_at = static_cast<size_t>(B) * q_tiles * ((Hq >> lgp) * sizeof(attn::RowInfo) + sizeof(attn::Range)) + 16;
   return *part_at + (*parts > 1 ? static_cast<size_t>(*parts) * 2 * B * Sk * Hkv * D * sizeof(float) : 0);
 }
 
@@ -735,6 +854,7 @@ int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, cons
   a.q_tiles = static_cast<int>(attn::q_tiles_of(Sq, a.s.lgp));
   a.info = static_cast<attn::RowInfo*>(workspace);
   a.ranges = reinterpret_cast<attn::Range*>(a.info + B * (Hq >> a.s.lgp) * a.q_tiles);
+  a.taken = reinterpret_cast<int*>(a.ranges + B * a.q_tiles);
   a.out = reinterpret_cast<const __nv_bfloat16*>(out);
   a.dout = reinterpret_cast<const __nv_bfloat16*>(dout);
   a.do_batch = strides[9];
@@ -756,22 +876,22 @@ int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, cons
       (rc = attn_map(&mdo, dout, strides[9], strides[10], strides[11], b, sq, Hq, D, pg, q_step)))
     return rc;
   const bool bias = softcap != 0.f || slopes;
-  const int64_t q_grid = attn::fwd_ctas(b, sq, Hq, Hkv);
+  a.items = attn::fwd_ctas(b, sq, Hq, Hkv);
   a.parts = 1;
-  a.tiles = static_cast<int>(q_grid / B / (Hq >> a.s.lgp));
-  rc = D <= 64 ? (bias ? attn::launch_bwd<64, true, true>(mq, mdo, mk, mv, a, q_grid, st)
-                       : attn::launch_bwd<64, true, false>(mq, mdo, mk, mv, a, q_grid, st))
-               : (bias ? attn::launch_bwd<128, true, true>(mq, mdo, mk, mv, a, q_grid, st)
-                       : attn::launch_bwd<128, true, false>(mq, mdo, mk, mv, a, q_grid, st));
+  a.tiles = static_cast<int>(a.items / B / (Hq >> a.s.lgp));
+  rc = D <= 64 ? (bias ? attn::launch_bwd<64, true, true>(mq, mdo, mk, mv, a, st)
+                       : attn::launch_bwd<64, true, false>(mq, mdo, mk, mv, a, st))
+               : (bias ? attn::launch_bwd<128, true, true>(mq, mdo, mk, mv, a, st)
+                       : attn::launch_bwd<128, true, false>(mq, mdo, mk, mv, a, st));
   if (rc) return rc;
   a.tiles = static_cast<int>(key_tiles);
   a.parts = parts;
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + part_at);
-  const int64_t kv_grid = key_tiles * B * Hkv * parts;
-  rc = D <= 64 ? (bias ? attn::launch_bwd<64, false, true>(mk, mv, mq, mdo, a, kv_grid, st)
-                       : attn::launch_bwd<64, false, false>(mk, mv, mq, mdo, a, kv_grid, st))
-               : (bias ? attn::launch_bwd<128, false, true>(mk, mv, mq, mdo, a, kv_grid, st)
-                       : attn::launch_bwd<128, false, false>(mk, mv, mq, mdo, a, kv_grid, st));
+  a.items = key_tiles * B * Hkv * parts;
+  rc = D <= 64 ? (bias ? attn::launch_bwd<64, false, true>(mk, mv, mq, mdo, a, st)
+                       : attn::launch_bwd<64, false, false>(mk, mv, mq, mdo, a, st))
+               : (bias ? attn::launch_bwd<128, false, true>(mk, mv, mq, mdo, a, st)
+                       : attn::launch_bwd<128, false, false>(mk, mv, mq, mdo, a, st));
   if (rc) return rc;
   if (parts > 1) {
     const int64_t n4 = B * Sk * Hkv * D / 4;
