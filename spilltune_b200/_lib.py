@@ -94,6 +94,12 @@ def load(path=None):
         return lib
 
 
+def function(name):
+    """The entry point `name` of the loaded library, for calls whose own cost counts
+    (``check`` its status)."""
+    return getattr(_lib if _lib is not None else load(), name)
+
+
 def check(code, what=""):
     if code != FL_OK:
         msg = load().fl_last_error().decode(errors="replace")

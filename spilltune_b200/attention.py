@@ -68,18 +68,17 @@ def row_ranges(batch, length, *, documents=None, prefix=None, window=None, lengt
 
 def _view(x):
     """x where the kernels can read it in place (adjacent columns, 16-byte rows, real strides), else a copy."""
-    st, sh = x.stride(), x.shape
-    if st[3] == 1 and x.data_ptr() % 16 == 0:
-        for i in (0, 1, 2):
-            if sh[i] > 1 and (st[i] <= 0 or st[i] % 8):
-                break
-        else:
-            return x
+    a, b, c, d = x.stride()
+    if d == 1 and a > 0 and b > 0 and c > 0 and not (a | b | c) & 7 and not x.data_ptr() & 15:
+        return x
+    sh, st = x.shape, (a, b, c)
+    if d == 1 and not x.data_ptr() & 15 and all(sh[i] == 1 or (st[i] > 0 and st[i] % 8 == 0) for i in (0, 1, 2)):
+        return x
     return x.clone(memory_format=torch.contiguous_format)
 
 
 def _check(q, k, v, begin, end, scale, softcap, slopes):
-    _need_cuda(q, k, v, begin, end, slopes)
+    _need_cuda(q, k, v, begin, end)
     bf16 = torch.bfloat16
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4 or t.dtype != bf16:
@@ -133,12 +132,12 @@ def fwd(q, k, v, begin, end, *, scale=None, softcap=0.0, slopes=None):
     begin, end = begin.contiguous(), end.contiguous()
     if slopes is not None:
         slopes = slopes.contiguous()
-    with on_device(dev):
-        n = _lib.load().fl_attn_fwd_workspace_bytes(B, Sq, Sk, Hq, Hkv, D)
-        ws = q.new_empty(n, dtype=torch.uint8) if n else None
-        _lib.call("fl_attn_fwd", _ptr(q), _ptr(k), _ptr(v),
-                  _Strides3(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), B, Sq, Sk, Hq, Hkv, D, _ptr(begin),
-                  _ptr(end), scale, softcap, _ptr(slopes), _ptr(out), _ptr(lse), _ptr(ws), n, stream_of(dev))
+    n = _lib.function("fl_attn_fwd_workspace_bytes")(B, Sq, Sk, Hq, Hkv, D)
+    ws = q.new_empty(n, dtype=torch.uint8) if n else None
+    _lib.check(on_device(dev, _lib.function("fl_attn_fwd"), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                         _Strides3(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), B, Sq, Sk, Hq, Hkv, D,
+                         begin.data_ptr(), end.data_ptr(), scale, softcap, _ptr(slopes), out.data_ptr(),
+                         lse.data_ptr(), _ptr(ws), n, stream_of(dev)), "fl_attn_fwd")
     return out, lse
 
 
@@ -146,7 +145,6 @@ def bwd(dout, q, k, v, out, lse, begin, end, *, scale=None, softcap=0.0, slopes=
     """(dq, dk, dv) of fwd(): bf16, contiguous; dk and dv summed over the query
     heads that share them, in a fixed order.  out and lse: what fwd() returned."""
     dev, B, Sq, Sk, Hq, Hkv, D, scale, softcap = _check(q, k, v, begin, end, scale, softcap, slopes)
-    _need_cuda(dout, out, lse)
     if dout.shape != q.shape or out.shape != q.shape or dout.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
         raise ValueError("dout and out must be bf16 of q's shape")
     if lse.shape != (B, Sq, Hq) or lse.dtype != torch.float32:
@@ -155,7 +153,7 @@ def bwd(dout, q, k, v, out, lse, begin, end, *, scale=None, softcap=0.0, slopes=
         raise ValueError("attention arguments must be on one device")
     dq = q.new_empty((B, Sq, Hq, D))
     dk = q.new_empty((B, Sk, Hkv, D))
-    dv = q.new_empty((B, Sk, Hkv, D))
+    dv = torch.empty_like(dk)
     if dq.numel() + dk.numel() == 0:
         return dq, dk, dv
     q, k, v, dout = _view(q), _view(k), _view(v), _view(dout)
@@ -163,13 +161,13 @@ def bwd(dout, q, k, v, out, lse, begin, end, *, scale=None, softcap=0.0, slopes=
     begin, end = begin.contiguous(), end.contiguous()
     if slopes is not None:
         slopes = slopes.contiguous()
-    with on_device(dev):
-        n = _lib.load().fl_attn_bwd_workspace_bytes(B, Sq, Sk, Hq, Hkv, D)
-        ws = q.new_empty(n, dtype=torch.uint8) if n else None
-        _lib.call("fl_attn_bwd", _ptr(dout), _ptr(q), _ptr(k), _ptr(v),
-                  _Strides4(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *dout.stride()[:3]), _ptr(out),
-                  _ptr(lse), B, Sq, Sk, Hq, Hkv, D, _ptr(begin), _ptr(end), scale, softcap, _ptr(slopes), _ptr(dq),
-                  _ptr(dk), _ptr(dv), _ptr(ws), n, stream_of(dev))
+    n = _lib.function("fl_attn_bwd_workspace_bytes")(B, Sq, Sk, Hq, Hkv, D)
+    ws = q.new_empty(n, dtype=torch.uint8) if n else None
+    _lib.check(on_device(dev, _lib.function("fl_attn_bwd"), dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                         _Strides4(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *dout.stride()[:3]),
+                         out.data_ptr(), lse.data_ptr(), B, Sq, Sk, Hq, Hkv, D, begin.data_ptr(), end.data_ptr(),
+                         scale, softcap, _ptr(slopes), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), n,
+                         stream_of(dev)), "fl_attn_bwd")
     return dq, dk, dv
 
 

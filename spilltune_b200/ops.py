@@ -11,8 +11,6 @@ unchanged and accumulates into ``grad_A``/``grad_B`` exactly as before.
 All work runs on the current CUDA stream.  CPU tensors are rejected: the path
 has no CPU fallback.
 """
-import contextlib
-
 import torch
 
 from . import _lib
@@ -35,19 +33,21 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-_SAME_DEVICE = contextlib.nullcontext()
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
-
-
-def on_device(device):
-    """Context in which `device` is the current one (none is entered when it is already)."""
-    return _SAME_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def stream_of(device):
     """Handle of the current stream of `device`.  The raw query is what torch's own generated
     code calls; building a Stream object around it takes 2 us, a tenth of a small call."""
-    return _raw_stream(device.index) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index)
+
+
+def on_device(device, call, *args):
+    """call(*args) with `device` current (it mostly is already)."""
+    if device.index == torch.cuda.current_device():
+        return call(*args)
+    with torch.cuda.device(device):
+        return call(*args)
 
 
 def dequant(weight: PackedWeight, out=None):

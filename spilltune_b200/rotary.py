@@ -114,7 +114,7 @@ def _rows(x, what):
 def _setup(q, k, positions, inv_freq, q_weight, k_weight, eps):
     """Argument checks of both passes and what they share: (tokens, key heads,
     positions, position bytes, inv_freq, rotated columns, weights, weight bytes, eps)."""
-    _need_cuda(q, k, positions, inv_freq, q_weight, k_weight)
+    _need_cuda(q, k, positions, inv_freq)
     dev, shape = q.device, q.shape
     if len(shape) < 3:
         raise ValueError("q must be [..., heads, head size]")
@@ -162,6 +162,11 @@ def _setup(q, k, positions, inv_freq, q_weight, k_weight, eps):
             wbytes, float(eps or 0.0))
 
 
+def _like(x):
+    """Contiguous uninitialised tensor of x's shape and type."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
 def fwd(q, k, positions, inv_freq, *, interleaved=False, factor=1.0, q_weight=None, k_weight=None, eps=None):
     """(q', k'): q [..., Hq, D] and k [..., Hk, D] (or None), bf16, with the first
     2 * len(inv_freq) columns of every head rotated by positions * inv_freq,
@@ -174,15 +179,15 @@ def fwd(q, k, positions, inv_freq, *, interleaved=False, factor=1.0, q_weight=No
                                                                                       q_weight, k_weight, eps)
     qr, qt, qh = _rows(q, "q")
     kr, kt, kh = _rows(k, "k") if k is not None else (None, 0, 0)
-    yq = q.new_empty(q.shape)
-    yk = None if k is None else k.new_empty(k.shape)
+    yq = _like(q)
+    yk = None if k is None else _like(k)
     if T == 0:
         return yq, yk
     dev = q.device
-    with on_device(dev):
-        _lib.call("fl_rotary_fwd", _ptr(qr), qt, qh, q.shape[-2], _ptr(kr), kt, kh, Hk, T, q.shape[-1],
-                  _ptr(positions), pbytes, _ptr(inv_freq), rot, int(bool(interleaved)), factor, _ptr(q_weight),
-                  _ptr(k_weight), wbytes, eps, _ptr(yq), _ptr(yk), stream_of(dev))
+    _lib.check(on_device(dev, _lib.function("fl_rotary_fwd"), qr.data_ptr(), qt, qh, q.shape[-2], _ptr(kr), kt, kh, Hk,
+                         T, q.shape[-1], positions.data_ptr(), pbytes, inv_freq.data_ptr(), rot,
+                         1 if interleaved else 0, factor, _ptr(q_weight), _ptr(k_weight), wbytes, eps, yq.data_ptr(),
+                         _ptr(yk), stream_of(dev)), "fl_rotary_fwd")
     return yq, yk
 
 
@@ -196,7 +201,6 @@ def bwd(dq, dk, q, k, positions, inv_freq, *, interleaved=False, factor=1.0, q_w
         raise ValueError("dk goes with k")
     T, Hk, positions, pbytes, inv_freq, rot, q_weight, k_weight, wbytes, eps = _setup(q, k, positions, inv_freq,
                                                                                       q_weight, k_weight, eps)
-    _need_cuda(dq, dk)
     if dq.shape != q.shape or k is not None and dk.shape != k.shape:
         raise ValueError("dq and dk must have the shapes of q and k")
     dev = q.device
@@ -212,21 +216,21 @@ def bwd(dq, dk, q, k, positions, inv_freq, *, interleaved=False, factor=1.0, q_w
         if k is not None:
             kr, kt, kh = _rows(k, "k")
     D = q.shape[-1]
-    gq = q.new_empty(q.shape)
-    gk = None if k is None else k.new_empty(k.shape)
+    gq = _like(dq)
+    gk = None if k is None else _like(dk)
     gqw = gkw = ws = None
     nbytes = 0
     if weight_grads:
         gqw = q.new_zeros(D, dtype=torch.float32) if T == 0 else q.new_empty(D, dtype=torch.float32)
         gkw = None if k is None else gqw.new_zeros(D) if T == 0 else gqw.new_empty(D)
-        nbytes = _lib.load().fl_rotary_bwd_workspace_bytes(D)
+        nbytes = _lib.function("fl_rotary_bwd_workspace_bytes")(D)
         ws = q.new_empty(nbytes, dtype=torch.uint8)
     if T:
-        with on_device(dev):
-            _lib.call("fl_rotary_bwd", _ptr(dqr), dqt, dqh, _ptr(dkr), dkt, dkh, _ptr(qr), qt, qh, q.shape[-2],
-                      _ptr(kr), kt, kh, Hk, T, D, _ptr(positions), pbytes, _ptr(inv_freq), rot,
-                      int(bool(interleaved)), factor, _ptr(q_weight), _ptr(k_weight), wbytes, eps, _ptr(gq), _ptr(gk),
-                      _ptr(gqw), _ptr(gkw), _ptr(ws), nbytes, stream_of(dev))
+        _lib.check(on_device(dev, _lib.function("fl_rotary_bwd"), dqr.data_ptr(), dqt, dqh, _ptr(dkr), dkt, dkh,
+                             _ptr(qr), qt, qh, q.shape[-2], _ptr(kr), kt, kh, Hk, T, D, positions.data_ptr(), pbytes,
+                             inv_freq.data_ptr(), rot, 1 if interleaved else 0, factor, _ptr(q_weight),
+                             _ptr(k_weight), wbytes, eps, gq.data_ptr(), _ptr(gk), _ptr(gqw), _ptr(gkw), _ptr(ws),
+                             nbytes, stream_of(dev)), "fl_rotary_bwd")
     return gq, gk, gqw, gkw
 
 
