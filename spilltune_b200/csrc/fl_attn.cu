@@ -28,14 +28,16 @@ namespace fl {
 namespace attn {
 
 constexpr int kFwdThreads = 192;
+constexpr int kKeys = 64;           // keys of a streamed tile
 constexpr float kRescale = 8.0f;   // growth of the maximum (in powers of two) that rescales O
 
 template <int HD>
 struct Fwd {
-  static constexpr int kStages = HD == 64 ? 2 : 1;       // K and V tiles in flight
-  static constexpr int kTileBytes = HD / 64 * kTile * 128;
-  static constexpr int kSmem = 1024 + (1 + 2 * kStages) * kTileBytes + 256;
-  static constexpr int kTmem = 256;                      // S (P over it) + O
+  static constexpr int kStages = HD == 64 ? 4 : 2;       // K and V tiles in flight
+  static constexpr int kQBytes = HD / 64 * kTile * 128;
+  static constexpr int kTileBytes = HD / 64 * kKeys * 128;
+  static constexpr int kSmem = 1024 + kQBytes + 2 * kStages * kTileBytes + 256;
+  static constexpr int kTmem = 256;                      // two S (P over each) + O
 };
 
 struct FwdArgs {
@@ -49,8 +51,9 @@ struct FwdArgs {
 };
 
 struct __align__(16) FwdBars {
-  uint64_t q_full, qk_done, p_full, pv_done;
-  uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2];
+  uint64_t q_full, pv_done, all_done;
+  uint64_t s_full[2], p_full[2];       // of the two S buffers
+  uint64_t k_full[4], v_full[4], k_empty[4], v_empty[4];
   uint32_t tmem, abort_word;
 };
 
@@ -62,7 +65,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* qs = smem;
-  uint8_t* ks = qs + C::kTileBytes;
+  uint8_t* ks = qs + C::kQBytes;
   uint8_t* vs = ks + C::kStages * C::kTileBytes;
   FwdBars* bars = reinterpret_cast<FwdBars*>(vs + C::kStages * C::kTileBytes);
   volatile uint32_t* abort_word = &bars->abort_word;
@@ -83,9 +86,12 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
-    mbar_init(&bars->qk_done, 1);
-    mbar_init(&bars->p_full, 4);
     mbar_init(&bars->pv_done, 1);
+    mbar_init(&bars->all_done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->p_full[i], 4);
+    }
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&bars->k_full[i], 1);
       mbar_init(&bars->v_full[i], 1);
@@ -103,8 +109,8 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
   const Range r = tile_range(s, b, t0, kTile >> s.lgp);
   int k_first = 0, n = 0;
   if (r.min_lo < r.max_hi) {
-    k_first = r.min_lo / kTile;
-    n = (r.max_hi + kTile - 1) / kTile - k_first;
+    k_first = r.min_lo / kKeys;
+    n = (r.max_hi + kKeys - 1) / kKeys - k_first;
   }
   if (a.splits > 1) {
     const int from = static_cast<int>(static_cast<int64_t>(n) * split / a.splits);
@@ -115,30 +121,30 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_s = bars->tmem, tmem_o = bars->tmem + kTile;
+  const uint32_t tmem_s = bars->tmem, tmem_o = bars->tmem + 2 * kKeys;
 
   if (warp == 0) {
     if (lane == 0 && n > 0) {
       tma_prefetch_desc(&tm_q);
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
-      mbar_arrive_expect_tx(&bars->q_full, C::kTileBytes);
+      mbar_arrive_expect_tx(&bars->q_full, C::kQBytes);
       for (int c = 0; c < HD / 64; ++c) tma_load_4d(qs + c * kTile * 128, &tm_q, 64 * c, h0, t0, b, &bars->q_full);
       bool ok = true;
       int kn = 0, vn = 0;  // loads issued
       for (int j = 0; j < n && ok; ++j) {
         const int st = j % C::kStages;
         const uint32_t ph = (j / C::kStages - 1) & 1;
-        const int key = (k_first + j) * kTile;
+        const int key = (k_first + j) * kKeys;
         if (j >= C::kStages && !mbar_wait_short(&bars->k_empty[st], ph, abort_word, a.status, kStatusTimeoutEmpty)) break;
         mbar_arrive_expect_tx(&bars->k_full[st], C::kTileBytes);
         for (int c = 0; c < HD / 64; ++c)
-          tma_load_4d(ks + st * C::kTileBytes + c * kTile * 128, &tm_k, 64 * c, kvh, key, b, &bars->k_full[st]);
+          tma_load_4d(ks + st * C::kTileBytes + c * kKeys * 128, &tm_k, 64 * c, kvh, key, b, &bars->k_full[st]);
         ++kn;
         if (j >= C::kStages && !mbar_wait_short(&bars->v_empty[st], ph, abort_word, a.status, kStatusTimeoutEmpty)) break;
         mbar_arrive_expect_tx(&bars->v_full[st], C::kTileBytes);
         for (int c = 0; c < HD / 64; ++c)
-          tma_load_4d(vs + st * C::kTileBytes + c * kTile * 128, &tm_v, 64 * c, kvh, key, b, &bars->v_full[st]);
+          tma_load_4d(vs + st * C::kTileBytes + c * kKeys * 128, &tm_v, 64 * c, kvh, key, b, &bars->v_full[st]);
         ++vn;
       }
       // No copy may be in flight when the CTA leaves.
@@ -153,43 +159,45 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
     // The whole warp walks and one lane issues: operands stay uniform, and the
     // issue takes few slots of the scheduler that the softmax warps share.
     if (n > 0) {
-      const uint32_t id_s = idesc_bf16_f32(kTile, kTile), id_o = idesc_bf16_f32_bmn(kTile, HD);
+      const uint32_t id_s = idesc_bf16_f32(kTile, kKeys), id_o = idesc_bf16_f32_bmn(kTile, HD);
       const uint64_t dq = sdesc_kmajor_sw128(smem_u32(qs)), dk = sdesc_kmajor_sw128(smem_u32(ks));
-      const uint64_t dv = cols_desc(smem_u32(vs));
-      auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t bit) {
-        return mbar_wait_short_warp(bar, parity, abort_word, a.status, bit);
+      const uint64_t dv = cols_desc<kKeys>(smem_u32(vs));
+      auto wait = [&](uint64_t* bar, int phase, uint32_t bit) {
+        return mbar_wait_short_warp(bar, phase & 1, abort_word, a.status, bit);
       };
-      bool ok = wait(&bars->q_full, 0, kStatusTimeoutFull);
-      int pv = 0, qk = 0;
+      auto scores = [&](int j) -> bool {
+        const int st = j % C::kStages;
+        if (!wait(&bars->k_full[st], j / C::kStages, kStatusTimeoutFull)) return false;
+        tc_fence_after();
+        if (elected()) {
+          mma_rows<HD, kKeys>(tmem_s + (j & 1) * kKeys, dq, dk + st * (C::kTileBytes >> 4), id_s);
+          tc_commit(&bars->k_empty[st]);
+          tc_commit(&bars->s_full[j & 1]);
+        }
+        __syncwarp();
+        return true;
+      };
+      bool ok = wait(&bars->q_full, 0, kStatusTimeoutFull) && scores(0) && (n == 1 || scores(1));
       for (int j = 0; j < n && ok; ++j) {
         const int st = j % C::kStages;
-        const uint32_t ph = (j / C::kStages) & 1;
-        // S shares its columns with P: the product that reads P(j - 1) has to be done.
-        if (!wait(&bars->k_full[st], ph, kStatusTimeoutFull) ||
-            (j > 0 && !wait(&bars->pv_done, (j - 1) & 1, kStatusTimeoutAccum)))
+        if (!wait(&bars->v_full[st], j / C::kStages, kStatusTimeoutFull) ||
+            !wait(&bars->p_full[j & 1], j >> 1, kStatusTimeoutFull))
           break;
         tc_fence_after();
         if (elected()) {
-          mma_rows<HD>(tmem_s, dq, dk + st * (C::kTileBytes >> 4), id_s);
-          tc_commit(&bars->k_empty[st]);
-          tc_commit(&bars->qk_done);
-        }
-        __syncwarp();
-        ++qk;
-        if (!wait(&bars->v_full[st], ph, kStatusTimeoutFull) || !wait(&bars->p_full, j & 1, kStatusTimeoutFull)) break;
-        tc_fence_after();
-        if (elected()) {
-          mma_cols<HD, kTile>(tmem_o, tmem_s, dv + st * (C::kTileBytes >> 4), id_o, j > 0);
+          mma_cols<HD, kKeys, kKeys>(tmem_o, tmem_s + (j & 1) * kKeys, dv + st * (C::kTileBytes >> 4), id_o, j > 0);
           tc_commit(&bars->v_empty[st]);
           tc_commit(&bars->pv_done);
         }
         __syncwarp();
-        ++pv;
+        // P(j) lies in the columns of S(j + 2): the product that reads it has to
+        // be done, which it is while the softmax of S(j + 1) goes on.
+        if (j + 2 < n) ok = wait(&bars->pv_done, j, kStatusTimeoutAccum) && scores(j + 2);
       }
       // The products still under way read shared memory and TMEM.
+      if (elected()) tc_commit(&bars->all_done);
       uint32_t none = 0;
-      if (qk) mbar_wait(&bars->qk_done, (qk - 1) & 1, &none, a.status, kStatusTimeoutDrain);
-      if (pv) mbar_wait(&bars->pv_done, (pv - 1) & 1, &none, a.status, kStatusTimeoutDrain);
+      mbar_wait(&bars->all_done, 0, &none, a.status, kStatusTimeoutDrain);
       __syncwarp();
     }
   } else {
@@ -205,22 +213,22 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      const int key0 = (k_first + j) * kTile;
-      const bool whole = r.max_lo <= key0 && r.min_hi >= key0 + kTile;
-      if (!mbar_wait_short_warp(&bars->qk_done, j & 1, abort_word, a.status, kStatusTimeoutAccum)) {
+      const int key0 = (k_first + j) * kKeys;
+      const uint32_t at_s = tmem_s + (j & 1) * kKeys + lanes;
+      const bool whole = r.max_lo <= key0 && r.min_hi >= key0 + kKeys;
+      if (!mbar_wait_short_warp(&bars->s_full[j & 1], (j >> 1) & 1, abort_word, a.status, kStatusTimeoutAccum)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      // The row's 128 scores, in registers from here on.
-      uint32_t v[kTile];
+      // The row's scores, in registers from here on.
+      uint32_t v[kKeys];
 #pragma unroll
-      for (int c = 0; c < kTile; c += 32)
-        tmem_ld_32x32b_x32(tmem_s + lanes + c, reinterpret_cast<uint32_t(&)[32]>(v[c]));
+      for (int c = 0; c < kKeys; c += 32) tmem_ld_32x32b_x32(at_s + c, reinterpret_cast<uint32_t(&)[32]>(v[c]));
       tmem_wait_ld();
       if constexpr (kBias) {
 #pragma unroll
-        for (int i = 0; i < kTile; ++i) {
+        for (int i = 0; i < kKeys; ++i) {
           float th;
           v[i] = __float_as_uint(score2(s, __uint_as_float(v[i]), slope2, qpos - (key0 + i), th));
         }
@@ -228,12 +236,12 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       if (!whole) {
         const int lo_c = lo - key0, hi_c = hi - key0;
 #pragma unroll
-        for (int i = 0; i < kTile; ++i)
+        for (int i = 0; i < kKeys; ++i)
           if (i < lo_c || i >= hi_c) v[i] = 0xff800000u;
       }
       float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < kTile; i += 8)
+      for (int i = 0; i < kKeys; i += 8)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           m4[e] = fmaxf(m4[e], fmaxf(__uint_as_float(v[i + e]), __uint_as_float(v[i + 4 + e])));
@@ -243,7 +251,12 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       } else {
         const bool grow = mx > m + kRescale;
         if (__any_sync(0xffffffffu, grow)) {
-          // O is at rest: S(j) was issued after P(j - 1) V had completed.
+          // O is at rest once P(j - 1) V is done (P(j - 2) V is, or S(j) would not be).
+          if (!mbar_wait_short_warp(&bars->pv_done, (j - 1) & 1, abort_word, a.status, kStatusTimeoutAccum)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
           const float by = grow ? ex2(m - mx) : 1.0f;
           if (grow) m = mx;
           l *= by;
@@ -263,7 +276,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       const uint64_t mult_2 = pair(mult, mult), neg_2 = pair(neg, neg);
       uint64_t sum0 = 0, sum1 = 0;   // (0, 0)
 #pragma unroll
-      for (int c = 0; c < kTile; c += 32) {
+      for (int c = 0; c < kKeys; c += 32) {
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
@@ -276,7 +289,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
           w[i] = pack_bf16x2(x0, x1);
           w[i + 1] = pack_bf16x2(x2, x3);
         }
-        tmem_st_32x32b_x16(tmem_s + lanes + c / 2, w);
+        tmem_st_32x32b_x16(at_s + c / 2, w);
       }
       float l0, l1;
       unpair(add2(sum0, sum1), l0, l1);
@@ -284,10 +297,10 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->p_full);
+      if (lane == 0) mbar_arrive(&bars->p_full[j & 1]);
     }
-    if (n > 0 && ok)
-      ok = mbar_wait_short_warp(&bars->pv_done, (n - 1) & 1, abort_word, a.status, kStatusTimeoutAccum);
+    // A barrier of its own: of pv_done's last two phases either may be the current one here.
+    if (n > 0 && ok) ok = mbar_wait_short_warp(&bars->all_done, 0, abort_word, a.status, kStatusTimeoutAccum);
     tc_fence_after();
     if (n == 0 || ok) {
       const int64_t at = (static_cast<int64_t>(b) * s.Sq + tok) * s.Hq + head;
@@ -539,8 +552,8 @@ int fl_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const i
   CUtensorMap mq{}, mk{}, mv{};
   if ((rc = attn_map(&mq, q, strides[0], strides[1], strides[2], (int)B, (int)Sq, Hq, D, pg, attn::kTile >> a.s.lgp)))
     return rc;
-  if (Sk && ((rc = attn_map(&mk, k, strides[3], strides[4], strides[5], (int)B, (int)Sk, Hkv, D, 1, attn::kTile)) ||
-             (rc = attn_map(&mv, v, strides[6], strides[7], strides[8], (int)B, (int)Sk, Hkv, D, 1, attn::kTile))))
+  if (Sk && ((rc = attn_map(&mk, k, strides[3], strides[4], strides[5], (int)B, (int)Sk, Hkv, D, 1, attn::kKeys)) ||
+             (rc = attn_map(&mv, v, strides[6], strides[7], strides[8], (int)B, (int)Sk, Hkv, D, 1, attn::kKeys))))
     return rc;
   const bool bias = softcap != 0.f || slopes;
   const int64_t grid = ctas * a.splits;

@@ -151,26 +151,28 @@ __device__ __forceinline__ bool elected() {
 // it, so a step is an addition: the issuing thread shares its scheduler with
 // element warps and has few slots between two products.
 //
-// D[128 x 128] = A . B^T, both K-major in shared memory: 128 rows as HD / 64
-// chunks of rows of 128 bytes; a and b from sdesc_kmajor_sw128.
-template <int HD>
+// D[128 x kRows] = A . B^T, both K-major in shared memory: A 128 rows, B kRows,
+// each as HD / 64 chunks of rows of 128 bytes; a and b from sdesc_kmajor_sw128.
+template <int HD, int kRows>
 __device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
 #pragma unroll
-  for (int kk = 0; kk < HD / 16; ++kk) {
-    const uint32_t step = (kk / 4) * (kTile * 128 >> 4) + 2 * (kk % 4);
-    mma_ss(d, a + step, b + step, idesc, kk != 0);
-  }
+  for (int kk = 0; kk < HD / 16; ++kk)
+    mma_ss(d, a + (kk / 4) * (kTile * 128 >> 4) + 2 * (kk % 4), b + (kk / 4) * (kRows * 128 >> 4) + 2 * (kk % 4), idesc,
+           kk != 0);
 }
 
-// D[128 x HD] (+)= A . B: A bf16 [128 x 128] in TMEM, each kGroup columns of A
-// from a_tmem + kGroup * group on; B [128 x HD] in shared memory (the same
-// chunks, read with the columns as the MN side), b from cols_desc.  kGroup =
-// 128: A is packed.
-__device__ __forceinline__ uint64_t cols_desc(uint32_t addr) { return sdesc_mnmajor_sw128(addr, kTile * 128, 1024); }
-template <int HD, int kGroup>
+// D[128 x HD] (+)= A . B: A bf16 [128 x kRows] in TMEM, each kGroup columns of A
+// from a_tmem + kGroup * group on; B [kRows x HD] in shared memory (the same
+// chunks, read with the columns as the MN side), b from cols_desc<kRows>.
+// kGroup = kRows: A is packed.
+template <int kRows>
+__device__ __forceinline__ uint64_t cols_desc(uint32_t addr) {
+  return sdesc_mnmajor_sw128(addr, kRows * 128, 1024);
+}
+template <int HD, int kRows, int kGroup>
 __device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, bool accumulate) {
 #pragma unroll
-  for (int kk = 0; kk < kTile / 16; ++kk)
+  for (int kk = 0; kk < kRows / 16; ++kk)
     mma_ts(d, a_tmem + kk * 16 / kGroup * kGroup + kk * 16 % kGroup / 2, b + kk * (2048 >> 4), idesc,
            accumulate || kk != 0);
 }

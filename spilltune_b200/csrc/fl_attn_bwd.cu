@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const uint32_t id_s = idesc_bf16_f32(kTile, kTile), id_acc = idesc_bf16_f32_bmn(kTile, HD);
     const uint32_t col_s = tmem, col_p = tmem + kColP;
     const uint64_t d_a[2] = {sdesc_kmajor_sw128(smem_u32(a1)), sdesc_kmajor_sw128(smem_u32(a2))};
-    const uint64_t d_rows = sdesc_kmajor_sw128(smem_u32(bs)), d_cols = cols_desc(smem_u32(bs));
+    const uint64_t d_rows = sdesc_kmajor_sw128(smem_u32(bs)), d_cols = cols_desc<kTile>(smem_u32(bs));
     auto at = [&](int g, int o) { return static_cast<uint64_t>((g % C::kStages) * 2 + o) * (C::kBytes >> 4); };
     int g0 = 0, k = 0;       // steps and items with steps before this one
     bool issued = false;
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (!wait(&bars->b_full[o][g % C::kStages], g / C::kStages, kStatusTimeoutFull)) return false;
       tc_fence_after();
       if (elected()) {
-        mma_rows<HD>(o ? col_p : col_s, d_a[o], d_rows + at(g, o), id_s);
+        mma_rows<HD, kTile>(o ? col_p : col_s, d_a[o], d_rows + at(g, o), id_s);
         tc_commit(o ? &bars->dp_full : &bars->s_full);
         if (o && last) tc_commit(&bars->a_empty);
       }
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         tc_fence_after();
         if (elected()) {
-          mma_cols<HD, kCols>(tmem + kColAcc, col_s, d_cols + at(g, kDq ? 0 : 1), id_acc, i > 0);
+          mma_cols<HD, kTile, kCols>(tmem + kColAcc, col_s, d_cols + at(g, kDq ? 0 : 1), id_acc, i > 0);
           tc_commit(&bars->b_empty[1][st]);
           tc_commit(&bars->acc1_done);
         }
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         tc_fence_after();
         if (elected()) {
-          mma_cols<HD, kCols>(tmem + kColAcc + HD, col_p, d_cols + at(g, 0), id_acc, i > 0);
+          mma_cols<HD, kTile, kCols>(tmem + kColAcc + HD, col_p, d_cols + at(g, 0), id_acc, i > 0);
           tc_commit(&bars->b_empty[0][st]);
           tc_commit(&bars->acc2_done);
           if (i + 1 == n) tc_commit(&bars->acc_full);
