@@ -57,11 +57,12 @@ struct __align__(16) FwdBars {
   uint32_t tmem, abort_word;
 };
 
-template <int HD, bool kBias>
+template <int HD, int kMode>
 __global__ void __launch_bounds__(kFwdThreads, 2)
     fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const FwdArgs a) {
   using C = Fwd<HD>;
+  constexpr bool kBias = kMode != kPlain;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* qs = smem;
@@ -227,10 +228,11 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       for (int c = 0; c < kKeys; c += 32) tmem_ld_32x32b_x32(at_s + c, reinterpret_cast<uint32_t(&)[32]>(v[c]));
       tmem_wait_ld();
       if constexpr (kBias) {
+        const float from_key0 = static_cast<float>(qpos - key0);
 #pragma unroll
         for (int i = 0; i < kKeys; ++i) {
           float th;
-          v[i] = __float_as_uint(score2(s, __uint_as_float(v[i]), slope2, qpos - (key0 + i), th));
+          v[i] = __float_as_uint(score2<kMode>(s, __uint_as_float(v[i]), slope2, from_key0 - i, th));
         }
       }
       if (!whole) {
@@ -283,7 +285,11 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
           float x0, x1, x2, x3;
           unpair(fma2(pair(v[c + 2 * i], v[c + 2 * i + 1]), mult_2, neg_2), x0, x1);
           unpair(fma2(pair(v[c + 2 * i + 2], v[c + 2 * i + 3]), mult_2, neg_2), x2, x3);
-          x0 = ex2(x0), x1 = ex2(x1), x2 = ex2(x2), x3 = ex2(x3);
+          if constexpr (kMode == kCapped)          // two of four: the tanh keeps the special units busy
+            ex2_pair(x0, x1, x0, x1);
+          else
+            x0 = ex2(x0), x1 = ex2(x1);
+          x2 = ex2(x2), x3 = ex2(x3);
           sum0 = add2(sum0, pair(x0, x1));
           sum1 = add2(sum1, pair(x2, x3));
           w[i] = pack_bf16x2(x0, x1);
@@ -435,12 +441,12 @@ int64_t fwd_ctas(int B, int Sq, int Hq, int Hkv) {
   return tiles * B * (Hq >> lgp);
 }
 
-template <int HD, bool kBias>
+template <int HD, int kMode>
 int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdArgs& a, int64_t grid,
                cudaStream_t stream) {
-  int rc = allow_smem(reinterpret_cast<const void*>(&fwd_kernel<HD, kBias>), Fwd<HD>::kSmem);
+  int rc = allow_smem(reinterpret_cast<const void*>(&fwd_kernel<HD, kMode>), Fwd<HD>::kSmem);
   if (rc) return rc;
-  fwd_kernel<HD, kBias><<<static_cast<unsigned>(grid), kFwdThreads, Fwd<HD>::kSmem, stream>>>(q, k, v, a);
+  fwd_kernel<HD, kMode><<<static_cast<unsigned>(grid), kFwdThreads, Fwd<HD>::kSmem, stream>>>(q, k, v, a);
   return FL_OK;
 }
 
@@ -555,12 +561,15 @@ int fl_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const i
   if (Sk && ((rc = attn_map(&mk, k, strides[3], strides[4], strides[5], (int)B, (int)Sk, Hkv, D, 1, attn::kKeys)) ||
              (rc = attn_map(&mv, v, strides[6], strides[7], strides[8], (int)B, (int)Sk, Hkv, D, 1, attn::kKeys))))
     return rc;
-  const bool bias = softcap != 0.f || slopes;
+  const int mode = softcap != 0.f ? attn::kCapped : slopes ? attn::kSlopes : attn::kPlain;
   const int64_t grid = ctas * a.splits;
-  rc = D <= 64 ? (bias ? attn::launch_fwd<64, true>(mq, mk, mv, a, grid, st)
-                       : attn::launch_fwd<64, false>(mq, mk, mv, a, grid, st))
-               : (bias ? attn::launch_fwd<128, true>(mq, mk, mv, a, grid, st)
-                       : attn::launch_fwd<128, false>(mq, mk, mv, a, grid, st));
+  using attn::launch_fwd;
+  rc = D <= 64 ? (mode == attn::kCapped   ? launch_fwd<64, attn::kCapped>(mq, mk, mv, a, grid, st)
+                  : mode == attn::kSlopes ? launch_fwd<64, attn::kSlopes>(mq, mk, mv, a, grid, st)
+                                          : launch_fwd<64, attn::kPlain>(mq, mk, mv, a, grid, st))
+               : (mode == attn::kCapped   ? launch_fwd<128, attn::kCapped>(mq, mk, mv, a, grid, st)
+                  : mode == attn::kSlopes ? launch_fwd<128, attn::kSlopes>(mq, mk, mv, a, grid, st)
+                                          : launch_fwd<128, attn::kPlain>(mq, mk, mv, a, grid, st));
   if (rc) return rc;
   if (a.splits > 1) {
     // A programmatic dependent: its launch overlaps the attention kernel, whose results it waits for.

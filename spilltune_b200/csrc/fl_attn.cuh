@@ -118,18 +118,24 @@ __device__ __forceinline__ void ex2_pair(float x0, float x1, float& y0, float& y
 // the cap multiplies (the hardware's tanh would leave 2^-11 of the cap).
 __device__ __forceinline__ float tanh_from(float two_y_log2e) { return 1.0f - 2.0f * rcp(1.0f + ex2(two_y_log2e)); }
 
+// What is done to a score before the softmax.
+enum Mode : int { kPlain = 0, kSlopes = 1, kCapped = 2 };   // capped: and slopes, if any
+
 // A score in units of log2: cap and distance applied.  th receives the tanh.
-__device__ __forceinline__ float score2(const Shape& s, float qk, float slope2, int dist, float& th) {
-  float x;
+template <int kMode>
+__device__ __forceinline__ float score2(const Shape& s, float qk, float slope2, float dist, float& th) {
   th = 0.f;
-  if (s.cap2 != 0.f) {
+  float x = qk * s.sl2;
+  if constexpr (kMode == kCapped) {
     th = tanh_from(qk * s.icap2);
     x = s.cap2 * th;
-  } else {
-    x = qk * s.sl2;
   }
-  return x - slope2 * static_cast<float>(abs(dist));
+  return fmaf(-slope2, fabsf(dist), x);
 }
+
+// A small non-negative integer as a float without the conversion unit (which
+// is the special-function unit).
+__device__ __forceinline__ float small_float(int v) { return __int_as_float(0x4B000000 | v) - 8388608.0f; }
 
 __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, int w,
                                             uint64_t* bar) {

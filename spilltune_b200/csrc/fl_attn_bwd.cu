@@ -56,6 +56,7 @@ constexpr int kColP = 128, kColAcc = 256;   // TMEM: S, P', the two accumulators
 struct __align__(16) RowInfo {
   float nlse2[kTile], ndelta[kTile];
   int lo[kTile], hi[kTile];
+  float slope2[kTile];             // with slopes: of the row's head, times log2(e)
   int max_lo[kGroups], min_hi[kGroups];
 };
 constexpr int kInfoBytes = sizeof(RowInfo);
@@ -123,12 +124,13 @@ __device__ __forceinline__ float dot8(const uint4& a, const uint4& b) {
 
 // kDq: rows are packed queries (A1 = q, A2 = do; B1 = k, B2 = v).
 // Otherwise rows are keys (A1 = k, A2 = v; B1 = q, B2 = do).
-template <int HD, bool kDq, bool kBias>
+template <int HD, bool kDq, int kMode>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant__ CUtensorMap tm_a2,
                const __grid_constant__ CUtensorMap tm_b1, const __grid_constant__ CUtensorMap tm_b2,
                const BwdArgs a) {
   using C = Bwd<HD>;
+  constexpr bool kBias = kMode != kPlain, kCap = kMode == kCapped;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* a1 = smem;
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const int g = g0 + i, st = g % C::kStages;
         const RowInfo& cols = info[st];              // dk, dv: of the step's columns
         bool whole;
-        int col0, h_first = 0;                       // dq: first key; else first token and head
+        int col0;                                    // dq: the group's first key; else its first token
         if (!kDq && !wait(&bars->b_full[0][st], g / C::kStages, kStatusTimeoutFull)) {
           ok = false;
           break;
@@ -469,7 +471,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           whole = it.seen.max_lo <= col0 && it.seen.min_hi >= col0 + kCols;
         } else {
           col0 = at.tile * q_step + (mine0 >> s.lgp);
-          h_first = kvh * G + at.group * pg;
           whole = cols.max_lo[group] <= row0 && cols.min_hi[group] >= row0 + kTile;
         }
         [[maybe_unused]] uint64_t nl_of[kDq ? 1 : kCols / 2];   // dk, dv: -lse2 of the columns
@@ -485,9 +486,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           break;
         }
         tc_fence_after();
+        // dq: from the row's token to the first key; else from the row's key to the first token.
+        [[maybe_unused]] const float dist0 = static_cast<float>((kDq ? tok : col0 - key) + s.Sk - s.Sq - (kDq ? col0 : 0));
         const uint32_t at_s = tmem + kCols * group + lanes, at_p = at_s + kColP;
         uint32_t x[kCols], w[kCols / 2];             // scores, then p; packed operands
-        [[maybe_unused]] __half2 fac[kBias ? kCols / 2 : 1];
+        [[maybe_unused]] __half2 fac[kCap ? kCols / 2 : 1];
         tmem_ld_32x32b_x32(at_s, x);
         tmem_wait_ld();
         // Which of the columns c .. c + 3 the row does not see.
@@ -517,18 +520,29 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           float p[4];
           [[maybe_unused]] float f[4];
           if constexpr (kBias) {
-            float l[4];
+            float l[4], slope2[4];
             unpair(nl[0], l[0], l[1]);
             unpair(nl[1], l[2], l[3]);
+            if constexpr (kDq) {
+              slope2[0] = slope2[1] = slope2[2] = slope2[3] = row_slope2;
+            } else {
+              const float4 v = *reinterpret_cast<const float4*>(cols.slope2 + mine0 + c);
+              slope2[0] = v.x, slope2[1] = v.y, slope2[2] = v.z, slope2[3] = v.w;
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int col = c + e;
-              const int at = kDq ? tok : col0 + (col >> s.lgp), k_at = kDq ? col0 + col : key;
-              const float slope2 = kDq ? row_slope2 : (s.slopes ? s.slopes[h_first + (col & (pg - 1))] * kLog2e : 0.f);
+              // dq: columns are keys; else those of a token's packed heads share its distance
+              const float dist = kDq ? dist0 - col : dist0 + small_float(col >> s.lgp);
               float th;
-              p[e] = ex2(score2(s, __uint_as_float(x[col]), slope2, at + s.Sk - s.Sq - k_at, th) + l[e]);
+              p[e] = score2<kMode>(s, __uint_as_float(x[col]), slope2[e], dist, th) + l[e];
               f[e] = 1.0f - th * th;
             }
+            if constexpr (kCap)                    // two of four: the tanh keeps the special units busy
+              ex2_pair(p[0], p[1], p[0], p[1]);
+            else
+              p[0] = ex2(p[0]), p[1] = ex2(p[1]);
+            p[2] = ex2(p[2]), p[3] = ex2(p[3]);
           } else {
 #pragma unroll
             for (int h = 0; h < 4; h += 2) {
@@ -550,7 +564,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[c + e] = __float_as_uint(p[e]);
-          if constexpr (kBias) {
+          if constexpr (kCap) {
             // f waits for dp in 16 bits: 2^-12 of a factor of ds, an eighth of ds's own rounding.
             fac[c / 2] = __floats2half2_rn(f[0], f[1]);
             fac[c / 2 + 1] = __floats2half2_rn(f[2], f[3]);
@@ -606,7 +620,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
               }
             }
             uint64_t pf = p;
-            if constexpr (kBias) {
+            if constexpr (kCap) {
               const float2 f = __half22float2(fac[col / 2]);
               pf = mul2(p, pair(f.x, f.y));
             }
@@ -659,6 +673,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         } else if (group == 1) {
           o->lo[row] = lo;
           o->hi[row] = hi;
+        } else if (kBias && group == 2) {
+          o->slope2[row] = row_slope2;
         }
         if (quarter == 0) {
           const Range h = tile_range(s, b, row0 + (mine0 >> s.lgp), max(kCols >> s.lgp, 1));
@@ -780,14 +796,26 @@ int device_sms() {
   return n;
 }
 
-template <int HD, bool kDq, bool kBias>
+template <int HD, bool kDq, int kMode>
 int launch_bwd(const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1, const CUtensorMap& b2,
                const BwdArgs& a, cudaStream_t stream) {
-  int rc = allow_smem(reinterpret_cast<const void*>(&bwd_kernel<HD, kDq, kBias>), Bwd<HD>::kSmem);
+  int rc = allow_smem(reinterpret_cast<const void*>(&bwd_kernel<HD, kDq, kMode>), Bwd<HD>::kSmem);
   if (rc) return rc;
   const int64_t grid = a.items < device_sms() ? a.items : device_sms();
-  bwd_kernel<HD, kDq, kBias><<<static_cast<unsigned>(grid), kBwdThreads, Bwd<HD>::kSmem, stream>>>(a1, a2, b1, b2, a);
+  bwd_kernel<HD, kDq, kMode><<<static_cast<unsigned>(grid), kBwdThreads, Bwd<HD>::kSmem, stream>>>(a1, a2, b1, b2, a);
   return FL_OK;
+}
+
+template <bool kDq>
+int launch_bwd_any(int D, int mode, const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1,
+                   const CUtensorMap& b2, const BwdArgs& a, cudaStream_t stream) {
+  if (D <= 64)
+    return mode == kCapped   ? launch_bwd<64, kDq, kCapped>(a1, a2, b1, b2, a, stream)
+           : mode == kSlopes ? launch_bwd<64, kDq, kSlopes>(a1, a2, b1, b2, a, stream)
+                             : launch_bwd<64, kDq, kPlain>(a1, a2, b1, b2, a, stream);
+  return mode == kCapped   ? launch_bwd<128, kDq, kCapped>(a1, a2, b1, b2, a, stream)
+         : mode == kSlopes ? launch_bwd<128, kDq, kSlopes>(a1, a2, b1, b2, a, stream)
+                           : launch_bwd<128, kDq, kPlain>(a1, a2, b1, b2, a, stream);
 }
 
 int64_t q_tiles_of(int64_t Sq, int lgp) { return (Sq + (kTile >> lgp) - 1) / (kTile >> lgp); }
@@ -875,23 +903,17 @@ int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, cons
       (rc = attn_map(&mv, v, strides[6], strides[7], strides[8], b, sk, Hkv, D, 1, attn::kTile)) ||
       (rc = attn_map(&mdo, dout, strides[9], strides[10], strides[11], b, sq, Hq, D, pg, q_step)))
     return rc;
-  const bool bias = softcap != 0.f || slopes;
+  const int mode = softcap != 0.f ? attn::kCapped : slopes ? attn::kSlopes : attn::kPlain;
   a.items = attn::fwd_ctas(b, sq, Hq, Hkv);
   a.parts = 1;
   a.tiles = static_cast<int>(a.items / B / (Hq >> a.s.lgp));
-  rc = D <= 64 ? (bias ? attn::launch_bwd<64, true, true>(mq, mdo, mk, mv, a, st)
-                       : attn::launch_bwd<64, true, false>(mq, mdo, mk, mv, a, st))
-               : (bias ? attn::launch_bwd<128, true, true>(mq, mdo, mk, mv, a, st)
-                       : attn::launch_bwd<128, true, false>(mq, mdo, mk, mv, a, st));
+  rc = attn::launch_bwd_any<true>(D, mode, mq, mdo, mk, mv, a, st);
   if (rc) return rc;
   a.tiles = static_cast<int>(key_tiles);
   a.parts = parts;
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + part_at);
   a.items = key_tiles * B * Hkv * parts;
-  rc = D <= 64 ? (bias ? attn::launch_bwd<64, false, true>(mk, mv, mq, mdo, a, st)
-                       : attn::launch_bwd<64, false, false>(mk, mv, mq, mdo, a, st))
-               : (bias ? attn::launch_bwd<128, false, true>(mk, mv, mq, mdo, a, st)
-                       : attn::launch_bwd<128, false, false>(mk, mv, mq, mdo, a, st));
+  rc = attn::launch_bwd_any<false>(D, mode, mk, mv, mq, mdo, a, st);
   if (rc) return rc;
   if (parts > 1) {
     const int64_t n4 = B * Sk * Hkv * D / 4;

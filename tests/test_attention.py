@@ -135,6 +135,9 @@ CASES = [  # B, Sq, Sk, H, K, D, mask, cap, slopes
     (1, 1, 5000, 7, 1, 64, "window", 0.0, False),
     (2, 5, 2000, 8, 2, 80, "holes", 50.0, True),
     (1, 1300, 1300, 4, 2, 128, "all", 0.0, False),
+    (1, 45, 300, 64, 1, 64, "causal", 0.0, True),
+    (1, 150, 150, 256, 2, 64, "documents", 30.0, True),
+    (1, 500, 500, 16, 1, 128, "holes", 0.0, True),
 ]
 
 
@@ -265,6 +268,26 @@ def test_equal_bits_other_stream_and_captured_passes(cuda_lib):
     flipped = captured(q.flip(1).contiguous())
     assert all(torch.equal(x, y) for x, y in zip(results[0], flipped))
     assert all(torch.equal(x, want[n]) for x, n in zip(results[1], ("out", "dq", "dk", "dv")))
+
+
+@pytest.mark.gpu
+def test_many_tiles(cuda_lib):
+    """Enough tiles that every CTA takes several and waits on its pipelines in every order: no wait expires, and
+    sampled heads agree with the formulas."""
+    B, S, H, K, D = 2, 2048, 32, 8, 128
+    q, k, v, do = _inputs(B, S, S, H, K, D, 12)
+    for kind in ("causal", "documents"):
+        begin, end = (t.cuda() for t in _ranges(kind, B, S, S, 1))
+        got = _both(q, k, v, begin, end, do)
+        for _ in range(3):
+            again = _both(q, k, v, begin, end, do)
+            assert all(torch.equal(again[n], got[n]) for n in got)
+        for b, h in ((0, 0), (1, 7)):
+            part = lambda t, n: t[b:b + 1, :, h * n:(h + 1) * n]  # noqa: E731
+            want = _oracle(part(q, 4), part(k, 1), part(v, 1), begin[b:b + 1], end[b:b + 1], D ** -0.5, 0.0, None,
+                           part(do, 4))
+            for n in got:
+                _within(n, part(got[n], 1 if n in ("dk", "dv") else 4), want[n])
 
 
 @pytest.mark.gpu
