@@ -41,7 +41,7 @@ def build(force=False, verbose=False, extra=()):
     if not force and not _stale():
         return LIB
     tmp = LIB + ".tmp"
-    cmd = [nvcc_path(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC,-O2",
+    cmd = [nvcc_path(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "--threads", "0", "-shared", "-Xcompiler", "-fPIC,-O2",
            "-I", os.path.join(ROOT, "include"), "-o", tmp,
            *[os.path.join(CSRC, s) for s in SOURCES], *extra]
     if verbose:

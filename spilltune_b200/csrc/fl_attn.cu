@@ -1,22 +1,33 @@
 // Attention forward over row ranges (see fl_attn.cuh for the formulas).
 //
-// A CTA takes a tile of 128 (packed) query rows and walks the 128-key tiles
-// that its rows see, with the running maximum m and sum l of a softmax:
-//   S = Q K^T (tcgen05, accumulator in TMEM)
+// A CTA takes a tile of 128 (packed) query rows and walks the 64-key tiles that
+// its rows see, with the running maximum m and sum l of a softmax:
+//   S = Q K^T (tcgen05, accumulator in TMEM, two buffers)
 //   p = 2^(x - m) in FP32, l += sum p, P = bf16(p) over S's columns in TMEM
 //   O += P V (tcgen05, A operand from TMEM)
 // Roles: one warp issues TMA loads, one the MMAs, four own the rows (a thread
-// per row, so row maxima and sums need no exchange).  Two CTAs share an SM:
-// one's softmax runs under the other's products.
+// per row, so row maxima and sums need no exchange).  Two CTAs share an SM: one's
+// softmax runs under the other's products.
+//
+// What bounds it is the chain scores - softmax - values of a CTA.  With 128-key
+// tiles and one S buffer (P lies over S) the next scores waited for the product
+// that reads P: 530 us for 8192 causal tokens, 32/8 heads of 128.  With 64-key
+// tiles S(j + 1) is there before the softmax of S(j) ends: 472 us, 1163 TFLOP/s
+// (70% of the burst rate of a bf16 GEMM), although 64 columns leave the scores'
+// product bound by its operands' fetches (48 cycles where 32 would do).  Two
+// threads to a row instead of one gained nothing (they meet once a tile).
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 over the
 // one in use (the sums then stay far inside FP32's range); otherwise the old
-// reference stays.  P is rounded to bf16 as the second product's operand: half
-// a step of each probability, of the same size as rounding the result.
+// reference stays.  P is rounded to bf16 as the second product's operand: half a
+// step of each probability, of the same size as rounding the result.
 //
-// Few rows over many keys (a decode step): the key tiles are split over
-// several CTAs whose normalised FP32 results and log sums are joined by a
-// second kernel.
+// Few rows over many keys (a decode step): the key tiles are split over several
+// CTAs whose normalised FP32 results and log sums are joined by a second
+// kernel.  There what P's rounding left follows as a second operand: the few
+// results of such a call show every rounding, and the products are not what
+// bounds it (one token over 8192 keys, 32/8 heads, 4 sequences: 28.8 us instead
+// of 26.1, error against 64 bits 1.7e-3 instead of 2.3e-3).
 #include <cuda_bf16.h>
 #include <cstdint>
 #include <map>
@@ -57,7 +68,8 @@ struct __align__(16) FwdBars {
   uint32_t tmem, abort_word;
 };
 
-template <int HD, int kMode>
+// kFine: P in two bf16 parts.
+template <int HD, int kMode, bool kFine>
 __global__ void __launch_bounds__(kFwdThreads, 2)
     fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const FwdArgs a) {
@@ -186,7 +198,9 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
           break;
         tc_fence_after();
         if (elected()) {
-          mma_cols<HD, kKeys, kKeys>(tmem_o, tmem_s + (j & 1) * kKeys, dv + st * (C::kTileBytes >> 4), id_o, j > 0);
+          const uint32_t p = tmem_s + (j & 1) * kKeys;
+          mma_cols<HD, kKeys, kKeys>(tmem_o, p, dv + st * (C::kTileBytes >> 4), id_o, j > 0);
+          if constexpr (kFine) mma_cols<HD, kKeys, kKeys>(tmem_o, p + kKeys / 2, dv + st * (C::kTileBytes >> 4), id_o, true);
           tc_commit(&bars->v_empty[st]);
           tc_commit(&bars->pv_done);
         }
@@ -280,6 +294,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
 #pragma unroll
       for (int c = 0; c < kKeys; c += 32) {
         uint32_t w[16];
+        [[maybe_unused]] uint32_t u[16];
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
           float x0, x1, x2, x3;
@@ -294,7 +309,12 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
           sum1 = add2(sum1, pair(x2, x3));
           w[i] = pack_bf16x2(x0, x1);
           w[i + 1] = pack_bf16x2(x2, x3);
+          if constexpr (kFine) {                            // what the rounding left, to be added as a second part
+            u[i] = pack_bf16x2(x0 - __uint_as_float(w[i] << 16), x1 - __uint_as_float(w[i] & 0xFFFF0000u));
+            u[i + 1] = pack_bf16x2(x2 - __uint_as_float(w[i + 1] << 16), x3 - __uint_as_float(w[i + 1] & 0xFFFF0000u));
+          }
         }
+        if constexpr (kFine) tmem_st_32x32b_x16(at_s + kKeys / 2 + c / 2, u);
         tmem_st_32x32b_x16(at_s + c / 2, w);
       }
       float l0, l1;
@@ -441,13 +461,21 @@ int64_t fwd_ctas(int B, int Sq, int Hq, int Hkv) {
   return tiles * B * (Hq >> lgp);
 }
 
-template <int HD, int kMode>
+template <int HD, int kMode, bool kFine>
 int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdArgs& a, int64_t grid,
                cudaStream_t stream) {
-  int rc = allow_smem(reinterpret_cast<const void*>(&fwd_kernel<HD, kMode>), Fwd<HD>::kSmem);
+  int rc = allow_smem(reinterpret_cast<const void*>(&fwd_kernel<HD, kMode, kFine>), Fwd<HD>::kSmem);
   if (rc) return rc;
-  fwd_kernel<HD, kMode><<<static_cast<unsigned>(grid), kFwdThreads, Fwd<HD>::kSmem, stream>>>(q, k, v, a);
+  fwd_kernel<HD, kMode, kFine><<<static_cast<unsigned>(grid), kFwdThreads, Fwd<HD>::kSmem, stream>>>(q, k, v, a);
   return FL_OK;
+}
+
+template <int HD, bool kFine>
+int launch_fwd_mode(int mode, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdArgs& a,
+                    int64_t grid, cudaStream_t stream) {
+  return mode == kCapped   ? launch_fwd<HD, kCapped, kFine>(q, k, v, a, grid, stream)
+         : mode == kSlopes ? launch_fwd<HD, kSlopes, kFine>(q, k, v, a, grid, stream)
+                           : launch_fwd<HD, kPlain, kFine>(q, k, v, a, grid, stream);
 }
 
 }  // namespace attn
@@ -563,13 +591,12 @@ int fl_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const i
     return rc;
   const int mode = softcap != 0.f ? attn::kCapped : slopes ? attn::kSlopes : attn::kPlain;
   const int64_t grid = ctas * a.splits;
-  using attn::launch_fwd;
-  rc = D <= 64 ? (mode == attn::kCapped   ? launch_fwd<64, attn::kCapped>(mq, mk, mv, a, grid, st)
-                  : mode == attn::kSlopes ? launch_fwd<64, attn::kSlopes>(mq, mk, mv, a, grid, st)
-                                          : launch_fwd<64, attn::kPlain>(mq, mk, mv, a, grid, st))
-               : (mode == attn::kCapped   ? launch_fwd<128, attn::kCapped>(mq, mk, mv, a, grid, st)
-                  : mode == attn::kSlopes ? launch_fwd<128, attn::kSlopes>(mq, mk, mv, a, grid, st)
-                                          : launch_fwd<128, attn::kPlain>(mq, mk, mv, a, grid, st));
+  if (a.splits > 1)
+    rc = D <= 64 ? attn::launch_fwd_mode<64, true>(mode, mq, mk, mv, a, grid, st)
+                 : attn::launch_fwd_mode<128, true>(mode, mq, mk, mv, a, grid, st);
+  else
+    rc = D <= 64 ? attn::launch_fwd_mode<64, false>(mode, mq, mk, mv, a, grid, st)
+                 : attn::launch_fwd_mode<128, false>(mode, mq, mk, mv, a, grid, st);
   if (rc) return rc;
   if (a.splits > 1) {
     // A programmatic dependent: its launch overlaps the attention kernel, whose results it waits for.
