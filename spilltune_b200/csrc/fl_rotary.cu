@@ -19,8 +19,14 @@
 // Vector form (head size and rot multiples of 16, 16-byte aligned rows): a
 // thread owns the two 8-column vectors whose columns pair up, so a rotation
 // needs no exchange between threads and a head's sum of squares is a shuffle
-// over head_dim/16 neighbouring lanes.  Other shapes take the scalar form, a
-// warp per head, which loads each column's partner as well.
+// over head_dim/16 neighbouring lanes.  Instructions come next after HBM, so the
+// arithmetic works on pairs of FP32 values, angles and weights lie in shared
+// memory as neighbouring lanes read them, and rows per block leave few lanes
+// idle.  Measured at 8192 tokens: 32 + 8 heads of 128 30 us forward or backward
+// (168 MB: 5.5 TB/s, 85% of a copy's rate); with a norm 32 + 4 heads 34.5 us
+// forward (4.4 TB/s) and 49 us backward (226 MB: 4.7 TB/s).  Other shapes take
+// the scalar form, a warp per head, which loads each column's partner as well
+// (1027 tokens, 16 heads of 80, 40 columns rotated: 11 us, 1.5 as a copy).
 #include <cuda_bf16.h>
 #include <cstdint>
 
