@@ -17,6 +17,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .ops import _need_cuda, _ptr, on_device, stream_of
@@ -105,8 +106,8 @@ def _check(q, k, v, begin, end, scale, softcap, slopes):
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError("scale must be positive and finite")
     softcap = float(softcap or 0.0)
-    if not (softcap >= 0 and math.isfinite(softcap)):
-        raise ValueError("softcap must be >= 0 and finite")
+    if not (softcap >= 0 and math.isfinite(softcap)) or softcap and scale / softcap > 1e30:
+        raise ValueError("softcap must be 0, or finite and not too small for the scale")
     return dev, B, Sq, Sk, Hq, Hkv, D, scale, softcap
 
 
@@ -180,6 +181,7 @@ class _Attend(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, begin, end, slopes = ctx.saved_tensors
         dq, dk, dv = bwd(dout, q, k, v, out, lse, begin, end, scale=ctx.scale, softcap=ctx.softcap, slopes=slopes)

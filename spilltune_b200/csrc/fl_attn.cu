@@ -149,12 +149,14 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
         const int st = j % C::kStages;
         const uint32_t ph = (j / C::kStages - 1) & 1;
         const int key = (k_first + j) * kKeys;
-        if (j >= C::kStages && !mbar_wait_short(&bars->k_empty[st], ph, abort_word, a.status, kStatusTimeoutEmpty)) break;
+        if (j >= C::kStages && !mbar_wait_short(&bars->k_empty[st], ph, abort_word, a.status, kStatusTimeoutEmpty))
+          break;
         mbar_arrive_expect_tx(&bars->k_full[st], C::kTileBytes);
         for (int c = 0; c < HD / 64; ++c)
           tma_load_4d(ks + st * C::kTileBytes + c * kKeys * 128, &tm_k, 64 * c, kvh, key, b, &bars->k_full[st]);
         ++kn;
-        if (j >= C::kStages && !mbar_wait_short(&bars->v_empty[st], ph, abort_word, a.status, kStatusTimeoutEmpty)) break;
+        if (j >= C::kStages && !mbar_wait_short(&bars->v_empty[st], ph, abort_word, a.status, kStatusTimeoutEmpty))
+          break;
         mbar_arrive_expect_tx(&bars->v_full[st], C::kTileBytes);
         for (int c = 0; c < HD / 64; ++c)
           tma_load_4d(vs + st * C::kTileBytes + c * kKeys * 128, &tm_v, 64 * c, kvh, key, b, &bars->v_full[st]);
@@ -200,7 +202,8 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
         if (elected()) {
           const uint32_t p = tmem_s + (j & 1) * kKeys;
           mma_cols<HD, kKeys, kKeys>(tmem_o, p, dv + st * (C::kTileBytes >> 4), id_o, j > 0);
-          if constexpr (kFine) mma_cols<HD, kKeys, kKeys>(tmem_o, p + kKeys / 2, dv + st * (C::kTileBytes >> 4), id_o, true);
+          if constexpr (kFine)
+            mma_cols<HD, kKeys, kKeys>(tmem_o, p + kKeys / 2, dv + st * (C::kTileBytes >> 4), id_o, true);
           tc_commit(&bars->v_empty[st]);
           tc_commit(&bars->pv_done);
         }
@@ -517,7 +520,8 @@ int attn_check(const char* who, int64_t B, int64_t Sq, int64_t Sk, int Hq, int H
     return set_error(FL_ERR_ARG, "%s: batch, length or head count too large", who);
   if (D < 8 || D > 128 || D % 8) return set_error(FL_ERR_ARG, "%s: head size must be a multiple of 8 in [8, 128]", who);
   if (!(scale > 0.f) || scale > 3.0e38f) return set_error(FL_ERR_ARG, "%s: scale must be positive and finite", who);
-  if (!(cap >= 0.f) || cap > 3.0e38f) return set_error(FL_ERR_ARG, "%s: the cap must be >= 0 and finite", who);
+  if (!(cap >= 0.f) || cap > 3.0e38f || (cap > 0.f && scale / cap > 1.0e30f))
+    return set_error(FL_ERR_ARG, "%s: the cap must be 0, or finite and not too small for the scale", who);
   if (B == 0 || Sq == 0) return FL_OK;
   if (!begin || !end) return set_error(FL_ERR_ARG, "%s: null pointer", who);
   if (attn::fwd_ctas(static_cast<int>(B), static_cast<int>(Sq), Hq, Hkv) > (int64_t(1) << 30))

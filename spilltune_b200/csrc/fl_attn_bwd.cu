@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         tc_fence_after();
         // dq: from the row's token to the first key; else from the row's key to the first token.
-        [[maybe_unused]] const float dist0 = static_cast<float>((kDq ? tok : col0 - key) + s.Sk - s.Sq - (kDq ? col0 : 0));
+        [[maybe_unused]] const float dist0 = static_cast<float>((kDq ? tok - col0 : col0 - key) + s.Sk - s.Sq);
         const uint32_t at_s = tmem + kCols * group + lanes, at_p = at_s + kColP;
         uint32_t x[kCols], w[kCols / 2];             // scores, then p; packed operands
         [[maybe_unused]] __half2 fac[kCap ? kCols / 2 : 1];

@@ -73,7 +73,7 @@ using namespace fl;
 
 extern "C" {
 
-int fl_version(void) { return 310; }  // 0.3.1: reduction splits (fl_*_workspace_bytes_split)
+int fl_version(void) { return 400; }  // 0.4.0: fl_rotary_*, fl_attn_*
 
 int fl_wait_selftest(uint64_t limit_ns, void* stream) {
   if (limit_ns == 0 || limit_ns > kWaitLimitNs)

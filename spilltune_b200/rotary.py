@@ -17,6 +17,7 @@ CUDA only; no CPU fallback.
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .ops import _need_cuda, _ptr, on_device, stream_of
@@ -238,15 +239,20 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, inv_freq, interleaved, factor, eps):
         ctx.opt = dict(interleaved=interleaved, factor=factor, eps=eps)
-        ctx.save_for_backward(q, k, q_weight, k_weight, positions, inv_freq)
+        # Without a norm the gradients need no inputs: nothing keeps them alive.
+        ctx.has_k, norm = k is not None, q_weight is not None
+        ctx.save_for_backward(q if norm else None, k if norm else None, q_weight, k_weight, positions, inv_freq)
         ctx.set_materialize_grads(True)
         yq, yk = fwd(q.detach(), None if k is None else k.detach(), positions, inv_freq, q_weight=q_weight,
                      k_weight=k_weight, **ctx.opt)
         return (yq,) if yk is None else (yq, yk)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk=None):
         q, k, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
+        if q is None:
+            q, k = dq, dk if ctx.has_k else None
         weights = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
         gq, gk, gqw, gkw = bwd(dq, dk, q, k, positions, inv_freq, q_weight=q_weight, k_weight=k_weight,
                                weight_grads=weights, **ctx.opt)

@@ -407,7 +407,7 @@ def test_c_entry_refusals():
 
     bad = [dict(B=-1), dict(Sq=-1), dict(Sk=-2), dict(Hq=0), dict(Hkv=0), dict(Hq=3), dict(D=4), dict(D=68),
            dict(D=136), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(cap=-1.0),
-           dict(cap=float("nan")), dict(strides=None), dict(strides=[12] + good[1:], B=2), dict(q=None),
+           dict(cap=float("nan")), dict(cap=1e-35), dict(strides=None), dict(strides=[12] + good[1:], B=2), dict(q=None),
            dict(q=p + 8), dict(begin=None), dict(out=None), dict(out=p + 2),
            dict(strides=[good[0], 0, 64] + good[3:]), dict(strides=[good[0], good[1], 36] + good[3:]),
            dict(B=1 << 20), dict(Sq=1 << 31), dict(Hq=1 << 13, Hkv=1 << 13)]
@@ -438,6 +438,7 @@ def test_refusals(cuda_lib):
            (lambda: attention.fwd(q, k, v, r, r[:, :4]), "end"),
            (lambda: attention.fwd(q, k, v, r, r, scale=0.0), "scale"),
            (lambda: attention.fwd(q, k, v, r, r, softcap=-1.0), "softcap"),
+           (lambda: attention.fwd(q, k, v, r, r, softcap=1e-35), "softcap"),
            (lambda: attention.fwd(q, k, v, r, r, slopes=torch.ones(2, device="cuda")), "slopes"),
            (lambda: attention.attend(q, k, v, r, r, slopes=torch.ones(4, device="cuda", requires_grad=True)),
             "no gradient"),
