@@ -576,8 +576,8 @@ int fl_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const i
   a.out = reinterpret_cast<__nv_bfloat16*>(out);
   a.lse = lse;
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || !(a.status = status_word(dev)))
-    return set_error(FL_ERR_CUDA, "fl_attn_fwd: status word unavailable");
+  if ((rc = current_context(&dev))) return rc;
+  if (!(a.status = status_word(dev))) return set_error(FL_ERR_CUDA, "fl_attn_fwd: status word unavailable");
   const int pg = 1 << a.s.lgp;
   const int64_t ctas = attn::fwd_ctas((int)B, (int)Sq, Hq, Hkv);
   a.tiles = static_cast<int>(ctas / B / (Hq >> a.s.lgp));

@@ -192,7 +192,8 @@ void fill_shape(Shape& s, int B, int Sq, int Sk, int Hq, int Hkv, int D, const i
 }  // namespace attn
 
 // Tiled tensor map of any rank: dims and box innermost first, stride_bytes of
-// the dimensions from the second on (fl_gemm.cu).
+// the dimensions from the second on; after current_context (fl_gemm.cu).
+int current_context(int* dev);
 int make_tensor_map(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int rank, const uint64_t* dims,
                     const uint64_t* stride_bytes, const uint32_t* box, CUtensorMapSwizzle swz);
 int allow_smem(const void* kernel, int bytes);

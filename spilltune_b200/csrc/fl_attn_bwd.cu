@@ -101,6 +101,7 @@ struct BwdArgs {
   int tiles;             // resident tiles per head
   int64_t items;         // pieces of work: tiles, heads, sequences, parts
   int* taken;            // items of dk and dv beyond the CTAs' first: 0 again after the dq kernel
+  int sms;               // of the device
   int parts;             // dk, dv: items that share a tile's walk
   float* part;           // their sums [parts][dv, dk][B, Sk, Hkv, D] (parts > 1)
 };
@@ -806,20 +807,12 @@ int bwd_parts(int64_t key_ctas, int64_t steps) {
   return n < 1 ? 1 : static_cast<int>(n);
 }
 
-int device_sms() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
-  return n;
-}
-
 template <int HD, bool kDq, int kMode>
 int launch_bwd(const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1, const CUtensorMap& b2,
                const BwdArgs& a, cudaStream_t stream) {
   int rc = allow_smem(reinterpret_cast<const void*>(&bwd_kernel<HD, kDq, kMode>), Bwd<HD>::kSmem);
   if (rc) return rc;
-  const int64_t grid = a.items < device_sms() ? a.items : device_sms();
+  const int64_t grid = a.items < a.sms ? a.items : a.sms;
   bwd_kernel<HD, kDq, kMode><<<static_cast<unsigned>(grid), kBwdThreads, Bwd<HD>::kSmem, stream>>>(a1, a2, b1, b2, a);
   return FL_OK;
 }
@@ -896,8 +889,9 @@ int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, cons
   attn::BwdArgs a{};
   attn::fill_shape(a.s, (int)B, (int)Sq, (int)Sk, Hq, Hkv, D, begin, end, scale, softcap, slopes);
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || !(a.status = status_word(dev)))
-    return set_error(FL_ERR_CUDA, "fl_attn_bwd: status word unavailable");
+  if ((rc = current_context(&dev))) return rc;
+  if (!(a.status = status_word(dev))) return set_error(FL_ERR_CUDA, "fl_attn_bwd: status word unavailable");
+  a.sms = device_sms(dev);
   a.q_tiles = static_cast<int>(attn::q_tiles_of(Sq, a.s.lgp));
   a.info = static_cast<attn::RowInfo*>(workspace);
   a.ranges = reinterpret_cast<attn::Range*>(a.info + B * (Hq >> a.s.lgp) * a.q_tiles);

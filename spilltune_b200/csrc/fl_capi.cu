@@ -2,6 +2,7 @@
 // Argument checking happens here, before any launch; kernels live in the other
 // translation units.
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -36,6 +37,16 @@ uint32_t* status_word(int device) {
     addr[device] = static_cast<uint32_t*>(p);
   }
   return addr[device];
+}
+
+int device_sms(int device) {
+  static std::atomic<int> known[64];
+  if (device < 0 || device >= 64) return 148;
+  int n = known[device].load(std::memory_order_relaxed);
+  if (n) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n < 1) return 148;
+  known[device].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

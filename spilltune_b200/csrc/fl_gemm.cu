@@ -522,16 +522,19 @@ static PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
   return fn;
 }
 
+// The encode is a driver call: makes the runtime's current device's primary
+// context current on this thread (e.g. torch's autograd worker thread may not
+// have touched the runtime yet).
+int current_context(int* dev) {
+  if (cudaGetDevice(dev) != cudaSuccess || cudaSetDevice(*dev) != cudaSuccess)
+    return set_error(FL_ERR_CUDA, "no current CUDA device for the tensor map");
+  return FL_OK;
+}
+
 int make_tensor_map(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int rank, const uint64_t* dims,
                     const uint64_t* stride_bytes, const uint32_t* box, CUtensorMapSwizzle swz) {
   auto fn = get_encode_fn();
   if (!fn) return set_error(FL_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-  // The encode is a driver call: make the runtime's current device's primary
-  // context current on this thread first (e.g. torch's autograd worker thread
-  // may not have touched the runtime yet).
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess)
-    return set_error(FL_ERR_CUDA, "no current CUDA device for the tensor map");
   cuuint64_t d[5], s[5];
   cuuint32_t b[5], estr[5];
   for (int i = 0; i < rank; ++i) {
@@ -549,6 +552,9 @@ int make_tensor_map(CUtensorMap* map, const void* base, CUtensorMapDataType dt, 
 
 int make_tensor_map_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, uint64_t inner, uint64_t outer,
                        uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swz) {
+  int dev = 0;
+  const int rc = current_context(&dev);
+  if (rc) return rc;
   const uint64_t dims[2] = {inner, outer};
   const uint32_t box[2] = {box_inner, box_outer};
   return make_tensor_map(map, base, dt, 2, dims, &row_stride_bytes, box, swz);

@@ -11,6 +11,7 @@ namespace fl {
 int set_error(int code, const char* fmt, ...);
 
 uint32_t* status_word(int device);  // device status word of the calling device
+int device_sms(int device);         // its SMs (148 when they cannot be queried); asked for once per device
 
 // Call chains.  `pdl` launches a kernel as a programmatic dependent of the
 // previous launch of the stream, which must be the chain's producer of the

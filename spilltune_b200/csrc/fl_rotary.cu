@@ -473,15 +473,9 @@ bool rows_fit(const void* p, int64_t tok, int64_t head, int heads) {
          tok * kMaxTokens + head * heads < (int64_t(1) << 31);
 }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
-  return n;
-}
-
 int launch(Args& a, bool norm, bool inter, bool bwd, float* dqw, float* dkw, cudaStream_t stream) {
+  int dev = 0;
+  const int sms = device_sms(cudaGetDevice(&dev) == cudaSuccess ? dev : -1);
   bool vec = a.D % 16 == 0 && a.rot % 16 == 0 && a.heads <= 4096;
   for (int i = 0; i < (a.heads > a.heads_q ? 2 : 1); ++i) {
     const Side& s = a.side[i];
@@ -507,7 +501,7 @@ int launch(Args& a, bool norm, bool inter, bool bwd, float* dqw, float* dkw, cud
     auto use = [&](int64_t n) { return static_cast<double>(n * a.heads) / ((n * a.heads + pass - 1) / pass * pass); };
     for (int64_t n = 2; n <= kMaxTokens && n * a.heads <= 2 * kChunk * pass; ++n)
       if (use(n) > use(tokens) + 0.01) tokens = n;
-    while (tokens > 1 && (a.T + tokens - 1) / tokens < 2 * sm_count()) --tokens;
+    while (tokens > 1 && (a.T + tokens - 1) / tokens < 2 * sms) --tokens;
     a.tokens = static_cast<int>(tokens);
     // exact while row * heads < 2^32
     a.heads_magic = static_cast<unsigned>(((uint64_t(1) << 32) + a.heads - 1) / a.heads);
@@ -516,7 +510,7 @@ int launch(Args& a, bool norm, bool inter, bool bwd, float* dqw, float* dkw, cud
     // Two rows to a warp at least, so that a block's angles serve them.
     int64_t tokens = (2 * (kThreads / 32) + a.heads - 1) / a.heads;
     if (tokens > kMaxTokens) tokens = kMaxTokens;
-    while (tokens > 1 && (a.T + tokens - 1) / tokens < 2 * sm_count()) --tokens;
+    while (tokens > 1 && (a.T + tokens - 1) / tokens < 2 * sms) --tokens;
     a.tokens = static_cast<int>(tokens);
     grid = (a.T + tokens - 1) / tokens;
   }
