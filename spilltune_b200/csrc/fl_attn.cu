@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
     const int tok = t0 + (row >> s.lgp), head = h0 + (row & ((1 << s.lgp) - 1));
     int lo = 0, hi = 0;
     if (tok < s.Sq) row_range(s, b, tok, lo, hi);
-    const float slope2 = kBias && s.slopes ? s.slopes[head] * kLog2e : 0.f;
+    const float slope2 = has_slopes(kMode) ? s.slopes[head] * kLog2e : 0.f;
     const int qpos = tok + s.Sk - s.Sq;
     const float mult = kBias ? 1.0f : s.sl2;   // from what TMEM holds to powers of two
     float m = -INFINITY, l = 0.f;
@@ -245,11 +245,18 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       for (int c = 0; c < kKeys; c += 32) tmem_ld_32x32b_x32(at_s + c, reinterpret_cast<uint32_t(&)[32]>(v[c]));
       tmem_wait_ld();
       if constexpr (kBias) {
-        const float from_key0 = static_cast<float>(qpos - key0);
+        [[maybe_unused]] const float from_key0 = static_cast<float>(qpos - key0);
+        const uint64_t sl2_2 = pair(s.sl2, s.sl2), cap2_2 = pair(s.cap2, s.cap2);
 #pragma unroll
-        for (int i = 0; i < kKeys; ++i) {
-          float th;
-          v[i] = __float_as_uint(score2<kMode>(s, __uint_as_float(v[i]), slope2, from_key0 - i, th));
+        for (int i = 0; i < kKeys; i += 2) {
+          uint64_t x = pair(v[i], v[i + 1]);
+          x = has_cap(kMode) ? capped2(s, cap_r2(s, x), cap2_2) : mul2(x, sl2_2);
+          if constexpr (has_slopes(kMode))
+            x = fma2(pair(-slope2, -slope2), pair(fabsf(from_key0 - i), fabsf(from_key0 - (i + 1))), x);
+          float x0, x1;
+          unpair(x, x0, x1);
+          v[i] = __float_as_uint(x0);
+          v[i + 1] = __float_as_uint(x1);
         }
       }
       if (!whole) {
@@ -303,7 +310,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
           float x0, x1, x2, x3;
           unpair(fma2(pair(v[c + 2 * i], v[c + 2 * i + 1]), mult_2, neg_2), x0, x1);
           unpair(fma2(pair(v[c + 2 * i + 2], v[c + 2 * i + 3]), mult_2, neg_2), x2, x3);
-          if constexpr (kMode == kCapped)          // two of four: the tanh keeps the special units busy
+          if constexpr (has_cap(kMode))            // two of four: the tanh keeps the special units busy
             ex2_pair(x0, x1, x0, x1);
           else
             x0 = ex2(x0), x1 = ex2(x1);
@@ -476,9 +483,10 @@ int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
 template <int HD, bool kFine>
 int launch_fwd_mode(int mode, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdArgs& a,
                     int64_t grid, cudaStream_t stream) {
-  return mode == kCapped   ? launch_fwd<HD, kCapped, kFine>(q, k, v, a, grid, stream)
-         : mode == kSlopes ? launch_fwd<HD, kSlopes, kFine>(q, k, v, a, grid, stream)
-                           : launch_fwd<HD, kPlain, kFine>(q, k, v, a, grid, stream);
+  return mode == kCappedSlopes ? launch_fwd<HD, kCappedSlopes, kFine>(q, k, v, a, grid, stream)
+         : mode == kCapped     ? launch_fwd<HD, kCapped, kFine>(q, k, v, a, grid, stream)
+         : mode == kSlopes     ? launch_fwd<HD, kSlopes, kFine>(q, k, v, a, grid, stream)
+                               : launch_fwd<HD, kPlain, kFine>(q, k, v, a, grid, stream);
 }
 
 }  // namespace attn
@@ -593,7 +601,7 @@ int fl_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const i
   if (Sk && ((rc = attn_map(&mk, k, strides[3], strides[4], strides[5], (int)B, (int)Sk, Hkv, D, 1, attn::kKeys)) ||
              (rc = attn_map(&mv, v, strides[6], strides[7], strides[8], (int)B, (int)Sk, Hkv, D, 1, attn::kKeys))))
     return rc;
-  const int mode = softcap != 0.f ? attn::kCapped : slopes ? attn::kSlopes : attn::kPlain;
+  const int mode = (softcap != 0.f ? attn::kCapped : attn::kPlain) + (slopes ? attn::kSlopes : 0);
   const int64_t grid = ctas * a.splits;
   if (a.splits > 1)
     rc = D <= 64 ? attn::launch_fwd_mode<64, true>(mode, mq, mk, mv, a, grid, st)

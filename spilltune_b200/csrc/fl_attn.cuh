@@ -114,23 +114,27 @@ __device__ __forceinline__ void ex2_pair(float x0, float x1, float& y0, float& y
   y1 = __int_as_float(__float_as_int(y1) + (__float_as_int(i1) << 23));
 }
 
-// tanh(y) from 2^(2 y log2 e): absolute error of a few 1e-7 everywhere, which
-// the cap multiplies (the hardware's tanh would leave 2^-11 of the cap).
-__device__ __forceinline__ float tanh_from(float two_y_log2e) { return 1.0f - 2.0f * rcp(1.0f + ex2(two_y_log2e)); }
-
 // What is done to a score before the softmax.
-enum Mode : int { kPlain = 0, kSlopes = 1, kCapped = 2 };   // capped: and slopes, if any
+enum Mode : int { kPlain = 0, kSlopes = 1, kCapped = 2, kCappedSlopes = 3 };
+__host__ __device__ constexpr bool has_cap(int mode) { return mode >= kCapped; }
+__host__ __device__ constexpr bool has_slopes(int mode) { return mode == kSlopes || mode == kCappedSlopes; }
 
-// A score in units of log2: cap and distance applied.  th receives the tanh.
-template <int kMode>
-__device__ __forceinline__ float score2(const Shape& s, float qk, float slope2, float dist, float& th) {
-  th = 0.f;
-  float x = qk * s.sl2;
-  if constexpr (kMode == kCapped) {
-    th = tanh_from(qk * s.icap2);
-    x = s.cap2 * th;
-  }
-  return fmaf(-slope2, fabsf(dist), x);
+// The cap, from r = 1 / (1 + 2^(2 y log2 e)): tanh(y) = 1 - 2 r with an absolute
+// error of a few 1e-7 everywhere, which the cap multiplies (the hardware's tanh
+// would leave 2^-11 of the cap); its derivative is 1 - tanh^2(y) = 4 r (1 - r).
+// r of two scores:
+__device__ __forceinline__ uint64_t cap_r2(const Shape& s, uint64_t qk) {
+  float y0, y1;
+  unpair(mul2(qk, pair(s.icap2, s.icap2)), y0, y1);
+  unpair(add2(pair(ex2(y0), ex2(y1)), pair(1.0f, 1.0f)), y0, y1);
+  return pair(rcp(y0), rcp(y1));
+}
+// cap log2(e) tanh + add:
+__device__ __forceinline__ uint64_t capped2(const Shape& s, uint64_t r, uint64_t add) {
+  return fma2(r, pair(-2.0f * s.cap2, -2.0f * s.cap2), add);   // add: with cap2 in it
+}
+__device__ __forceinline__ uint64_t cap_slope2(uint64_t r) {
+  return mul2(r, fma2(r, pair(-4.0f, -4.0f), pair(4.0f, 4.0f)));
 }
 
 // A small non-negative integer as a float without the conversion unit (which

@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                const __grid_constant__ CUtensorMap tm_b1, const __grid_constant__ CUtensorMap tm_b2,
                const BwdArgs a) {
   using C = Bwd<HD>;
-  constexpr bool kBias = kMode != kPlain, kCap = kMode == kCapped;
+  constexpr bool kBias = kMode != kPlain, kCap = has_cap(kMode), kSlope = has_slopes(kMode);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* a1 = smem;
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!meet()) break;
         d0 = dots[row];
       }
-      const float row_slope2 = kDq && kBias && s.slopes ? s.slopes[head] * kLog2e : 0.f;
+      const float row_slope2 = kDq && kSlope ? s.slopes[head] * kLog2e : 0.f;
       bool ok = true;
       Walk at(it);
       for (int i = 0; i < it.n; ++i, at.step(it)) {
@@ -536,25 +536,31 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             nl[0] = nl_of[c / 2], nl[1] = nl_of[c / 2 + 1];
           }
           float p[4];
-          [[maybe_unused]] float f[4];
+          [[maybe_unused]] uint64_t f[2];
           if constexpr (kBias) {
-            float l[4], slope2[4];
-            unpair(nl[0], l[0], l[1]);
-            unpair(nl[1], l[2], l[3]);
-            if constexpr (kDq) {
-              slope2[0] = slope2[1] = slope2[2] = slope2[3] = row_slope2;
-            } else {
+            [[maybe_unused]] float slope2[4] = {row_slope2, row_slope2, row_slope2, row_slope2};
+            if constexpr (!kDq && kSlope) {
               const float4 v = *reinterpret_cast<const float4*>(cols.slope2 + mine0 + c);
               slope2[0] = v.x, slope2[1] = v.y, slope2[2] = v.z, slope2[3] = v.w;
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int col = c + e;
-              // dq: columns are keys; else those of a token's packed heads share its distance
-              const float dist = kDq ? dist0 - col : dist0 + small_float(col >> s.lgp);
-              float th;
-              p[e] = score2<kMode>(s, __uint_as_float(x[col]), slope2[e], dist, th) + l[e];
-              f[e] = 1.0f - th * th;
+            for (int h = 0; h < 4; h += 2) {
+              const int col = c + h;
+              uint64_t e = pair(x[col], x[col + 1]);
+              if constexpr (kCap) {
+                const uint64_t r = cap_r2(s, e);
+                e = capped2(s, r, add2(nl[h / 2], pair(s.cap2, s.cap2)));
+                f[h / 2] = cap_slope2(r);
+              } else {
+                e = fma2(e, sl2_2, nl[h / 2]);
+              }
+              if constexpr (kSlope) {
+                // dq: columns are keys; else those of a token's packed heads share its distance
+                const float d_0 = kDq ? dist0 - col : dist0 + small_float(col >> s.lgp);
+                const float d_1 = kDq ? dist0 - (col + 1) : dist0 + small_float((col + 1) >> s.lgp);
+                e = fma2(pair(-slope2[h], -slope2[h + 1]), pair(fabsf(d_0), fabsf(d_1)), e);
+              }
+              unpair(e, p[h], p[h + 1]);
             }
             if constexpr (kCap)                    // two of four: the tanh keeps the special units busy
               ex2_pair(p[0], p[1], p[0], p[1]);
@@ -584,11 +590,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           for (int e = 0; e < 4; ++e) x[c + e] = __float_as_uint(p[e]);
           if constexpr (kCap) {
             // f waits for dp in 16 bits: 2^-12 of a factor of ds, an eighth of ds's own rounding.
-            fac[c / 2] = __floats2half2_rn(f[0], f[1]);
-            fac[c / 2 + 1] = __floats2half2_rn(f[2], f[3]);
-            if constexpr (kDq) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) p[e] *= f[e];
+            for (int h = 0; h < 4; h += 2) {
+              float f_0, f_1;
+              unpair(f[h / 2], f_0, f_1);
+              fac[(c + h) / 2] = __floats2half2_rn(f_0, f_1);
+              if constexpr (kDq) unpair(mul2(pair(p[h], p[h + 1]), f[h / 2]), p[h], p[h + 1]);
             }
           }
           w[c / 2] = pack_bf16x2(p[0], p[1]);
@@ -691,7 +698,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         } else if (group == 1) {
           o->lo[row] = lo;
           o->hi[row] = hi;
-        } else if (kBias && group == 2) {
+        } else if (kSlope && group == 2) {
           o->slope2[row] = row_slope2;
         }
         if (quarter == 0) {
@@ -817,16 +824,21 @@ int launch_bwd(const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& 
   return FL_OK;
 }
 
+template <int HD, bool kDq>
+int launch_bwd_mode(int mode, const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1,
+                    const CUtensorMap& b2, const BwdArgs& a, cudaStream_t stream) {
+  return mode == kCappedSlopes ? launch_bwd<HD, kDq, kCappedSlopes>(a1, a2, b1, b2, a, stream)
+         : mode == kCapped     ? launch_bwd<HD, kDq, kCapped>(a1, a2, b1, b2, a, stream)
+         : mode == kSlopes     ? launch_bwd<HD, kDq, kSlopes>(a1, a2, b1, b2, a, stream)
+                               : launch_bwd<HD, kDq, kPlain>(a1, a2, b1, b2, a, stream);
+}
+
 template <bool kDq>
 int launch_bwd_any(int D, int mode, const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1,
                    const CUtensorMap& b2, const BwdArgs& a, cudaStream_t stream) {
   if (D <= 64)
-    return mode == kCapped   ? launch_bwd<64, kDq, kCapped>(a1, a2, b1, b2, a, stream)
-           : mode == kSlopes ? launch_bwd<64, kDq, kSlopes>(a1, a2, b1, b2, a, stream)
-                             : launch_bwd<64, kDq, kPlain>(a1, a2, b1, b2, a, stream);
-  return mode == kCapped   ? launch_bwd<128, kDq, kCapped>(a1, a2, b1, b2, a, stream)
-         : mode == kSlopes ? launch_bwd<128, kDq, kSlopes>(a1, a2, b1, b2, a, stream)
-                           : launch_bwd<128, kDq, kPlain>(a1, a2, b1, b2, a, stream);
+    return launch_bwd_mode<64, kDq>(mode, a1, a2, b1, b2, a, stream);
+  return launch_bwd_mode<128, kDq>(mode, a1, a2, b1, b2, a, stream);
 }
 
 int64_t q_tiles_of(int64_t Sq, int lgp) { return (Sq + (kTile >> lgp) - 1) / (kTile >> lgp); }
@@ -916,7 +928,7 @@ int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, cons
       (rc = attn_map(&mv, v, strides[6], strides[7], strides[8], b, sk, Hkv, D, 1, attn::kTile)) ||
       (rc = attn_map(&mdo, dout, strides[9], strides[10], strides[11], b, sq, Hq, D, pg, q_step)))
     return rc;
-  const int mode = softcap != 0.f ? attn::kCapped : slopes ? attn::kSlopes : attn::kPlain;
+  const int mode = (softcap != 0.f ? attn::kCapped : attn::kPlain) + (slopes ? attn::kSlopes : 0);
   a.items = attn::fwd_ctas(b, sq, Hq, Hkv);
   a.parts = 1;
   a.tiles = static_cast<int>(a.items / B / (Hq >> a.s.lgp));
