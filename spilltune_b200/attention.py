@@ -122,6 +122,9 @@ def fwd(q, k, v, begin, end, *, scale=None, softcap=0.0, slopes=None):
 
     begin, end: int32 [B, Sq], the keys each query sees (see ``row_ranges``); a
     query that sees none gets 0 and a log sum of -inf.
+    Keys and values that no query sees, queries that see none and their
+    gradients may hold anything, NaN too; a key that one query sees has to be
+    finite for the queries around it as well (0 times infinity).
     scale: of q . k, default D ** -0.5.  softcap > 0: softcap * tanh(x / softcap).
     slopes: fp32 [Hq]; x -= slopes[h] * |i + Sk - Sq - j|."""
     dev, B, Sq, Sk, Hq, Hkv, D, scale, softcap = _check(q, k, v, begin, end, scale, softcap, slopes)

@@ -65,6 +65,7 @@ struct __align__(16) FwdBars {
   uint64_t q_full, pv_done, all_done;
   uint64_t s_full[2], p_full[2];       // of the two S buffers
   uint64_t k_full[4], v_full[4], k_empty[4], v_empty[4];
+  uint64_t v_clear[2];                 // of the first and the last tile
   uint32_t tmem, abort_word;
 };
 
@@ -101,6 +102,8 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
     mbar_init(&bars->q_full, 1);
     mbar_init(&bars->pv_done, 1);
     mbar_init(&bars->all_done, 1);
+    mbar_init(&bars->v_clear[0], 1);
+    mbar_init(&bars->v_clear[1], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->p_full[i], 4);
@@ -136,31 +139,66 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
   tc_fence_after();
   const uint32_t tmem_s = bars->tmem, tmem_o = bars->tmem + 2 * kKeys;
 
+  auto wait = [&](uint64_t* bar, int phase, uint32_t bit) {
+    return mbar_wait_short_warp(bar, phase & 1, abort_word, a.status, bit);
+  };
+  // Values that no row of the tile sees may be anything, and 0 times infinity is
+  // not 0: where they share a key tile with seen ones (the walk's first and last
+  // tile at most) they are cleared.  Past the last key the loads bring zeros.
+  auto edge = [&](int j) {
+    const int key0 = (k_first + j) * kKeys;
+    return key0 < r.min_lo || (key0 + kKeys > r.max_hi && r.max_hi < s.Sk);
+  };
+
   if (warp == 0) {
-    if (lane == 0 && n > 0) {
-      tma_prefetch_desc(&tm_q);
-      tma_prefetch_desc(&tm_k);
-      tma_prefetch_desc(&tm_v);
-      mbar_arrive_expect_tx(&bars->q_full, C::kQBytes);
-      for (int c = 0; c < HD / 64; ++c) tma_load_4d(qs + c * kTile * 128, &tm_q, 64 * c, h0, t0, b, &bars->q_full);
-      bool ok = true;
+    if (n > 0) {
+      if (elected()) {
+        tma_prefetch_desc(&tm_q);
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
+        mbar_arrive_expect_tx(&bars->q_full, C::kQBytes);
+        for (int c = 0; c < HD / 64; ++c) tma_load_4d(qs + c * kTile * 128, &tm_q, 64 * c, h0, t0, b, &bars->q_full);
+      }
+      __syncwarp();
       int kn = 0, vn = 0;  // loads issued
-      for (int j = 0; j < n && ok; ++j) {
+      auto clear = [&](int j) -> bool {
+        const int st = j % C::kStages, key0 = (k_first + j) * kKeys;
+        if (!wait(&bars->v_full[st], j / C::kStages, kStatusTimeoutFull)) return false;
+        uint4* tile = reinterpret_cast<uint4*>(vs + st * C::kTileBytes);   // chunks of kKeys rows of 8
+        for (int i = lane; i < C::kTileBytes / 16; i += 32) {
+          const int key = key0 + (i >> 3) % kKeys;
+          if (key < r.min_lo || key >= r.max_hi) tile[i] = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->v_clear[j ? 1 : 0]);
+        return true;
+      };
+      for (int j = 0; j < n; ++j) {
         const int st = j % C::kStages;
-        const uint32_t ph = (j / C::kStages - 1) & 1;
         const int key = (k_first + j) * kKeys;
-        if (j >= C::kStages && !mbar_wait_short(&bars->k_empty[st], ph, abort_word, a.status, kStatusTimeoutEmpty))
-          break;
-        mbar_arrive_expect_tx(&bars->k_full[st], C::kTileBytes);
-        for (int c = 0; c < HD / 64; ++c)
-          tma_load_4d(ks + st * C::kTileBytes + c * kKeys * 128, &tm_k, 64 * c, kvh, key, b, &bars->k_full[st]);
+        // The first tile is cleared when the second's loads are under way.
+        if (j == 2 && edge(0) && !clear(0)) break;
+        if (j >= C::kStages && !wait(&bars->k_empty[st], j / C::kStages - 1, kStatusTimeoutEmpty)) break;
+        if (elected()) {
+          mbar_arrive_expect_tx(&bars->k_full[st], C::kTileBytes);
+          for (int c = 0; c < HD / 64; ++c)
+            tma_load_4d(ks + st * C::kTileBytes + c * kKeys * 128, &tm_k, 64 * c, kvh, key, b, &bars->k_full[st]);
+        }
+        __syncwarp();
         ++kn;
-        if (j >= C::kStages && !mbar_wait_short(&bars->v_empty[st], ph, abort_word, a.status, kStatusTimeoutEmpty))
-          break;
-        mbar_arrive_expect_tx(&bars->v_full[st], C::kTileBytes);
-        for (int c = 0; c < HD / 64; ++c)
-          tma_load_4d(vs + st * C::kTileBytes + c * kKeys * 128, &tm_v, 64 * c, kvh, key, b, &bars->v_full[st]);
+        if (j >= C::kStages && !wait(&bars->v_empty[st], j / C::kStages - 1, kStatusTimeoutEmpty)) break;
+        if (elected()) {
+          mbar_arrive_expect_tx(&bars->v_full[st], C::kTileBytes);
+          for (int c = 0; c < HD / 64; ++c)
+            tma_load_4d(vs + st * C::kTileBytes + c * kKeys * 128, &tm_v, 64 * c, kvh, key, b, &bars->v_full[st]);
+        }
+        __syncwarp();
         ++vn;
+      }
+      if (vn == n) {
+        bool ok = n > 2 || !edge(0) || clear(0);
+        if (ok && n > 1 && edge(n - 1)) clear(n - 1);
       }
       // No copy may be in flight when the CTA leaves.
       uint32_t none = 0;
@@ -169,6 +207,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
         mbar_wait(&bars->k_full[i % C::kStages], (i / C::kStages) & 1, &none, a.status, kStatusTimeoutDrain);
       for (int i = max(vn - C::kStages, 0); i < vn; ++i)
         mbar_wait(&bars->v_full[i % C::kStages], (i / C::kStages) & 1, &none, a.status, kStatusTimeoutDrain);
+      __syncwarp();
     }
   } else if (warp == 1) {
     // The whole warp walks and one lane issues: operands stay uniform, and the
@@ -177,9 +216,6 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       const uint32_t id_s = idesc_bf16_f32(kTile, kKeys), id_o = idesc_bf16_f32_bmn(kTile, HD);
       const uint64_t dq = sdesc_kmajor_sw128(smem_u32(qs)), dk = sdesc_kmajor_sw128(smem_u32(ks));
       const uint64_t dv = cols_desc<kKeys>(smem_u32(vs));
-      auto wait = [&](uint64_t* bar, int phase, uint32_t bit) {
-        return mbar_wait_short_warp(bar, phase & 1, abort_word, a.status, bit);
-      };
       auto scores = [&](int j) -> bool {
         const int st = j % C::kStages;
         if (!wait(&bars->k_full[st], j / C::kStages, kStatusTimeoutFull)) return false;
@@ -196,6 +232,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       for (int j = 0; j < n && ok; ++j) {
         const int st = j % C::kStages;
         if (!wait(&bars->v_full[st], j / C::kStages, kStatusTimeoutFull) ||
+            ((j == 0 || j + 1 == n) && edge(j) && !wait(&bars->v_clear[j ? 1 : 0], 0, kStatusTimeoutFull)) ||
             !wait(&bars->p_full[j & 1], j >> 1, kStatusTimeoutFull))
           break;
         tc_fence_after();

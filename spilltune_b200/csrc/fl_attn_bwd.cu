@@ -69,7 +69,8 @@ constexpr int kColP = 128, kColAcc = 256;   // TMEM: S, P', the two accumulators
 // What the dk/dv kernel needs of 128 packed query rows, left by the dq kernel
 // and loaded with the tile: -lse log2(e), -delta, begin and end of each row,
 // then {max begin, min end} of each kCols rows inside the sequence.  Rows
-// past the sequence get a first entry of -inf, which makes p 0.
+// past the sequence get a first entry of -inf, which makes p 0, and the range
+// (-1, -1); of no rows inside the sequence, max begin is kNone - 1.
 struct __align__(16) RowInfo {
   float nlse2[kTile], ndelta[kTile];
   int lo[kTile], hi[kTile];
@@ -504,6 +505,37 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           break;
         }
         tc_fence_after();
+        // 0 times infinity is not 0: what no row of this tile (dq) or no key at all
+        // (dk, dv) meets but shares a streamed tile with what is met is cleared.
+        // S has been read by now, P' is waited for where its operand is cleared.
+        if constexpr (kDq) {
+          const int from = it.seen.min_lo - (col0 - mine0), to = it.seen.max_hi - (col0 - mine0);
+          if (from > 0 || (to < kTile && it.seen.max_hi < s.Sk)) {
+            uint4* tile = reinterpret_cast<uint4*>(bs + st * 2 * C::kBytes);   // chunks of kTile rows of 8
+            for (int e = threadIdx.x - 64; e < C::kBytes / 16; e += 128 * kGroups) {
+              const int at_row = (e >> 3) % kTile;
+              if (at_row < from || at_row >= to) tile[e] = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+          }
+        } else if (cols.max_lo[group] == kNone) {    // some row sees nothing
+          // (past the sequence the loads brought zeros)
+          const int first = cols.lo[mine0 + lane];
+          const uint32_t none = __ballot_sync(0xffffffffu, first >= cols.hi[mine0 + lane] && first >= 0);
+          if (none) {
+            if (!wait(&bars->dp_full, g, kStatusTimeoutAccum)) {
+              ok = false;
+              break;
+            }
+            // Each of the group's warps clears its 8 of the 32 rows, in both operands.
+            uint4* tile = reinterpret_cast<uint4*>(bs + st * 2 * C::kBytes);
+            for (int e = lane; e < 2 * HD / 64 * 64; e += 32) {
+              const int at_row = quarter * 8 + ((e >> 3) & 7);
+              if (none >> at_row & 1) tile[((e >> 6) * kTile + mine0 + at_row) * 8 + (e & 7)] = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+          }
+        }
         // dq: from the row's token to the first key; else from the row's key to the first token.
         [[maybe_unused]] const float dist0 = static_cast<float>((kDq ? tok - col0 : col0 - key) + s.Sk - s.Sq);
         const uint32_t at_s = tmem + kCols * group + lanes, at_p = at_s + kColP;
@@ -585,6 +617,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (hide[e]) p[e] = 0.f;
+            if constexpr (kCap) {                  // f of a hidden score may not be finite
+#pragma unroll
+              for (int h = 0; h < 4; h += 2) {
+                float f_0, f_1;
+                unpair(f[h / 2], f_0, f_1);
+                f[h / 2] = pair(hide[h] ? 0.f : f_0, hide[h + 1] ? 0.f : f_1);
+              }
+            }
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[c + e] = __float_as_uint(p[e]);
@@ -690,21 +730,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         dsum = 0.f;
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) dsum += sums[q * kTile + row];
-        fix = d0 - dsum;
+        fix = lo < hi ? d0 - dsum : 0.f;             // a row that sees nothing: whatever its dout
         RowInfo* o = a.info + (static_cast<int64_t>(b) * heads + it.hg) * a.q_tiles + it.tile;
         if (group == 0) {
           o->nlse2[row] = tok < s.Sq ? -lse2 : -INFINITY;
           o->ndelta[row] = tok < s.Sq ? -dsum : 0.f;
         } else if (group == 1) {
-          o->lo[row] = lo;
-          o->hi[row] = hi;
+          o->lo[row] = tok < s.Sq ? lo : -1;         // (-1, -1): past the sequence
+          o->hi[row] = tok < s.Sq ? hi : -1;
         } else if (kSlope && group == 2) {
           o->slope2[row] = row_slope2;
         }
         if (quarter == 0) {
           const Range h = tile_range(s, b, row0 + (mine0 >> s.lgp), max(kCols >> s.lgp, 1));
           if (lane == 0) {
-            o->max_lo[group] = h.max_lo;
+            // None inside the sequence: -inf + NaN is not masked, so not whole either.
+            o->max_lo[group] = h.min_hi == kNone ? kNone - 1 : h.max_lo;
             o->min_hi[group] = h.min_hi;
             if (it.hg == 0 && group == 0) a.ranges[static_cast<int64_t>(b) * a.q_tiles + it.tile] = it.seen;
           }

@@ -210,6 +210,46 @@ def test_values_out_of_sight(cuda_lib):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,K,D,cap,slopes", [(4, 2, 64, 0.0, False), (8, 2, 128, 0.0, False), (6, 2, 128, 0.0, True),
+                                              (8, 1, 80, 30.0, False), (4, 4, 64, 20.0, True)])
+def test_padding_that_is_not_finite(cuda_lib, H, K, D, cap, slopes):
+    """Keys, values, queries and gradients of padding tokens may be anything, also
+    where the padding begins inside a tile: the other results are the same bits."""
+    from spilltune_b200 import attention
+    B, S = 3, 200
+    q, k, v, do = _inputs(B, S, S, H, K, D, 6)
+    sl = 2.0 ** -(1.0 + torch.arange(H, device="cuda").float() * 7 / H) if slopes else None
+    begin, end = (x.cuda() for x in attention.row_ranges(B, S, lengths=torch.tensor([130, 65, 0])))
+    want = _both(q, k, v, begin, end, do, cap, sl)
+    bad = [x.clone() for x in (q, k, v, do)]
+    for i, x in enumerate(bad):
+        for b, live in enumerate((130, 65, 0)):
+            x[b, live:] = (float("nan"), float("inf"), float("-inf"))[(b + i) % 3]
+    got = _both(*bad[:3], begin, end, bad[3], cap, sl)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq", [1, 4])
+def test_cache_that_is_not_filled(cuda_lib, Sq):
+    """A few tokens over a long cache of which the first and the last rows hold anything."""
+    from spilltune_b200 import attention
+    B, Sk, H, K, D = 2, 4000, 8, 2, 128
+    q, k, v, _ = _inputs(B, Sq, Sk, H, K, D, 7)
+    begin = torch.tensor([[5], [70]], dtype=torch.int32, device="cuda").expand(B, Sq)
+    end = torch.tensor([[3001], [90]], dtype=torch.int32, device="cuda") + \
+        torch.arange(Sq, dtype=torch.int32, device="cuda")
+    want = attention.fwd(q, k, v, begin, end)
+    for b in range(B):
+        for x in (k, v):
+            x[b, :int(begin[b, 0])] = float("nan")
+            x[b, int(end[b, -1]):] = float("inf")
+    got = attention.fwd(q, k, v, begin, end)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
 def test_empty_rows_and_rows_behind_the_last(cuda_lib):
     """Rows that see nothing: zero output and gradient, log sum -inf; empty inputs."""
     from spilltune_b200 import attention
