@@ -328,9 +328,10 @@ int fl_rotary_bwd(const uint16_t* dq, int64_t dq_token_stride, int64_t dq_head_s
  *   begin, end  int32 [B, Sq];  slopes fp32 [Hq] or NULL;
  *   out         bf16 [B, Sq, Hq, D];  lse fp32 [B, Sq, Hq], the natural log of
  *               the softmax's denominator.
- * Values in keys no row sees do not reach the result where whole 128-key tiles
- * are unseen; inside a tile that some row sees they must be finite (a product
- * with the probability 0), as in the eager form.
+ * Keys and values before the first or behind the last key that a sequence's
+ * rows see, rows that see none and their dout may hold anything; keys in between
+ * have to be finite (a product with the probability 0).  softcap is 0 or at most
+ * 1024: the tanh's error of 3e-7 times the cap is the score's.
  * fl_attn_bwd: dq, dk, dv (contiguous bf16) from dout; out and lse as the
  * forward left them.  No atomics: equal inputs give equal bits.
  * Workspaces: the *_workspace_bytes sizes, 16-byte aligned.

@@ -23,6 +23,7 @@ from . import _lib
 from .ops import _need_cuda, _ptr, on_device, stream_of
 
 MAX_HEAD_DIM = 128
+MAX_SOFTCAP = 1024  # the tanh's error times the cap is the score's
 
 
 def row_ranges(batch, length, *, documents=None, prefix=None, window=None, lengths=None, causal=True, device=None):
@@ -106,8 +107,8 @@ def _check(q, k, v, begin, end, scale, softcap, slopes):
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError("scale must be positive and finite")
     softcap = float(softcap or 0.0)
-    if not (softcap >= 0 and math.isfinite(softcap)) or softcap and scale / softcap > 1e30:
-        raise ValueError("softcap must be 0, or finite and not too small for the scale")
+    if not 0 <= softcap <= MAX_SOFTCAP or softcap and scale / softcap > 1e30:
+        raise ValueError(f"softcap must be 0, or at most {MAX_SOFTCAP} and not too small for the scale")
     return dev, B, Sq, Sk, Hq, Hkv, D, scale, softcap
 
 
@@ -122,10 +123,10 @@ def fwd(q, k, v, begin, end, *, scale=None, softcap=0.0, slopes=None):
 
     begin, end: int32 [B, Sq], the keys each query sees (see ``row_ranges``); a
     query that sees none gets 0 and a log sum of -inf.
-    Keys and values that no query sees, queries that see none and their
-    gradients may hold anything, NaN too; a key that one query sees has to be
-    finite for the queries around it as well (0 times infinity).
-    scale: of q . k, default D ** -0.5.  softcap > 0: softcap * tanh(x / softcap).
+    Keys and values before the first or behind the last that a sequence's
+    queries see, queries that see none and their gradients may hold anything,
+    NaN too; a key in between has to be finite (0 times infinity).
+    scale: of q . k, default D ** -0.5.  softcap in (0, 1024]: softcap * tanh(x / softcap).
     slopes: fp32 [Hq]; x -= slopes[h] * |i + Sk - Sq - j|."""
     dev, B, Sq, Sk, Hq, Hkv, D, scale, softcap = _check(q, k, v, begin, end, scale, softcap, slopes)
     out = q.new_empty((B, Sq, Hq, D))

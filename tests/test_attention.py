@@ -464,6 +464,28 @@ def test_c_entry_refusals():
 
 
 @pytest.mark.gpu
+def test_large_cap(cuda_lib):
+    """At the largest cap a score is off by the tanh's error (under 2^-21: an
+    exponential, a sum and a reciprocal of half a step to two steps of 2^-24 each
+    around 1) times the cap, 2^-11: a probability by less than bf16's half step.
+    Larger caps are refused."""
+    from spilltune_b200 import attention
+    B, S, H, K, D = 1, 150, 4, 2, 64
+    q, k, v, _ = _inputs(B, S, S, H, K, D, 8)
+    begin, end = (x.cuda() for x in _ranges("causal", B, S, S, 8))
+    got = _both(q, k, v, begin, end, None, cap=1024.0)
+    want = _oracle(q, k, v, begin, end, D ** -0.5, 1024.0, None)
+    assert float((got["lse"].double() - want["lse"][0]).abs().max()) <= 2.0 ** -11 + 2.0 ** -18
+    out, vmax = want["out"][0], float(v.double().abs().max())
+    # twice the scores' error (numerator and sum), P's and the result's rounding
+    assert float((got["out"].double() - out).abs().max()) <= vmax * (2 * 2.0 ** -11 + 2.0 ** -8 + 2.0 ** -8)
+    with pytest.raises(ValueError, match="softcap"):
+        attention.fwd(q, k, v, begin, end, softcap=1025.0)
+    with pytest.raises(ValueError, match="softcap"):
+        attention.fwd(q, k, v, begin, end, softcap=float("inf"))
+
+
+@pytest.mark.gpu
 def test_refusals(cuda_lib):
     from spilltune_b200 import attention
     q, k, v, do = _inputs(1, 8, 8, 4, 2, 64, 1)
