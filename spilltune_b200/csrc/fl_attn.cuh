@@ -187,6 +187,16 @@ __device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a_tmem, uint64_t b
            accumulate || kk != 0);
 }
 
+// The part of the same product that takes half of each group's columns (kGroup = 32: 16 of them).
+template <int HD, int kRows, int kGroup>
+__device__ __forceinline__ void mma_cols_half(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, int half,
+                                              bool accumulate) {
+  static_assert(kGroup == 32, "two slices of 16 to a group");
+#pragma unroll
+  for (int kk = 0; kk < kRows / 16; kk += 2)
+    mma_ts(d, a_tmem + kk * 16 + half * 8, b + (kk + half) * (2048 >> 4), idesc, accumulate || kk + half != 0);
+}
+
 int packed_log2(int Hq, int Hkv);
 // Row tiles of kTile packed rows over all heads and sequences.
 int64_t fwd_ctas(int B, int Sq, int Hq, int Hkv);

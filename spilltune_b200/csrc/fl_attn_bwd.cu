@@ -38,6 +38,9 @@
 // * One elected lane of a warp that walks as one issues them: a divergent lane's
 //   operands went through vector registers, 120 cycles from one product to the
 //   next beside busy element warps (dq 391 -> 321 us).
+// * The second product of a pair starts when half of its operand is there (16 of
+//   a group's 32 columns): dk/dv 296 -> 279 us, 262 -> 223 us where documents
+//   make short walks; no gain for dq.
 // * A quarter of the exponentials (half under a cap, whose tanh takes two more
 //   results) run on the FMA pipes.
 // * The columns' statistics come with their tile by a bulk copy, left in that
@@ -120,7 +123,7 @@ struct __align__(16) BwdBars {
   uint64_t a_full, a_empty;
   uint64_t b_full[2][2], b_empty[2][2];   // [B1, B2][stage]
   uint64_t s_full, dp_full;               // S, P' written
-  uint64_t p_full, ds_full;               // p, ds written over them
+  uint64_t p_full[2], ds_full[2];         // p, ds written over them: half of each group's columns, all
   uint64_t acc1_done, acc2_done;
   uint64_t acc_full, acc_empty;           // accumulators summed, read
   uint64_t met;                           // dq: the element warps among themselves
@@ -181,8 +184,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
     mbar_init(&bars->s_full, 1);
     mbar_init(&bars->dp_full, 1);
-    mbar_init(&bars->p_full, 4 * kGroups);
-    mbar_init(&bars->ds_full, 4 * kGroups);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->p_full[i], 4 * kGroups);
+      mbar_init(&bars->ds_full[i], 4 * kGroups);
+    }
     mbar_init(&bars->acc1_done, 1);
     mbar_init(&bars->acc2_done, 1);
     mbar_init(&bars->acc_full, 1);
@@ -370,31 +375,38 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       ok = wait(&bars->a_full, k, kStatusTimeoutFull) && scores(g0, 0, false) && scores(g0, 1, n == 1);
       for (int i = 0; i < n && ok; ++i) {
         const int g = g0 + i, st = g % C::kStages;
-        if (!wait(&bars->p_full, g, kStatusTimeoutFull) ||
-            (i == 0 && k > 0 && !wait(&bars->acc_empty, k - 1, kStatusTimeoutAccum))) {
-          ok = false;
-          break;
+        // Each product in two parts: the first runs while the other half of its
+        // operand is still computed.
+        for (int half = 0; half < 2 && ok; ++half) {
+          ok = wait(&bars->p_full[half], g, kStatusTimeoutFull) &&
+               (half || i > 0 || k == 0 || wait(&bars->acc_empty, k - 1, kStatusTimeoutAccum));
+          if (!ok) break;
+          tc_fence_after();
+          if (elected()) {
+            mma_cols_half<HD, kTile, kCols>(tmem + kColAcc, col_s, d_cols + at(g, kDq ? 0 : 1), id_acc, half, i > 0);
+            if (half) {
+              tc_commit(&bars->b_empty[1][st]);
+              tc_commit(&bars->acc1_done);
+            }
+          }
+          __syncwarp();
         }
-        tc_fence_after();
-        if (elected()) {
-          mma_cols<HD, kTile, kCols>(tmem + kColAcc, col_s, d_cols + at(g, kDq ? 0 : 1), id_acc, i > 0);
-          tc_commit(&bars->b_empty[1][st]);
-          tc_commit(&bars->acc1_done);
+        ok = ok && (i + 1 == n || scores(g + 1, 0, false));
+        for (int half = 0; half < 2 && ok; ++half) {
+          ok = wait(&bars->ds_full[half], g, kStatusTimeoutFull);
+          if (!ok) break;
+          tc_fence_after();
+          if (elected()) {
+            mma_cols_half<HD, kTile, kCols>(tmem + kColAcc + HD, col_p, d_cols + at(g, 0), id_acc, half, i > 0);
+            if (half) {
+              tc_commit(&bars->b_empty[0][st]);
+              tc_commit(&bars->acc2_done);
+              if (i + 1 == n) tc_commit(&bars->acc_full);
+            }
+          }
+          __syncwarp();
         }
-        __syncwarp();
-        if (i + 1 < n && !scores(g + 1, 0, false)) ok = false;
-        if (!ok || !wait(&bars->ds_full, g, kStatusTimeoutFull)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        if (elected()) {
-          mma_cols<HD, kTile, kCols>(tmem + kColAcc + HD, col_p, d_cols + at(g, 0), id_acc, i > 0);
-          tc_commit(&bars->b_empty[0][st]);
-          tc_commit(&bars->acc2_done);
-          if (i + 1 == n) tc_commit(&bars->acc_full);
-        }
-        __syncwarp();
+        if (!ok) break;
         if (i + 1 < n && !scores(g + 1, 1, i + 2 == n)) ok = false;
       }
       g0 += n;
@@ -539,7 +551,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         // dq: from the row's token to the first key; else from the row's key to the first token.
         [[maybe_unused]] const float dist0 = static_cast<float>((kDq ? tok - col0 : col0 - key) + s.Sk - s.Sq);
         const uint32_t at_s = tmem + kCols * group + lanes, at_p = at_s + kColP;
-        uint32_t x[kCols], w[kCols / 2];             // scores, then p; packed operands
+        uint32_t x[kCols], w[kCols / 4];             // scores, then p; half the packed operands
         [[maybe_unused]] __half2 fac[kCap ? kCols / 2 : 1];
         tmem_ld_32x32b_x32(at_s, x);
         tmem_wait_ld();
@@ -638,21 +650,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
               if constexpr (kDq) unpair(mul2(pair(p[h], p[h + 1]), f[h / 2]), p[h], p[h + 1]);
             }
           }
-          w[c / 2] = pack_bf16x2(p[0], p[1]);
-          w[c / 2 + 1] = pack_bf16x2(p[2], p[3]);
+          w[c % 16 / 2] = pack_bf16x2(p[0], p[1]);
+          w[c % 16 / 2 + 1] = pack_bf16x2(p[2], p[3]);
         };
-        if (whole) {
+        // The operands' first or second half (of the group's columns) to TMEM.
+        auto hand_over = [&](uint32_t at_w, uint64_t* bar) {
+          tmem_st_32x32b_x8(at_w, w);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar);
+        };
 #pragma unroll
-          for (int c = 0; c < kCols; c += 4) exponentials(c, std::false_type{});
-        } else {
+        for (int c0 = 0; c0 < kCols; c0 += 16) {
+          if (whole) {
 #pragma unroll
-          for (int c = 0; c < kCols; c += 4) exponentials(c, std::true_type{});
+            for (int c = 0; c < 16; c += 4) exponentials(c0 + c, std::false_type{});
+          } else {
+#pragma unroll
+            for (int c = 0; c < 16; c += 4) exponentials(c0 + c, std::true_type{});
+          }
+          hand_over(at_s + c0 / 2, &bars->p_full[c0 / 16]);
         }
-        tmem_st_32x32b_x16(at_s, w);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->p_full);
 
         if (!wait(&bars->dp_full, g, kStatusTimeoutAccum)) {
           ok = false;
@@ -695,7 +714,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
               if (hide[h]) ds[0] = 0.f;
               if (hide[h + 1]) ds[1] = 0.f;
             }
-            w[col / 2] = pack_bf16x2(ds[0], ds[1]);
+            w[col % 16 / 2] = pack_bf16x2(ds[0], ds[1]);
           }
         };
 #pragma unroll
@@ -710,12 +729,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
             for (int c = 0; c < 16; c += 4) gradients(y + c, c0 + c, std::true_type{});
           }
+          hand_over(at_p + c0 / 2, &bars->ds_full[c0 / 16]);
         }
-        tmem_st_32x32b_x16(at_p, w);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->ds_full);
       }
       g0 += it.n;
       float fix = 0.f;
