@@ -38,6 +38,10 @@
 // * One elected lane of a warp that walks as one issues them: a divergent lane's
 //   operands went through vector registers, 120 cycles from one product to the
 //   next beside busy element warps (dq 391 -> 321 us).
+// * Shared memory is declared aligned, not aligned by hand: a pointer that went
+//   through an integer is generic to the compiler (64-bit, and its accesses
+//   slower), and 96 registers had no room for that: dk/dv 278 -> 235 us, no
+//   spills.  The slack saved lets dq keep a third key tile (303 -> 280 us).
 // * The second product of a pair starts when half of its operand is there (16 of
 //   a group's 32 columns): dk/dv 296 -> 279 us, 262 -> 223 us where documents
 //   make short walks; no gain for dq.
@@ -82,11 +86,15 @@ struct __align__(16) RowInfo {
 };
 constexpr int kInfoBytes = sizeof(RowInfo);
 
-template <int HD>
+template <int HD, bool kDq>
 struct Bwd {
-  static constexpr int kStages = 2;
+  // Of B1 and B2.  dq has no row infos to keep (but sums, and dots of do and o),
+  // which leaves room for a third tile of keys: all 227 KB of an SM.
+  static constexpr int kStages[2] = {kDq ? 3 : 2, 2};
   static constexpr int kBytes = HD / 64 * kTile * 128;     // a tile of 128 rows
-  static constexpr int kSmem = 1024 + (2 + 2 * kStages) * kBytes + kStages * kInfoBytes + 512;
+  static constexpr int kExtra = kDq ? (kGroups + 1) * kTile * static_cast<int>(sizeof(float)) : 2 * kInfoBytes;
+  static constexpr int kSmem = (2 + kStages[0] + kStages[1]) * kBytes + kExtra + 512;
+  static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
 struct BwdArgs {
@@ -121,7 +129,7 @@ struct Item {
 struct __align__(16) BwdBars {
   uint64_t item_full[2], item_empty[2];
   uint64_t a_full, a_empty;
-  uint64_t b_full[2][2], b_empty[2][2];   // [B1, B2][stage]
+  uint64_t b_full[2][3], b_empty[2][3];   // [B1, B2][stage]
   uint64_t s_full, dp_full;               // S, P' written
   uint64_t p_full[2], ds_full[2];         // p, ds written over them: half of each group's columns, all
   uint64_t acc1_done, acc2_done;
@@ -151,15 +159,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant__ CUtensorMap tm_a2,
                const __grid_constant__ CUtensorMap tm_b1, const __grid_constant__ CUtensorMap tm_b2,
                const BwdArgs a) {
-  using C = Bwd<HD>;
+  using C = Bwd<HD, kDq>;
+  constexpr int kS1 = C::kStages[0], kS2 = C::kStages[1];
   constexpr bool kBias = kMode != kPlain, kCap = has_cap(kMode), kSlope = has_slopes(kMode);
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* a1 = smem;
   uint8_t* a2 = a1 + C::kBytes;
-  uint8_t* bs = a2 + C::kBytes;                            // [stage][B1, B2]
-  RowInfo* info = reinterpret_cast<RowInfo*>(bs + C::kStages * 2 * C::kBytes);   // [stage]
-  BwdBars* bars = reinterpret_cast<BwdBars*>(info + C::kStages);
+  uint8_t* bs = a2 + C::kBytes;                            // B1 [stage], B2 [stage]
+  uint8_t* extra = bs + (kS1 + kS2) * C::kBytes;
+  RowInfo* info = reinterpret_cast<RowInfo*>(extra);       // dk, dv: [stage of B1]
+  BwdBars* bars = reinterpret_cast<BwdBars*>(extra + C::kExtra);
   volatile uint32_t* abort_word = &bars->abort_word;
   // Broadcast so that the compiler knows a warp to be of one mind.
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -177,8 +186,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     mbar_init(&bars->a_full, 1);
     mbar_init(&bars->a_empty, 1);
-    for (int i = 0; i < C::kStages; ++i)
-      for (int o = 0; o < 2; ++o) {
+    for (int o = 0; o < 2; ++o)
+      for (int i = 0; i < (o ? kS2 : kS1); ++i) {
         mbar_init(&bars->b_full[o][i], 1);
         mbar_init(&bars->b_empty[o][i], 1);
       }
@@ -306,16 +315,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       bool ok = true;
       Walk at(it);
       for (int i = 0; i < it.n && ok; ++i, ++g, at.step(it)) {
-        const int st = g % C::kStages;
         const int bh = kDq ? kvh : kvh * G + at.group * pg;
         const int br = kDq ? (it.first + i) * kTile : at.tile * q_step;
         for (int o = 0; o < 2 && ok; ++o) {
-          if (g >= C::kStages && !wait(&bars->b_empty[o][st], g / C::kStages - 1, kStatusTimeoutEmpty)) {
+          const int stages = o ? kS2 : kS1, st = g % stages;
+          if (g >= stages && !wait(&bars->b_empty[o][st], g / stages - 1, kStatusTimeoutEmpty)) {
             ok = false;
             break;
           }
           if (elected()) {
-            uint8_t* dst = bs + (st * 2 + o) * C::kBytes;
+            uint8_t* dst = bs + (o * kS1 + st) * C::kBytes;
             mbar_arrive_expect_tx(&bars->b_full[o][st], C::kBytes + (!kDq && o == 0 ? kInfoBytes : 0));
             if (!kDq && o == 0)
               bulk_load(info + st,
@@ -335,8 +344,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     uint32_t none = 0;
     if (loads_a) mbar_wait(&bars->a_full, (loads_a - 1) & 1, &none, a.status, kStatusTimeoutDrain);
     for (int o = 0; o < 2; ++o)
-      for (int i = max(loads_b[o] - C::kStages, 0); i < loads_b[o]; ++i)
-        mbar_wait(&bars->b_full[o][i % C::kStages], (i / C::kStages) & 1, &none, a.status, kStatusTimeoutDrain);
+      for (int stages = o ? kS2 : kS1, i = max(loads_b[o] - stages, 0); i < loads_b[o]; ++i)
+        mbar_wait(&bars->b_full[o][i % stages], (i / stages) & 1, &none, a.status, kStatusTimeoutDrain);
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------- products
@@ -346,14 +355,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const uint32_t col_s = tmem, col_p = tmem + kColP;
     const uint64_t d_a[2] = {sdesc_kmajor_sw128(smem_u32(a1)), sdesc_kmajor_sw128(smem_u32(a2))};
     const uint64_t d_rows = sdesc_kmajor_sw128(smem_u32(bs)), d_cols = cols_desc<kTile>(smem_u32(bs));
-    auto at = [&](int g, int o) { return static_cast<uint64_t>((g % C::kStages) * 2 + o) * (C::kBytes >> 4); };
+    auto at = [&](int g, int o) {
+      return static_cast<uint64_t>(o ? kS1 + g % kS2 : g % kS1) * (C::kBytes >> 4);
+    };
     int g0 = 0, k = 0;       // steps and items with steps before this one
     bool issued = false;
     // S (o = 0) or P' (o = 1) of step g, once the products that read the p or
     // ds in its columns are done; the item's last P' frees the resident tiles.
     auto scores = [&](int g, int o, bool last) -> bool {
       if (g > 0 && !wait(o ? &bars->acc2_done : &bars->acc1_done, g - 1, kStatusTimeoutAccum)) return false;
-      if (!wait(&bars->b_full[o][g % C::kStages], g / C::kStages, kStatusTimeoutFull)) return false;
+      const int stages = o ? kS2 : kS1;
+      if (!wait(&bars->b_full[o][g % stages], g / stages, kStatusTimeoutFull)) return false;
       tc_fence_after();
       if (elected()) {
         mma_rows<HD, kTile>(o ? col_p : col_s, d_a[o], d_rows + at(g, o), id_s);
@@ -374,7 +386,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (n == 0) continue;
       ok = wait(&bars->a_full, k, kStatusTimeoutFull) && scores(g0, 0, false) && scores(g0, 1, n == 1);
       for (int i = 0; i < n && ok; ++i) {
-        const int g = g0 + i, st = g % C::kStages;
+        const int g = g0 + i;
         // Each product in two parts: the first runs while the other half of its
         // operand is still computed.
         for (int half = 0; half < 2 && ok; ++half) {
@@ -385,7 +397,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           if (elected()) {
             mma_cols_half<HD, kTile, kCols>(tmem + kColAcc, col_s, d_cols + at(g, kDq ? 0 : 1), id_acc, half, i > 0);
             if (half) {
-              tc_commit(&bars->b_empty[1][st]);
+              tc_commit(&bars->b_empty[1][g % kS2]);
               tc_commit(&bars->acc1_done);
             }
           }
@@ -399,7 +411,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           if (elected()) {
             mma_cols_half<HD, kTile, kCols>(tmem + kColAcc + HD, col_p, d_cols + at(g, 0), id_acc, half, i > 0);
             if (half) {
-              tc_commit(&bars->b_empty[0][st]);
+              tc_commit(&bars->b_empty[0][g % kS1]);
               tc_commit(&bars->acc2_done);
               if (i + 1 == n) tc_commit(&bars->acc_full);
             }
@@ -457,7 +469,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const float lse = a.lse[at * s.Hq + head];
         // d0 = do . o: 16 lanes to a row, two rows of a warp at a time, handed to
         // the rows' owners through shared memory.
-        float* dots = reinterpret_cast<float*>(info + 1) + (turn & 1) * kTile;
+        // (read before the item's second meeting, written after it)
+        float* dots = reinterpret_cast<float*>(extra) + kGroups * kTile;
         const bool in_row = (lane & 15) * 8 < s.D;
         const int d = in_row ? (lane & 15) * 8 : 0;
         constexpr int kRounds = kTile / (8 * kGroups);
@@ -489,11 +502,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       bool ok = true;
       Walk at(it);
       for (int i = 0; i < it.n; ++i, at.step(it)) {
-        const int g = g0 + i, st = g % C::kStages;
-        const RowInfo& cols = info[st];              // dk, dv: of the step's columns
+        const int g = g0 + i, st = g % kS1;
+        const RowInfo& cols = info[kDq ? 0 : st];              // dk, dv: of the step's columns
         bool whole;
         int col0;                                    // dq: the group's first key; else its first token
-        if (!kDq && !wait(&bars->b_full[0][st], g / C::kStages, kStatusTimeoutFull)) {
+        if (!kDq && !wait(&bars->b_full[0][st], g / kS1, kStatusTimeoutFull)) {
           ok = false;
           break;
         }
@@ -523,7 +536,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if constexpr (kDq) {
           const int from = it.seen.min_lo - (col0 - mine0), to = it.seen.max_hi - (col0 - mine0);
           if (from > 0 || (to < kTile && it.seen.max_hi < s.Sk)) {
-            uint4* tile = reinterpret_cast<uint4*>(bs + st * 2 * C::kBytes);   // chunks of kTile rows of 8
+            uint4* tile = reinterpret_cast<uint4*>(bs + st * C::kBytes);   // chunks of kTile rows of 8
             for (int e = threadIdx.x - 64; e < C::kBytes / 16; e += 128 * kGroups) {
               const int at_row = (e >> 3) % kTile;
               if (at_row < from || at_row >= to) tile[e] = make_uint4(0, 0, 0, 0);
@@ -540,10 +553,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
               break;
             }
             // Each of the group's warps clears its 8 of the 32 rows, in both operands.
-            uint4* tile = reinterpret_cast<uint4*>(bs + st * 2 * C::kBytes);
-            for (int e = lane; e < 2 * HD / 64 * 64; e += 32) {
-              const int at_row = quarter * 8 + ((e >> 3) & 7);
-              if (none >> at_row & 1) tile[((e >> 6) * kTile + mine0 + at_row) * 8 + (e & 7)] = make_uint4(0, 0, 0, 0);
+            for (int o = 0; o < 2; ++o) {
+              uint4* tile = reinterpret_cast<uint4*>(bs + (o ? kS1 + g % kS2 : st) * C::kBytes);
+              for (int e = lane; e < HD; e += 32) {            // chunks of 64 columns, rows, pieces of 16 bytes
+                const int at_row = quarter * 8 + ((e >> 3) & 7);
+                if (none >> at_row & 1) tile[((e >> 6) * kTile + mine0 + at_row) * 8 + (e & 7)] = make_uint4(0, 0, 0, 0);
+              }
             }
             fence_proxy_async_smem();
           }
@@ -738,8 +753,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         // Each group summed delta over its columns.
         float dsum, odd;
         unpair(dsum2, dsum, odd);
-        float* sums = reinterpret_cast<float*>(info);   // [kGroups][128]
-        static_assert(kGroups * kTile * sizeof(float) <= kInfoBytes, "the sums use the first row info's space");
+        float* sums = reinterpret_cast<float*>(extra);   // [kGroups][128]
         sums[group * kTile + row] = dsum + odd;
         if (!ok || !meet()) break;
         dsum = 0.f;
@@ -873,10 +887,10 @@ int bwd_parts(int64_t key_ctas, int64_t steps) {
 template <int HD, bool kDq, int kMode>
 int launch_bwd(const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1, const CUtensorMap& b2,
                const BwdArgs& a, cudaStream_t stream) {
-  int rc = allow_smem(reinterpret_cast<const void*>(&bwd_kernel<HD, kDq, kMode>), Bwd<HD>::kSmem);
+  int rc = allow_smem(reinterpret_cast<const void*>(&bwd_kernel<HD, kDq, kMode>), Bwd<HD, kDq>::kSmem);
   if (rc) return rc;
   const int64_t grid = a.items < a.sms ? a.items : a.sms;
-  bwd_kernel<HD, kDq, kMode><<<static_cast<unsigned>(grid), kBwdThreads, Bwd<HD>::kSmem, stream>>>(a1, a2, b1, b2, a);
+  bwd_kernel<HD, kDq, kMode><<<static_cast<unsigned>(grid), kBwdThreads, Bwd<HD, kDq>::kSmem, stream>>>(a1, a2, b1, b2, a);
   return FL_OK;
 }
 
