@@ -47,7 +47,7 @@ struct Fwd {
   static constexpr int kStages = HD == 64 ? 4 : 2;       // K and V tiles in flight
   static constexpr int kQBytes = HD / 64 * kTile * 128;
   static constexpr int kTileBytes = HD / 64 * kKeys * 128;
-  static constexpr int kSmem = 1024 + kQBytes + 2 * kStages * kTileBytes + 256;
+  static constexpr int kSmem = kQBytes + 2 * kStages * kTileBytes + 256;
   static constexpr int kTmem = 256;                      // two S (P over each) + O
 };
 
@@ -76,8 +76,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
                const __grid_constant__ CUtensorMap tm_v, const FwdArgs a) {
   using C = Fwd<HD>;
   constexpr bool kBias = kMode != kPlain;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* qs = smem;
   uint8_t* ks = qs + C::kQBytes;
   uint8_t* vs = ks + C::kStages * C::kTileBytes;
