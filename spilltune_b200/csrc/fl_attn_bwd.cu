@@ -30,21 +30,14 @@
 // S, P' and the accumulators fill TMEM, so nothing is double-buffered; the order
 // acc1(i), S(i + 1), acc2(i), P'(i + 1) keeps the tensor cores on one pair while
 // the sixteen element warps (four to each 32 columns) work on the other.  What
-// bounds a step is that chain: S 720 cycles from issue to arrival, exponentials
-// 1000 - 1500, acc1 900; 3280 cycles a step (dq) and 3570 (dk, dv), where the
-// four products take 2048.
+// bounds a step is that chain (measured before the two steps at the end of this
+// list: S 720 cycles from issue to arrival, exponentials 1000 - 1500, acc1 900;
+// 3280 cycles a step in dq and 3570 in dk/dv, where the four products take 2048).
 // * Products are 128 columns wide: with 64, the fetch of the resident operand
 //   makes a product take 48 cycles where 32 would do (measured back to back).
 // * One elected lane of a warp that walks as one issues them: a divergent lane's
 //   operands went through vector registers, 120 cycles from one product to the
 //   next beside busy element warps (dq 391 -> 321 us).
-// * Shared memory is declared aligned, not aligned by hand: a pointer that went
-//   through an integer is generic to the compiler (64-bit, and its accesses
-//   slower), and 96 registers had no room for that: dk/dv 278 -> 235 us, no
-//   spills.  The slack saved lets dq keep a third key tile (303 -> 280 us).
-// * The second product of a pair starts when half of its operand is there (16 of
-//   a group's 32 columns): dk/dv 296 -> 279 us, 262 -> 223 us where documents
-//   make short walks; no gain for dq.
 // * A quarter of the exponentials (half under a cap, whose tanh takes two more
 //   results) run on the FMA pipes.
 // * The columns' statistics come with their tile by a bulk copy, left in that
@@ -52,8 +45,15 @@
 //   step.
 // * CTAs are persistent: the next item's loads, scores and products start while
 //   the last one's results are stored.
-// Measured at 4 x 2048 causal tokens, 32/8 heads of 128: dq 300 us, dk/dv 295 us
-// (five products at 550 TFLOP/s; the eight that run at 880, 53% of the burst
+// * The second product of a pair starts when half of its operand is there (16 of
+//   a group's 32 columns): dk/dv 296 -> 279 us, 262 -> 223 us where documents
+//   make short walks; no gain for dq.
+// * Shared memory is declared aligned, not aligned by hand: a pointer that went
+//   through an integer is generic to the compiler (64-bit, and its accesses
+//   slower), and 96 registers had no room for that: dk/dv 278 -> 235 us, no
+//   spills.  The slack saved lets dq keep a third key tile (303 -> 280 us).
+// Measured at 4 x 2048 causal tokens, 32/8 heads of 128: dq 266 us, dk/dv 236 us
+// (five products at 685 TFLOP/s; the eight that run at 1096, 66% of the burst
 // rate of a bf16 GEMM).
 // bf16 p and ds are the products' operands: half a step of each term, of the
 // same size as rounding the result.
@@ -446,12 +446,47 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (lane == 0) mbar_arrive(&bars->met);
       return wait(&bars->met, meetings++, kStatusTimeoutAccum);
     };
-    for (int turn = 0;; ++turn) {
-      if (!wait(&bars->item_full[turn & 1], turn >> 1, kStatusTimeoutFull)) break;
-      const Item it = bars->item[turn & 1];
+    // dq: what the item's rows need from memory.  Every load at once, from the
+    // last row where there is none.  Of do and o 16 lanes have a row, two rows to a
+    // warp.  kAhead: for the next item before this one's results are stored (at
+    // the end of the work the first tile's: always, so that the registers are
+    // free in between; 280 -> 266 us, short walks of documents 203 -> 184).  Not
+    // under a cap, whose registers it would spill (105 -> 110 us).
+    constexpr bool kAhead = kDq && !kCap;
+    constexpr int kRounds = kTile / (8 * kGroups);
+    [[maybe_unused]] uint4 do_row[kDq ? kRounds : 1], o_row[kDq ? kRounds : 1];
+    [[maybe_unused]] int row_begin = 0, row_end = 0;
+    [[maybe_unused]] float row_lse = 0.f;
+    const bool in_row = (lane & 15) * 8 < s.D;
+    auto fetch = [&](const Item& it) {
+      const int last = s.Sq - 1, row0 = max(it.tile, 0) * q_step, d = in_row ? (lane & 15) * 8 : 0;
+      const int64_t tokens = static_cast<int64_t>(it.b) * s.Sq;
+      const int64_t at = tokens + min(row0 + (row >> s.lgp), last);
+      row_begin = s.begin[at], row_end = s.end[at];
+      row_lse = a.lse[at * s.Hq + (it.hg << s.lgp) + (row & (pg - 1))];
+#pragma unroll
+      for (int i = 0; i < kRounds; ++i) {
+        const int rr = ((warp - 2) * kRounds + i) * 2 + (lane >> 4);
+        const int rt = min(row0 + (rr >> s.lgp), last), rh = (it.hg << s.lgp) + (rr & (pg - 1));
+        do_row[i] = *reinterpret_cast<const uint4*>(a.dout + it.b * a.do_batch + rt * a.do_token + rh * a.do_head + d);
+        o_row[i] = *reinterpret_cast<const uint4*>(a.out + ((tokens + rt) * s.Hq + rh) * s.D + d);
+      }
+    };
+    auto take = [&](int turn, Item& it) -> bool {
+      if (!wait(&bars->item_full[turn & 1], turn >> 1, kStatusTimeoutFull)) return false;
+      it = bars->item[turn & 1];
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->item_empty[turn & 1]);
+      return true;
+    };
+    Item it{-1};
+    const bool begun = !kAhead || take(0, it);
+    if constexpr (kAhead) fetch(it);
+    for (int turn = 0; begun; ++turn) {
+      if constexpr (!kAhead)
+        if (!take(turn, it)) break;
       if (it.tile < 0) break;
+      if constexpr (kDq && !kAhead) fetch(it);
       const int kvh = kDq ? it.hg / s.groups : it.hg, b = it.b;
       const int row0 = it.tile * (kDq ? q_step : kTile);
       // dq: the row's token, head, range and statistics; else the row's key.
@@ -462,35 +497,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if constexpr (kDq) {
         tok = row0 + (row >> s.lgp);
         head = (it.hg << s.lgp) + (row & (pg - 1));
-        // Every load first, from the last row where there is none: one latency, not four.
-        const int last = s.Sq - 1;
-        const int64_t at = static_cast<int64_t>(b) * s.Sq + min(tok, last);
-        const int begin = s.begin[at], end = s.end[at];
-        const float lse = a.lse[at * s.Hq + head];
-        // d0 = do . o: 16 lanes to a row, two rows of a warp at a time, handed to
-        // the rows' owners through shared memory.
-        // (read before the item's second meeting, written after it)
+        // d0 = do . o, handed to the rows' owners through shared memory (read before
+        // the item's second meeting, written after it).
         float* dots = reinterpret_cast<float*>(extra) + kGroups * kTile;
-        const bool in_row = (lane & 15) * 8 < s.D;
-        const int d = in_row ? (lane & 15) * 8 : 0;
-        constexpr int kRounds = kTile / (8 * kGroups);
-        uint4 x[kRounds], y[kRounds];
-#pragma unroll
-        for (int i = 0; i < kRounds; ++i) {
-          const int rr = ((warp - 2) * kRounds + i) * 2 + (lane >> 4);
-          const int rt = min(row0 + (rr >> s.lgp), last), rh = (it.hg << s.lgp) + (rr & (pg - 1));
-          x[i] = *reinterpret_cast<const uint4*>(a.dout + b * a.do_batch + rt * a.do_token + rh * a.do_head + d);
-          y[i] = *reinterpret_cast<const uint4*>(a.out + ((static_cast<int64_t>(b) * s.Sq + rt) * s.Hq + rh) * s.D + d);
-        }
         if (tok < s.Sq) {
-          lo = max(begin, 0);
-          hi = min(end, s.Sk);
+          lo = max(row_begin, 0);
+          hi = min(row_end, s.Sk);
           if (lo >= hi) lo = hi = 0;
-          lse2 = lse * kLog2e;
+          lse2 = row_lse * kLog2e;
         }
 #pragma unroll
         for (int i = 0; i < kRounds; ++i) {
-          float sum = in_row ? dot8(x[i], y[i]) : 0.f;
+          float sum = in_row ? dot8(do_row[i], o_row[i]) : 0.f;
 #pragma unroll
           for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
           if ((lane & 15) == 0) dots[((warp - 2) * kRounds + i) * 2 + (lane >> 4)] = sum;
@@ -770,15 +788,24 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         } else if (kSlope && group == 2) {
           o->slope2[row] = row_slope2;
         }
-        if (quarter == 0) {
-          const Range h = tile_range(s, b, row0 + (mine0 >> s.lgp), max(kCols >> s.lgp, 1));
+        if (group == 3) {
+          // The rows of a quarter are a group's columns there.  None inside the
+          // sequence: -inf + NaN is not masked, so not whole either.
+          static_assert(kCols == 32 && kGroups == 4, "a quarter's rows");
+          const bool in = tok < s.Sq;
+          const int max_lo = __reduce_max_sync(0xffffffffu, !in ? -1 : lo < hi ? lo : kNone);
+          const int min_hi = __reduce_min_sync(0xffffffffu, !in ? kNone : hi);
           if (lane == 0) {
-            // None inside the sequence: -inf + NaN is not masked, so not whole either.
-            o->max_lo[group] = h.min_hi == kNone ? kNone - 1 : h.max_lo;
-            o->min_hi[group] = h.min_hi;
-            if (it.hg == 0 && group == 0) a.ranges[static_cast<int64_t>(b) * a.q_tiles + it.tile] = it.seen;
+            o->max_lo[quarter] = min_hi == kNone ? kNone - 1 : max_lo;
+            o->min_hi[quarter] = min_hi;
+            if (it.hg == 0 && quarter == 0) a.ranges[static_cast<int64_t>(b) * a.q_tiles + it.tile] = it.seen;
           }
         }
+      }
+      [[maybe_unused]] Item next;
+      if constexpr (kAhead) {
+        if (!take(turn + 1, next)) break;            // (after a wait that gave up, dq has left above)
+        fetch(next);
       }
       if (it.n > 0) {
         ok = ok && wait(&bars->acc_full, k, kStatusTimeoutAccum);
@@ -847,6 +874,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->acc_empty);
       }
+      if constexpr (kAhead) it = next;
     }
   }
 
