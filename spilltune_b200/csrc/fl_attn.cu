@@ -237,9 +237,9 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
         tc_fence_after();
         if (elected()) {
           const uint32_t p = tmem_s + (j & 1) * kKeys;
-          mma_cols<HD, kKeys, kKeys>(tmem_o, p, dv + st * (C::kTileBytes >> 4), id_o, j > 0);
+          mma_cols<HD, kKeys>(tmem_o, p, dv + st * (C::kTileBytes >> 4), id_o, j > 0);
           if constexpr (kFine)
-            mma_cols<HD, kKeys, kKeys>(tmem_o, p + kKeys / 2, dv + st * (C::kTileBytes >> 4), id_o, true);
+            mma_cols<HD, kKeys>(tmem_o, p + kKeys / 2, dv + st * (C::kTileBytes >> 4), id_o, true);
           tc_commit(&bars->v_empty[st]);
           tc_commit(&bars->pv_done);
         }

@@ -171,27 +171,25 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, uin
            kk != 0);
 }
 
-// D[128 x HD] (+)= A . B: A bf16 [128 x kRows] in TMEM, each kGroup columns of A
-// from a_tmem + kGroup * group on; B [kRows x HD] in shared memory (the same
-// chunks, read with the columns as the MN side), b from cols_desc<kRows>.
-// kGroup = kRows: A is packed.
+// D[128 x HD] (+)= A . B: A bf16 [128 x kRows] in TMEM; B [kRows x HD] in shared
+// memory (the same chunks, read with the columns as the MN side), b from
+// cols_desc<kRows>.
 template <int kRows>
 __device__ __forceinline__ uint64_t cols_desc(uint32_t addr) {
   return sdesc_mnmajor_sw128(addr, kRows * 128, 1024);
 }
-template <int HD, int kRows, int kGroup>
+template <int HD, int kRows>
 __device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, bool accumulate) {
 #pragma unroll
   for (int kk = 0; kk < kRows / 16; ++kk)
-    mma_ts(d, a_tmem + kk * 16 / kGroup * kGroup + kk * 16 % kGroup / 2, b + kk * (2048 >> 4), idesc,
-           accumulate || kk != 0);
+    mma_ts(d, a_tmem + kk * 8, b + kk * (2048 >> 4), idesc, accumulate || kk != 0);
 }
 
-// The part of the same product that takes half of each group's columns (kGroup = 32: 16 of them).
-template <int HD, int kRows, int kGroup>
+// The part of that product that takes the first or second 16 of every 32 columns
+// of A, which lie in the first half of the 32 columns of FP32 that they were.
+template <int HD, int kRows>
 __device__ __forceinline__ void mma_cols_half(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, int half,
                                               bool accumulate) {
-  static_assert(kGroup == 32, "two slices of 16 to a group");
 #pragma unroll
   for (int kk = 0; kk < kRows / 16; kk += 2)
     mma_ts(d, a_tmem + kk * 16 + half * 8, b + (kk + half) * (2048 >> 4), idesc, accumulate || kk + half != 0);

@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           if (!ok) break;
           tc_fence_after();
           if (elected()) {
-            mma_cols_half<HD, kTile, kCols>(tmem + kColAcc, col_s, d_cols + at(g, kDq ? 0 : 1), id_acc, half, i > 0);
+            mma_cols_half<HD, kTile>(tmem + kColAcc, col_s, d_cols + at(g, kDq ? 0 : 1), id_acc, half, i > 0);
             if (half) {
               tc_commit(&bars->b_empty[1][g % kS2]);
               tc_commit(&bars->acc1_done);
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           if (!ok) break;
           tc_fence_after();
           if (elected()) {
-            mma_cols_half<HD, kTile, kCols>(tmem + kColAcc + HD, col_p, d_cols + at(g, 0), id_acc, half, i > 0);
+            mma_cols_half<HD, kTile>(tmem + kColAcc + HD, col_p, d_cols + at(g, 0), id_acc, half, i > 0);
             if (half) {
               tc_commit(&bars->b_empty[0][g % kS1]);
               tc_commit(&bars->acc2_done);
@@ -915,10 +915,11 @@ int bwd_parts(int64_t key_ctas, int64_t steps) {
 template <int HD, bool kDq, int kMode>
 int launch_bwd(const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1, const CUtensorMap& b2,
                const BwdArgs& a, cudaStream_t stream) {
-  int rc = allow_smem(reinterpret_cast<const void*>(&bwd_kernel<HD, kDq, kMode>), Bwd<HD, kDq>::kSmem);
+  constexpr int kSmem = Bwd<HD, kDq>::kSmem;
+  int rc = allow_smem(reinterpret_cast<const void*>(&bwd_kernel<HD, kDq, kMode>), kSmem);
   if (rc) return rc;
   const int64_t grid = a.items < a.sms ? a.items : a.sms;
-  bwd_kernel<HD, kDq, kMode><<<static_cast<unsigned>(grid), kBwdThreads, Bwd<HD, kDq>::kSmem, stream>>>(a1, a2, b1, b2, a);
+  bwd_kernel<HD, kDq, kMode><<<static_cast<unsigned>(grid), kBwdThreads, kSmem, stream>>>(a1, a2, b1, b2, a);
   return FL_OK;
 }
 
