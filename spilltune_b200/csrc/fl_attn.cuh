@@ -92,8 +92,9 @@ __device__ __forceinline__ float rcp(float x) {
 // 2^x of two values without the special-function unit, whose 16 results a
 // cycle and SM bound the exponentials: x = i + f with i the nearest integer
 // (by adding 1.5 * 2^23), 2^f on [-1/2, 1/2] by the polynomial of degree 5 with
-// value 1 at 0 whose largest relative error is smallest (1.1e-7, less than the
-// special-function unit's), i added to the exponent.  x <= -127 gives 0.
+// value 1 at 0 whose largest relative error is smallest (1.1e-7), times 2^i, whose
+// bits are made from those of i.  x under -126.5 gives 0; a product and not an
+// addition to the exponent's bits, so that NaN stays NaN.
 __device__ __forceinline__ void ex2_pair(float x0, float x1, float& y0, float& y1) {
   const float round = 12582912.0f;
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-127.0f));
@@ -109,9 +110,9 @@ __device__ __forceinline__ void ex2_pair(float x0, float x1, float& y0, float& y
   p = fma2(f, p, pair(1.0f, 1.0f));
   float i0, i1;
   unpair(i, i0, i1);
-  unpair(p, y0, y1);
-  y0 = __int_as_float(__float_as_int(y0) + (__float_as_int(i0) << 23));
-  y1 = __int_as_float(__float_as_int(y1) + (__float_as_int(i1) << 23));
+  i0 = __int_as_float((__float_as_int(i0) << 23) + 0x3F800000);
+  i1 = __int_as_float((__float_as_int(i1) << 23) + 0x3F800000);
+  unpair(mul2(p, pair(i0, i1)), y0, y1);
 }
 
 // What is done to a score before the softmax.

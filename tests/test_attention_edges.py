@@ -1,0 +1,63 @@
+"""Calls of spilltune_b200.attention at the edge of what it takes: scores that are not numbers."""
+import pytest
+import torch
+
+
+def _inputs(B, Sq, Sk, H, K, D, seed):
+    g = torch.Generator().manual_seed(seed)
+    bf = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16).cuda()  # noqa: E731
+    return bf(B, Sq, H, D), bf(B, Sk, K, D), bf(B, Sk, K, D), bf(B, Sq, H, D)
+
+
+def _all_keys(B, Sq, Sk):
+    begin = torch.zeros(B, Sq, dtype=torch.int32, device="cuda")
+    return begin, begin + Sk
+
+
+MODES = [(0.0, False), (30.0, False), (0.0, True), (30.0, True)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap,slopes", MODES)
+@pytest.mark.parametrize("Sq,Sk,H,K,D", [(40, 40, 4, 2, 64), (20, 150, 3, 3, 128), (1, 2000, 8, 2, 64)])
+def test_a_key_that_is_not_a_number(cuda_lib, Sq, Sk, H, K, D, cap, slopes):
+    """One NaN key that every row sees, at each place among eight neighbouring columns of a score tile: every log
+    sum and result of its heads is NaN, and those of the other heads are what they were."""
+    from spilltune_b200 import _lib, attention
+    q, k, v, _ = _inputs(1, Sq, Sk, H, K, D, Sk)
+    begin, end = _all_keys(1, Sq, Sk)
+    opt = dict(softcap=cap, slopes=torch.full((H,), 0.01, device="cuda") if slopes else None)
+    want = attention.fwd(q, k, v, begin, end, **opt)
+    G = H // K
+    for at in list(range(8)) + [Sk - 1]:
+        bad = k.clone()
+        bad[:, at, 0] = float("nan")
+        out, lse = attention.fwd(q, bad, v, begin, end, **opt)
+        assert bool(lse[:, :, :G].isnan().all()) and bool(out[:, :, :G].isnan().all()), at
+        assert torch.equal(lse[:, :, G:], want[1][:, :, G:]) and torch.equal(out[:, :, G:], want[0][:, :, G:]), at
+    assert _lib.status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap,slopes", MODES)
+@pytest.mark.parametrize("S,H,K,D", [(40, 2, 2, 64), (150, 4, 2, 128)])
+def test_a_query_that_is_not_a_number(cuda_lib, S, H, K, D, cap, slopes):
+    """A NaN query of one head: NaN in its own row, its own gradient and the gradients of every key it sees (of its
+    key/value head), and nowhere else."""
+    from spilltune_b200 import _lib, attention
+    q, k, v, do = _inputs(1, S, S, H, K, D, S)
+    begin, end = _all_keys(1, S, S)
+    opt = dict(softcap=cap, slopes=torch.full((H,), 0.01, device="cuda") if slopes else None)
+    for at in range(8):
+        bad = q.clone()
+        bad[:, at, 0] = float("nan")
+        out, lse = attention.fwd(bad, k, v, begin, end, **opt)
+        dq, dk, dv = attention.bwd(do, bad, k, v, out, lse, begin, end, **opt)
+        hit = torch.zeros(1, S, H, dtype=torch.bool, device="cuda")
+        hit[:, at, 0] = True
+        assert torch.equal(lse.isnan(), hit), at
+        for x in (out, dq):
+            assert torch.equal(x.isnan(), hit[..., None].expand_as(x)), at
+        for x in (dk, dv):
+            assert bool(x[:, :, 0].isnan().all()) and not bool(x[:, :, 1:].isnan().any()), at
+    assert _lib.status() == 0
