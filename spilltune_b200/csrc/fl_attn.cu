@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
 #pragma unroll
         for (int i = 0; i < kKeys; i += 2) {
           uint64_t x = pair(v[i], v[i + 1]);
-          x = has_cap(kMode) ? capped2(s, cap_r2(s, x), cap2_2) : mul2(x, sl2_2);
+          x = has_cap(kMode) ? capped2(s, cap_r2(cap_u2(cap_arg2(s, x))), cap2_2) : mul2(x, sl2_2);
           if constexpr (has_slopes(kMode))
             x = fma2(pair(-slope2, -slope2), pair(fabsf(from_key0 - i), fabsf(from_key0 - (i + 1))), x);
           float x0, x1;

@@ -120,22 +120,42 @@ enum Mode : int { kPlain = 0, kSlopes = 1, kCapped = 2, kCappedSlopes = 3 };
 __host__ __device__ constexpr bool has_cap(int mode) { return mode >= kCapped; }
 __host__ __device__ constexpr bool has_slopes(int mode) { return mode == kSlopes || mode == kCappedSlopes; }
 
-// The cap, from r = 1 / (1 + 2^(2 y log2 e)): tanh(y) = 1 - 2 r with an absolute
-// error of a few 1e-7 everywhere, which the cap multiplies (the hardware's tanh
-// would leave 2^-11 of the cap); its derivative is 1 - tanh^2(y) = 4 r (1 - r).
-// r of two scores:
-__device__ __forceinline__ uint64_t cap_r2(const Shape& s, uint64_t qk) {
+// The cap, from u = 2^(2 y log2 e) and r = 1 / (1 + u): tanh(y) = 1 - 2 r with an
+// absolute error of a few 1e-7 everywhere, which the cap multiplies (the hardware's
+// tanh would leave 2^-11 of the cap); its derivative is 1 - tanh^2(y) = 4 r (u r),
+// to a few 1e-6 of itself on either side (1 - r would leave nothing of it where r
+// is near 1).  2 y log2 e of two scores, and r of it:
+__device__ __forceinline__ uint64_t cap_arg2(const Shape& s, uint64_t qk) {
+  return mul2(qk, pair(s.icap2, s.icap2));
+}
+__device__ __forceinline__ uint64_t cap_u2(uint64_t arg) {
   float y0, y1;
-  unpair(mul2(qk, pair(s.icap2, s.icap2)), y0, y1);
-  unpair(add2(pair(ex2(y0), ex2(y1)), pair(1.0f, 1.0f)), y0, y1);
+  unpair(arg, y0, y1);
+  return pair(ex2(y0), ex2(y1));
+}
+__device__ __forceinline__ uint64_t cap_r2(uint64_t u) {
+  float y0, y1;
+  unpair(add2(u, pair(1.0f, 1.0f)), y0, y1);
   return pair(rcp(y0), rcp(y1));
 }
 // cap log2(e) tanh + add:
 __device__ __forceinline__ uint64_t capped2(const Shape& s, uint64_t r, uint64_t add) {
   return fma2(r, pair(-2.0f * s.cap2, -2.0f * s.cap2), add);   // add: with cap2 in it
 }
-__device__ __forceinline__ uint64_t cap_slope2(uint64_t r) {
-  return mul2(r, fma2(r, pair(-4.0f, -4.0f), pair(4.0f, 4.0f)));
+// The derivative times 2^15: between the two places that use it it is held in fp16,
+// whose 11 bits then reach down to 2^-29 (scores of 10.7 caps; at 1 they would end at
+// 2^-14, 5.5 caps); dp - delta is formed over 2^15 for it.
+constexpr float kCapSlope = 32768.0f;
+// u of an argument for it: finite, so that r is not 0 and u r is 1 at the far end.
+__device__ __forceinline__ uint64_t cap_u2_finite(uint64_t arg) {
+  float y0, y1;
+  unpair(arg, y0, y1);
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(y0) : "f"(126.0f));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(y1) : "f"(126.0f));
+  return pair(ex2(y0), ex2(y1));
+}
+__device__ __forceinline__ uint64_t cap_slope2(uint64_t r, uint64_t u) {
+  return mul2(mul2(r, pair(4.0f * kCapSlope, 4.0f * kCapSlope)), mul2(u, r));
 }
 
 // A small non-negative integer as a float without the conversion unit (which

@@ -74,7 +74,8 @@ constexpr int kTmemCols = 512;
 constexpr int kColP = 128, kColAcc = 256;   // TMEM: S, P', the two accumulators
 
 // What the dk/dv kernel needs of 128 packed query rows, left by the dq kernel
-// and loaded with the tile: -lse log2(e), -delta, begin and end of each row,
+// and loaded with the tile: -lse log2(e), -delta (over kCapSlope under a cap,
+// as dp there), begin and end of each row,
 // then {max begin, min end} of each kCols rows inside the sequence.  Rows
 // past the sequence get a first entry of -inf, which makes p 0, and the range
 // (-1, -1); of no rows inside the sequence, max begin is kNone - 1.
@@ -625,9 +626,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
               const int col = c + h;
               uint64_t e = pair(x[col], x[col + 1]);
               if constexpr (kCap) {
-                const uint64_t r = cap_r2(s, e);
+                const uint64_t u = cap_u2_finite(cap_arg2(s, e)), r = cap_r2(u);
                 e = capped2(s, r, add2(nl[h / 2], pair(s.cap2, s.cap2)));
-                f[h / 2] = cap_slope2(r);
+                f[h / 2] = cap_slope2(r, u);
               } else {
                 e = fma2(e, sl2_2, nl[h / 2]);
               }
@@ -674,7 +675,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[c + e] = __float_as_uint(p[e]);
           if constexpr (kCap) {
-            // f waits for dp in 16 bits: 2^-12 of a factor of ds, an eighth of ds's own rounding.
+            // f, 2^15 times the derivative, waits for dp in 16 bits: half a step, 2^-11 of a
+            // factor of ds, an eighth of ds's own rounding, up to scores of 10.7 caps.
 #pragma unroll
             for (int h = 0; h < 4; h += 2) {
               float f_0, f_1;
@@ -713,9 +715,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_after();
         // dp of the columns c .. c + 3 in y; ds into w.
         auto gradients = [&](const uint32_t* y, int c, auto masked) {
-          uint64_t nd[2];                            // -delta of the columns
+          uint64_t nd[2];                            // -delta of the columns, times unit
+          constexpr float unit = kCap ? 1.0f / kCapSlope : 1.0f;
           if constexpr (kDq) {
-            nd[0] = nd[1] = pair(-d0, -d0);
+            nd[0] = nd[1] = pair(-d0 * unit, -d0 * unit);
           } else {
             const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(cols.ndelta + mine0 + c);
             nd[0] = v.x, nd[1] = v.y;
@@ -736,13 +739,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                 dsum2 = fma2(p, dp, dsum2);
               }
             }
-            uint64_t pf = p;
+            float ds[2];
             if constexpr (kCap) {
               const float2 f = __half22float2(fac[col / 2]);
-              pf = mul2(p, pair(f.x, f.y));
+              unpair(mul2(mul2(p, pair(f.x, f.y)), fma2(dp, pair(unit, unit), nd[h / 2])), ds[0], ds[1]);
+            } else {
+              unpair(mul2(p, add2(dp, nd[h / 2])), ds[0], ds[1]);
             }
-            float ds[2];
-            unpair(mul2(pf, add2(dp, nd[h / 2])), ds[0], ds[1]);
             if constexpr (decltype(masked)::value) {
               if (hide[h]) ds[0] = 0.f;
               if (hide[h + 1]) ds[1] = 0.f;
@@ -778,10 +781,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) dsum += sums[q * kTile + row];
         fix = lo < hi ? d0 - dsum : 0.f;             // a row that sees nothing: whatever its dout
+        if constexpr (kCap) fix *= 1.0f / kCapSlope; // the sum of p f k has it
         RowInfo* o = a.info + (static_cast<int64_t>(b) * heads + it.hg) * a.q_tiles + it.tile;
         if (group == 0) {
           o->nlse2[row] = tok < s.Sq ? -lse2 : -INFINITY;
-          o->ndelta[row] = tok < s.Sq ? -dsum : 0.f;
+          o->ndelta[row] = tok < s.Sq ? -dsum * (kCap ? 1.0f / kCapSlope : 1.0f) : 0.f;
         } else if (group == 1) {
           o->lo[row] = tok < s.Sq ? lo : -1;         // (-1, -1): past the sequence
           o->hi[row] = tok < s.Sq ? hi : -1;

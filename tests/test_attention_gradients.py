@@ -111,3 +111,39 @@ def test_delta_is_not_taken_from_the_rounded_output(cuda_lib, B, S, H, K, D, wid
         over = (got[n].double() - value).abs() - bound
         assert bool((over <= 0).all()), (n, float(over.max()), int((over > 0).sum()))
         assert bool(((wrong - value).abs() > bound).any()), n
+
+
+def _saturated(B, S, H, K, D, cap, times, seed):
+    """Scores of about `times` caps, mostly within a tenth."""
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    side = (abs(times) * cap * D ** -0.5) ** 0.5   # q . k D^-1/2 = side^2 D^1/2
+    q = side * (1 + 0.1 * n(B, S, H, D)) * (-1 if times < 0 else 1)
+    k = side * (1 + 0.05 * n(B, S, K, 1) + 0.1 * n(B, S, K, D))
+    return [x.to(torch.bfloat16) for x in (q, k, n(B, S, K, D), n(B, S, H, D))]
+
+
+SATURATED = [  # B, S, H, K, D, cap, scores in caps, slopes
+    (1, 70, 4, 2, 64, 20.0, 6.0, False),
+    (1, 70, 4, 2, 128, 30.0, 8.0, False),
+    (2, 150, 6, 2, 64, 20.0, -7.0, False),
+    (1, 140, 2, 2, 80, 50.0, -8.0, False),
+    (1, 90, 8, 1, 64, 10.0, 7.0, True),
+    (1, 200, 4, 4, 64, 20.0, 9.0, False),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,H,K,D,cap,times,slopes", SATURATED)
+def test_gradients_of_scores_far_over_their_cap(cuda_lib, B, S, H, K, D, cap, times, slopes):
+    """f = 1 - tanh^2 is 2e-5 at six caps, 6e-8 at nine, to either side: its relative error is what counts.  Held
+    as it is in 16 bits it would be off by more than these bounds from 8 caps on."""
+    q, k, v, do = (x.cuda() for x in _saturated(B, S, H, K, D, cap, times, S + D))
+    begin, end = (x.cuda() for x in _short_rows(B, S, 4, "window"))
+    sl = 2.0 ** -(4.0 + torch.arange(H, device="cuda").float() * 4 / H) if slopes else None
+    out, got = _run(q, k, v, begin, end, do, softcap=cap, slopes=sl)
+    coarse = _gradients(q, k, v, begin, end, do, out, cap, sl, half_f=True)
+    for n, (value, bound, _) in _gradients(q, k, v, begin, end, do, out, cap, sl).items():
+        over = (got[n].double() - value).abs() - bound
+        assert bool((over <= 0).all()), (n, float(over.max()), int((over > 0).sum()))
+        assert bool(((coarse[n][0] - value).abs() > bound).any()) or abs(times) < 8, n
