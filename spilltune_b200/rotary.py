@@ -256,8 +256,10 @@ class _Rotary(torch.autograd.Function):
         weights = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
         gq, gk, gqw, gkw = bwd(dq, dk, q, k, positions, inv_freq, q_weight=q_weight, k_weight=k_weight,
                                weight_grads=weights, **ctx.opt)
+        # a key norm's weight without keys has no part in the result: no gradient
         return (gq, gk, gqw.to(q_weight.dtype) if ctx.needs_input_grad[2] else None,
-                gkw.to(k_weight.dtype) if ctx.needs_input_grad[3] else None, None, None, None, None, None)
+                gkw.to(k_weight.dtype) if ctx.needs_input_grad[3] and gkw is not None else None,
+                None, None, None, None, None)
 
 
 def rotate(q, k, positions, inv_freq, *, interleaved=False, factor=1.0):

@@ -1,0 +1,24 @@
+"""Calls of spilltune_b200.rotary at the edge of what it takes."""
+import pytest
+import torch
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 40])
+def test_norm_of_queries_only_with_trainable_weights(cuda_lib, D):
+    """Without keys the key norm's weight has no part in the result: the other gradients are those of the call
+    without it, and it gets none."""
+    from spilltune_b200 import rotary
+    g = torch.Generator().manual_seed(D)
+    q = torch.randn(21, 3, D, generator=g).to(torch.bfloat16).cuda().requires_grad_(True)
+    dq = torch.randn(21, 3, D, generator=g).to(torch.bfloat16).cuda()
+    qw = (1 + 0.2 * torch.randn(D, generator=g)).cuda().requires_grad_(True)
+    kw = (1 + 0.2 * torch.randn(D, generator=g)).cuda().requires_grad_(True)
+    pos, inv = torch.arange(21, device="cuda"), rotary.frequencies(D)[0].cuda()
+    y, none = rotary.norm_rotate(q, None, qw, kw, pos, inv, eps=1e-6)
+    assert none is None
+    got = torch.autograd.grad(y, (q, qw, kw), dq, allow_unused=True)
+    want = torch.autograd.grad(rotary.norm_rotate(q, None, qw, None, pos, inv, eps=1e-6)[0], (q, qw), dq)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and got[2] is None
+    alone = torch.autograd.grad(rotary.norm_rotate(q, None, qw.detach(), kw, pos, inv, eps=1e-6)[0], q, dq)
+    assert torch.equal(alone[0], want[0])
