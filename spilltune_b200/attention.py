@@ -34,7 +34,7 @@ def row_ranges(batch, length, *, documents=None, prefix=None, window=None, lengt
     documents: int [batch, length] ids; a token sees its own document only (the
         tokens with its id around it, ids in runs).
     prefix: int [batch]; the first prefix[b] tokens are seen by every token of
-        their document.
+        their document.  Not with a window: that is not one range a row.
     window: int >= 1; only the last `window` tokens up to itself (causal masks).
     lengths: int [batch]; tokens from lengths[b] on are padding: they see
         nothing and nothing sees them."""
@@ -42,6 +42,8 @@ def row_ranges(batch, length, *, documents=None, prefix=None, window=None, lengt
         raise ValueError("batch and length must not be negative")
     if window is not None and (not causal or window < 1):
         raise ValueError("a window needs a causal mask and a size >= 1")
+    if window is not None and prefix is not None:
+        raise ValueError("unsupported_capability: a prefix with a window is not one range a row")
     given = [t for t in (documents, prefix, lengths) if t is not None]
     if device is None and given:
         device = given[0].device

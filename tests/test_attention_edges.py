@@ -1,4 +1,5 @@
-"""Calls of spilltune_b200.attention at the edge of what it takes: scores that are not numbers."""
+"""Calls of spilltune_b200.attention at the edge of what it takes: scores that are not numbers, masks that are
+not one range a row."""
 import pytest
 import torch
 
@@ -61,3 +62,12 @@ def test_a_query_that_is_not_a_number(cuda_lib, S, H, K, D, cap, slopes):
         for x in (dk, dv):
             assert bool(x[:, :, 0].isnan().all()) and not bool(x[:, :, 1:].isnan().any()), at
     assert _lib.status() == 0
+
+
+def test_a_prefix_with_a_window_is_refused():
+    """A token past its window would see the prefix and its last keys: two ranges."""
+    from spilltune_b200.attention import row_ranges
+    with pytest.raises(ValueError, match="unsupported_capability: .*prefix.*window"):
+        row_ranges(1, 10, prefix=torch.tensor([4]), window=2)
+    assert row_ranges(1, 4, prefix=torch.tensor([2]))[1].tolist() == [[2, 2, 3, 4]]
+    assert row_ranges(1, 4, window=2)[0].tolist() == [[0, 0, 1, 2]]
