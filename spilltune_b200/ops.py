@@ -33,13 +33,11 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
 def stream_of(device):
     """Handle of the current stream of `device`.  The raw query is what torch's own generated
-    code calls; building a Stream object around it takes 2 us, a tenth of a small call."""
-    return _raw_stream(device.index)
+    code calls; building a Stream object around it takes 2 us, a tenth of a small call.  Looked
+    up here: a torch built without CUDA does not have it."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def on_device(device, call, *args):
