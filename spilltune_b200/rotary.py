@@ -262,8 +262,15 @@ class _Rotary(torch.autograd.Function):
                 None, None, None, None, None)
 
 
+def _constant(inv_freq):
+    if inv_freq.requires_grad and torch.is_grad_enabled():
+        raise ValueError("unsupported_capability: inv_freq gets no gradient")
+
+
 def rotate(q, k, positions, inv_freq, *, interleaved=False, factor=1.0):
-    """fwd() without a norm, differentiable in q and k.  k None: returns (q', None)."""
+    """fwd() without a norm, differentiable in q and k (positions and frequencies are
+    constants).  k None: returns (q', None)."""
+    _constant(inv_freq)
     out = _Rotary.apply(q, k, None, None, positions, inv_freq, bool(interleaved), float(factor), None)
     return out[0], out[1] if k is not None else None
 
@@ -272,5 +279,6 @@ def norm_rotate(q, k, q_weight, k_weight, positions, inv_freq, *, eps, interleav
     """fwd() with the norm of every head, differentiable in q, k and the norm weights."""
     if q_weight is None:
         raise ValueError("norm_rotate needs the norm weights (rotate has none)")
+    _constant(inv_freq)
     out = _Rotary.apply(q, k, q_weight, k_weight, positions, inv_freq, bool(interleaved), float(factor), eps)
     return out[0], out[1] if k is not None else None

@@ -22,3 +22,15 @@ def test_norm_of_queries_only_with_trainable_weights(cuda_lib, D):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and got[2] is None
     alone = torch.autograd.grad(rotary.norm_rotate(q, None, qw.detach(), kw, pos, inv, eps=1e-6)[0], q, dq)
     assert torch.equal(alone[0], want[0])
+
+
+def test_frequencies_that_want_a_gradient_are_refused():
+    """Refused before anything else, so on the CPU too; without a graph they are numbers like any other."""
+    from spilltune_b200 import rotary
+    q, pos = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.arange(2)
+    inv, w = torch.ones(32, requires_grad=True), torch.ones(64)
+    for call in (lambda: rotary.rotate(q, q, pos, inv), lambda: rotary.norm_rotate(q, q, w, w, pos, inv, eps=1e-6)):
+        with pytest.raises(ValueError, match="unsupported_capability: inv_freq gets no gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA tensors"):
+            call()
