@@ -324,7 +324,7 @@ int fl_rotary_bwd(const uint16_t* dq, int64_t dq_token_stride, int64_t dq_head_s
  * q [B, Sq, Hq, D], k and v [B, Sk, Hkv, D] bf16 with element strides
  * (a HOST array: batch, token, head of q, k, v[, dout]; columns adjacent); head
  * h reads key/value head h / (Hq / Hkv).  D a multiple of 8, 8 <= D <= 128;
- * scale > 0; pointers 16-byte aligned, strides positive multiples of 8.
+ * 0 < scale <= 2.3e38; pointers 16-byte aligned, strides positive multiples of 8.
  *   begin, end  int32 [B, Sq];  slopes fp32 [Hq] or NULL;
  *   out         bf16 [B, Sq, Hq, D];  lse fp32 [B, Sq, Hq], the natural log of
  *               the softmax's denominator.

@@ -563,7 +563,8 @@ int attn_check(const char* who, int64_t B, int64_t Sq, int64_t Sk, int Hq, int H
   if (B > (1 << 16) || Sq > (1 << 30) || Sk > (1 << 30) || Hq > (1 << 12))
     return set_error(FL_ERR_ARG, "%s: batch, length or head count too large", who);
   if (D < 8 || D > 128 || D % 8) return set_error(FL_ERR_ARG, "%s: head size must be a multiple of 8 in [8, 128]", who);
-  if (!(scale > 0.f) || scale > 3.0e38f) return set_error(FL_ERR_ARG, "%s: scale must be positive and finite", who);
+  // scale log2(e) has to be finite.
+  if (!(scale > 0.f) || scale > 2.3e38f) return set_error(FL_ERR_ARG, "%s: scale must be in (0, 2.3e38]", who);
   // The tanh's error, a few 1e-7, times the cap stays under a quarter of P's half step.
   if (!(cap >= 0.f) || cap > 1024.f || (cap > 0.f && scale / cap > 1.0e30f))
     return set_error(FL_ERR_ARG, "%s: the cap must be 0, or at most 1024 and not too small for the scale", who);

@@ -71,3 +71,18 @@ def test_a_prefix_with_a_window_is_refused():
         row_ranges(1, 10, prefix=torch.tensor([4]), window=2)
     assert row_ranges(1, 4, prefix=torch.tensor([2]))[1].tolist() == [[2, 2, 3, 4]]
     assert row_ranges(1, 4, window=2)[0].tolist() == [[0, 0, 1, 2]]
+
+
+def test_c_entries_refuse_a_scale_whose_power_of_two_form_overflows():
+    """The kernels multiply by scale log2(e): from 2.36e38 on that is infinite, and a score of 0 NaN."""
+    import ctypes
+
+    from spilltune_b200 import _lib, build
+    build.build()
+    lib = _lib.load()
+    p, strides = 4096, (ctypes.c_int64 * 12)(*[512, 128, 64] * 4)  # p is never read: each call is refused first
+    for scale in (2.5e38, 3.4e38):
+        assert lib.fl_attn_fwd(p, p, p, strides, 1, 4, 4, 2, 2, 64, p, p, scale, 0.0, None, p, p, None, 0,
+                               None) == _lib.FL_ERR_ARG
+        assert lib.fl_attn_bwd(p, p, p, p, strides, p, p, 1, 4, 4, 2, 2, 64, p, p, scale, 0.0, None, p, p, p, p,
+                               1 << 20, None) == _lib.FL_ERR_ARG
