@@ -61,13 +61,13 @@ def frequencies(dim, theta=10000.0, scaling=None):
     if unknown or missing:
         raise ValueError(f"rotary scaling {kind!r}: missing {missing}, unknown {sorted(unknown)}")
     by = float(opt["factor"])
-    if not by >= 1.0:
-        raise ValueError("rotary scaling factor must be >= 1")
+    if not 1.0 <= by < math.inf:
+        raise ValueError("rotary scaling factor must be >= 1 and finite")
     if kind == "linear":
         return (inv / by).float(), 1.0
     length = float(opt["original_length"])
-    if not length > 0:
-        raise ValueError("rotary scaling original_length must be positive")
+    if not 0 < length < math.inf:
+        raise ValueError("rotary scaling original_length must be positive and finite")
     if kind == "llama3":
         low, high = float(opt["low_freq_factor"]), float(opt["high_freq_factor"])
         if not high > low > 0:
@@ -75,6 +75,8 @@ def frequencies(dim, theta=10000.0, scaling=None):
         turns = length * inv / (2 * math.pi)
         keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
         return (keep * inv + (1 - keep) * inv / by).float(), 1.0
+    if not theta > 1:
+        raise ValueError("rotary scaling 'yarn' needs theta > 1")
     fast, slow = float(opt.get("beta_fast", 32.0)), float(opt.get("beta_slow", 1.0))
     if not fast > slow > 0:
         raise ValueError("rotary scaling needs beta_fast > beta_slow > 0")

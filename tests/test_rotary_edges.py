@@ -34,3 +34,19 @@ def test_frequencies_that_want_a_gradient_are_refused():
             call()
         with torch.no_grad(), pytest.raises(ValueError, match="CUDA tensors"):
             call()
+
+
+@pytest.mark.parametrize("theta,scaling,match", [
+    (1.0, {"type": "yarn", "factor": 4.0, "original_length": 512}, "theta > 1"),
+    (0.5, {"type": "yarn", "factor": 4.0, "original_length": 512}, "theta > 1"),
+    (1e4, {"type": "yarn", "factor": float("inf"), "original_length": 512}, "factor"),
+    (1e4, {"type": "linear", "factor": float("inf")}, "factor"),
+    (1e4, {"type": "yarn", "factor": 4.0, "original_length": float("inf")}, "original_length"),
+    (1e4, {"type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+           "original_length": float("nan")}, "original_length")])
+def test_scalings_without_a_value_are_refused(theta, scaling, match):
+    """YaRN's ramp divides by ln(theta); an infinite factor or length leaves frequencies or cosines without a value."""
+    from spilltune_b200 import rotary
+    with pytest.raises(ValueError, match=match):
+        rotary.frequencies(64, theta, scaling)
+    assert bool(rotary.frequencies(64, 1.0)[0].eq(1).all())
