@@ -86,3 +86,31 @@ def test_c_entries_refuse_a_scale_whose_power_of_two_form_overflows():
                                None) == _lib.FL_ERR_ARG
         assert lib.fl_attn_bwd(p, p, p, p, strides, p, p, 1, 4, 4, 2, 2, 64, p, p, scale, 0.0, None, p, p, p, p,
                                1 << 20, None) == _lib.FL_ERR_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq", [1, 70])
+def test_offsets_past_32_bits(cuda_lib, Sq):
+    """The last keys of the second of two caches of 2^31 elements together and more: results and gradients are those
+    of these keys alone, and the other keys' gradients 0."""
+    from spilltune_b200 import _lib, attention
+    B, Sk, H, K, D, seen = 2, 280_001, 32, 32, 128, 90
+    assert (B - 0.5) * Sk * K * D > 2 ** 30 and B * Sk * K * D > 2 ** 31
+    q, k0, v0, do = _inputs(B, Sq, seen, H, K, D, 3)
+    k, v = (torch.zeros(B, Sk, K, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    k[:, Sk - seen:], v[:, Sk - seen:] = k0, v0
+    begin = torch.full((B, Sq), Sk - seen, dtype=torch.int32, device="cuda")
+    end = torch.full_like(begin, Sk)
+    out, lse = attention.fwd(q, k, v, begin, end)
+    dq, dk, dv = attention.bwd(do, q, k, v, out, lse, begin, end)
+    zero = torch.zeros_like(begin)
+    want, wlse = attention.fwd(q, k0, v0, zero, zero + seen)
+    grads = attention.bwd(do, q, k0, v0, want, wlse, zero, zero + seen)
+    assert _lib.status() == 0
+    assert not bool(dk[:, :Sk - seen].any()) and not bool(dv[:, :Sk - seen].any())
+    # Other tiles and splits, so other roundings of P or ds and another order.  A rounding to bf16 is off by up to
+    # 2^-8, over a binade 1.7e-3 in the mean square; two results with two each differ by twice that, under 2^-7.
+    # A log sum is off by up to 2^-17 sum |q k| scale, which is under 8 in the mean of 128 products over 11.3.
+    for got, other in ((out, want), (dq, grads[0]), (dk[:, Sk - seen:], grads[1]), (dv[:, Sk - seen:], grads[2])):
+        assert float((got.double() - other.double()).norm() / other.double().norm()) < 2.0 ** -7
+    assert float((lse - wlse).abs().max()) < 2 * 8 * 2.0 ** -17

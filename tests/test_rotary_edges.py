@@ -50,3 +50,22 @@ def test_scalings_without_a_value_are_refused(theta, scaling, match):
     with pytest.raises(ValueError, match=match):
         rotary.frequencies(64, theta, scaling)
     assert bool(rotary.frequencies(64, 1.0)[0].eq(1).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("norm", [False, True])
+def test_offsets_past_32_bits(cuda_lib, norm):
+    """The last tokens of 2^31 elements and more: the bits that they give alone, forward and backward."""
+    from spilltune_b200 import rotary
+    T, H, D, last = 270_000, 64, 128, 40
+    assert T * H * D > 2 ** 31
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.zeros(T, H, D, dtype=torch.bfloat16, device="cuda")
+    x[-last:] = torch.randn(last, H, D, generator=g, device="cuda").to(torch.bfloat16)
+    pos, inv = torch.arange(T, device="cuda"), rotary.frequencies(D)[0].cuda()
+    w = torch.rand(D, generator=g, device="cuda") + 0.5
+    opt = dict(q_weight=w, eps=1e-6) if norm else {}
+    y, _ = rotary.fwd(x, None, pos, inv, **opt)
+    assert torch.equal(y[-last:], rotary.fwd(x[-last:], None, pos[-last:], inv, **opt)[0])
+    dx = rotary.bwd(y, None, x, None, pos, inv, **opt)[0]
+    assert torch.equal(dx[-last:], rotary.bwd(y[-last:], None, x[-last:], None, pos[-last:], inv, **opt)[0])
