@@ -56,7 +56,7 @@
 // (five products at 685 TFLOP/s; the eight that run at 1096, 66% of the burst
 // rate of a bf16 GEMM).
 // bf16 p and ds are the products' operands: half a step of each term, of the
-// same size as rounding the result.
+// same size as rounding the result; in two parts in small calls (few_products).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
@@ -155,7 +155,8 @@ __device__ __forceinline__ float dot8(const uint4& a, const uint4& b) {
 
 // kDq: rows are packed queries (A1 = q, A2 = do; B1 = k, B2 = v).
 // Otherwise rows are keys (A1 = k, A2 = v; B1 = q, B2 = do).
-template <int HD, bool kDq, int kMode>
+// kFine: ds (and p of dv) in two bf16 parts.
+template <int HD, bool kDq, int kMode, bool kFine>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant__ CUtensorMap tm_a2,
                const __grid_constant__ CUtensorMap tm_b1, const __grid_constant__ CUtensorMap tm_b2,
@@ -397,6 +398,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           tc_fence_after();
           if (elected()) {
             mma_cols_half<HD, kTile>(tmem + kColAcc, col_s, d_cols + at(g, kDq ? 0 : 1), id_acc, half, i > 0);
+            if constexpr (kFine && !kDq)
+              mma_cols_half<HD, kTile>(tmem + kColAcc, col_s + kCols / 2, d_cols + at(g, 1), id_acc, half, true);
             if (half) {
               tc_commit(&bars->b_empty[1][g % kS2]);
               tc_commit(&bars->acc1_done);
@@ -411,6 +414,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           tc_fence_after();
           if (elected()) {
             mma_cols_half<HD, kTile>(tmem + kColAcc + HD, col_p, d_cols + at(g, 0), id_acc, half, i > 0);
+            if constexpr (kFine)
+              mma_cols_half<HD, kTile>(tmem + kColAcc + HD, col_p + kCols / 2, d_cols + at(g, 0), id_acc, half, true);
             if (half) {
               tc_commit(&bars->b_empty[0][g % kS1]);
               tc_commit(&bars->acc2_done);
@@ -586,6 +591,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         [[maybe_unused]] const float dist0 = static_cast<float>((kDq ? tok - col0 : col0 - key) + s.Sk - s.Sq);
         const uint32_t at_s = tmem + kCols * group + lanes, at_p = at_s + kColP;
         uint32_t x[kCols], w[kCols / 4];             // scores, then p; half the packed operands
+        [[maybe_unused]] uint32_t u[kCols / 4];      // kFine: what their rounding left
+        auto left = [](uint32_t hi, float a, float b) {
+          return pack_bf16x2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xFFFF0000u));
+        };
         [[maybe_unused]] __half2 fac[kCap ? kCols / 2 : 1];
         tmem_ld_32x32b_x32(at_s, x);
         tmem_wait_ld();
@@ -687,10 +696,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           }
           w[c % 16 / 2] = pack_bf16x2(p[0], p[1]);
           w[c % 16 / 2 + 1] = pack_bf16x2(p[2], p[3]);
+          if constexpr (kFine && !kDq) {
+            u[c % 16 / 2] = left(w[c % 16 / 2], p[0], p[1]);
+            u[c % 16 / 2 + 1] = left(w[c % 16 / 2 + 1], p[2], p[3]);
+          }
         };
-        // The operands' first or second half (of the group's columns) to TMEM.
-        auto hand_over = [&](uint32_t at_w, uint64_t* bar) {
+        // The operands' first or second half (of the group's columns) to TMEM; what
+        // their rounding left into the second half of the group's columns there.
+        auto hand_over = [&](uint32_t at_w, uint64_t* bar, auto two) {
           tmem_st_32x32b_x8(at_w, w);
+          if constexpr (decltype(two)::value) tmem_st_32x32b_x8(at_w + kCols / 2, u);
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
@@ -705,7 +720,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
             for (int c = 0; c < 16; c += 4) exponentials(c0 + c, std::true_type{});
           }
-          hand_over(at_s + c0 / 2, &bars->p_full[c0 / 16]);
+          hand_over(at_s + c0 / 2, &bars->p_full[c0 / 16], std::bool_constant<kFine && !kDq>{});
         }
 
         if (!wait(&bars->dp_full, g, kStatusTimeoutAccum)) {
@@ -751,13 +766,26 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
               if (hide[h + 1]) ds[1] = 0.f;
             }
             w[col % 16 / 2] = pack_bf16x2(ds[0], ds[1]);
+            if constexpr (kFine) u[col % 16 / 2] = left(w[col % 16 / 2], ds[0], ds[1]);
           }
         };
+        [[maybe_unused]] uint32_t y_next[kFine ? 16 : 1];
 #pragma unroll
         for (int c0 = 0; c0 < kCols; c0 += 16) {
           uint32_t y[16];
-          tmem_ld_32x32b_x16(at_p + c0, y);
-          tmem_wait_ld();
+          if constexpr (kFine) {
+            if (c0 == 0) {
+              tmem_ld_32x32b_x16(at_p, y);
+              tmem_ld_32x32b_x16(at_p + 16, y_next);   // u goes over these columns
+              tmem_wait_ld();
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) y[e] = y_next[e];
+            }
+          } else {
+            tmem_ld_32x32b_x16(at_p + c0, y);
+            tmem_wait_ld();
+          }
           if (whole) {
 #pragma unroll
             for (int c = 0; c < 16; c += 4) gradients(y + c, c0 + c, std::false_type{});
@@ -765,7 +793,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
             for (int c = 0; c < 16; c += 4) gradients(y + c, c0 + c, std::true_type{});
           }
-          hand_over(at_p + c0 / 2, &bars->ds_full[c0 / 16]);
+          hand_over(at_p + c0 / 2, &bars->ds_full[c0 / 16], std::bool_constant<kFine>{});
         }
       }
       g0 += it.n;
@@ -916,32 +944,34 @@ int bwd_parts(int64_t key_ctas, int64_t steps) {
   return n < 1 ? 1 : static_cast<int>(n);
 }
 
-template <int HD, bool kDq, int kMode>
+template <int HD, bool kDq, int kMode, bool kFine>
 int launch_bwd(const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1, const CUtensorMap& b2,
                const BwdArgs& a, cudaStream_t stream) {
   constexpr int kSmem = Bwd<HD, kDq>::kSmem;
-  int rc = allow_smem(reinterpret_cast<const void*>(&bwd_kernel<HD, kDq, kMode>), kSmem);
+  int rc = allow_smem(reinterpret_cast<const void*>(&bwd_kernel<HD, kDq, kMode, kFine>), kSmem);
   if (rc) return rc;
   const int64_t grid = a.items < a.sms ? a.items : a.sms;
-  bwd_kernel<HD, kDq, kMode><<<static_cast<unsigned>(grid), kBwdThreads, kSmem, stream>>>(a1, a2, b1, b2, a);
+  bwd_kernel<HD, kDq, kMode, kFine><<<static_cast<unsigned>(grid), kBwdThreads, kSmem, stream>>>(a1, a2, b1, b2, a);
   return FL_OK;
 }
 
-template <int HD, bool kDq>
+template <int HD, bool kDq, bool kFine>
 int launch_bwd_mode(int mode, const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1,
                     const CUtensorMap& b2, const BwdArgs& a, cudaStream_t stream) {
-  return mode == kCappedSlopes ? launch_bwd<HD, kDq, kCappedSlopes>(a1, a2, b1, b2, a, stream)
-         : mode == kCapped     ? launch_bwd<HD, kDq, kCapped>(a1, a2, b1, b2, a, stream)
-         : mode == kSlopes     ? launch_bwd<HD, kDq, kSlopes>(a1, a2, b1, b2, a, stream)
-                               : launch_bwd<HD, kDq, kPlain>(a1, a2, b1, b2, a, stream);
+  return mode == kCappedSlopes ? launch_bwd<HD, kDq, kCappedSlopes, kFine>(a1, a2, b1, b2, a, stream)
+         : mode == kCapped     ? launch_bwd<HD, kDq, kCapped, kFine>(a1, a2, b1, b2, a, stream)
+         : mode == kSlopes     ? launch_bwd<HD, kDq, kSlopes, kFine>(a1, a2, b1, b2, a, stream)
+                               : launch_bwd<HD, kDq, kPlain, kFine>(a1, a2, b1, b2, a, stream);
 }
 
 template <bool kDq>
-int launch_bwd_any(int D, int mode, const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1,
+int launch_bwd_any(int D, int mode, bool fine, const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1,
                    const CUtensorMap& b2, const BwdArgs& a, cudaStream_t stream) {
   if (D <= 64)
-    return launch_bwd_mode<64, kDq>(mode, a1, a2, b1, b2, a, stream);
-  return launch_bwd_mode<128, kDq>(mode, a1, a2, b1, b2, a, stream);
+    return fine ? launch_bwd_mode<64, kDq, true>(mode, a1, a2, b1, b2, a, stream)
+                : launch_bwd_mode<64, kDq, false>(mode, a1, a2, b1, b2, a, stream);
+  return fine ? launch_bwd_mode<128, kDq, true>(mode, a1, a2, b1, b2, a, stream)
+              : launch_bwd_mode<128, kDq, false>(mode, a1, a2, b1, b2, a, stream);
 }
 
 int64_t q_tiles_of(int64_t Sq, int lgp) { return (Sq + (kTile >> lgp) - 1) / (kTile >> lgp); }
@@ -1035,13 +1065,14 @@ int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, cons
   a.items = attn::fwd_ctas(b, sq, Hq, Hkv);
   a.parts = 1;
   a.tiles = static_cast<int>(a.items / B / (Hq >> a.s.lgp));
-  rc = attn::launch_bwd_any<true>(D, mode, mq, mdo, mk, mv, a, st);
+  const bool fine = attn::few_products(a.items, Sk);
+  rc = attn::launch_bwd_any<true>(D, mode, fine, mq, mdo, mk, mv, a, st);
   if (rc) return rc;
   a.tiles = static_cast<int>(key_tiles);
   a.parts = parts;
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + part_at);
   a.items = key_tiles * B * Hkv * parts;
-  rc = attn::launch_bwd_any<false>(D, mode, mk, mv, mq, mdo, a, st);
+  rc = attn::launch_bwd_any<false>(D, mode, fine, mk, mv, mq, mdo, a, st);
   if (rc) return rc;
   if (parts > 1) {
     const int64_t n4 = B * Sk * Hkv * D / 4;
