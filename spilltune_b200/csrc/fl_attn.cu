@@ -28,7 +28,7 @@
 // results of such a call show every rounding, and the products are not what
 // bounds it (one token over 8192 keys, 32/8 heads, 4 sequences: 28.8 us instead
 // of 26.1, error against 64 bits 1.7e-3 instead of 2.3e-3).  Small calls without
-// splits do so too (few_products).
+// splits do so too (few_results).
 #include <cuda_bf16.h>
 #include <cstdint>
 #include <map>
@@ -642,7 +642,7 @@ int fl_attn_fwd(const uint16_t* q, const uint16_t* k, const uint16_t* v, const i
     return rc;
   const int mode = (softcap != 0.f ? attn::kCapped : attn::kPlain) + (slopes ? attn::kSlopes : 0);
   const int64_t grid = ctas * a.splits;
-  if (a.splits > 1 || attn::few_products(ctas, Sk))
+  if (a.splits > 1 || attn::few_results(rows, Sk))
     rc = D <= 64 ? attn::launch_fwd_mode<64, true>(mode, mq, mk, mv, a, grid, st)
                  : attn::launch_fwd_mode<128, true>(mode, mq, mk, mv, a, grid, st);
   else

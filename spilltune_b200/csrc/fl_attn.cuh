@@ -220,14 +220,15 @@ __device__ __forceinline__ void mma_cols_half(uint32_t d, uint32_t a_tmem, uint6
 int packed_log2(int Hq, int Hkv);
 // Row tiles of kTile packed rows over all heads and sequences.
 int64_t fwd_ctas(int B, int Sq, int Hq, int Hkv);
-// A call of at most 148 row tiles (one to an SM) over at most 512 keys: its results
-// can be so few that a second rounding of each shows (2 tokens: dq off by 3.6e-3 of
-// its norm instead of 1.7e-3; of 5788 drawn calls 210 were over 1.5 times what FP32
-// rounded once is, none now), and its time is mostly latency.  The products'
-// rounded operands come in two bf16 parts there, forward and backward: 2 x 128
-// tokens, 4/2 heads of 64 6.2 + 19.5 us instead of 5.9 + 19.3; at the border, 1 x 512,
-// 32/8 heads of 128, 12.6 + 43.0 instead of 11.4 + 39.5.
-inline bool few_products(int64_t row_tiles, int64_t Sk) { return row_tiles <= 148 && Sk <= 4 * kTile; }
+// A call of at most 2048 rows (tokens x heads) over at most 512 keys: its results can
+// be so few that a second rounding of each shows, and its time is mostly latency.
+// The products' rounded operands come in two bf16 parts there, forward and backward.
+// With one part 210 of 5788 drawn calls were over 1.5 times as far off as FP32
+// rounded once (2 tokens: 2.4 times), all of them this small; with two none.  It
+// costs 2 x 128 tokens, 4/2 heads of 64 6.3 + 19.6 us instead of 6.0 + 19.4, and at
+// the border (1 x 512 tokens, 4/2 heads of 128) a backward of 37.6 instead of 33.8.
+// Beyond it the roundings of more results average out to 1.41 - 1.47 times.
+inline bool few_results(int64_t rows, int64_t Sk) { return rows <= 2048 && Sk <= 4 * kTile; }
 void fill_shape(Shape& s, int B, int Sq, int Sk, int Hq, int Hkv, int D, const int* begin, const int* end, float scale,
                 float cap, const float* slopes);
 

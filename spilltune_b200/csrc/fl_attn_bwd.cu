@@ -56,7 +56,7 @@
 // (five products at 685 TFLOP/s; the eight that run at 1096, 66% of the burst
 // rate of a bf16 GEMM).
 // bf16 p and ds are the products' operands: half a step of each term, of the
-// same size as rounding the result; in two parts in small calls (few_products).
+// same size as rounding the result; in two parts in small calls (few_results).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
@@ -1065,7 +1065,7 @@ int fl_attn_bwd(const uint16_t* dout, const uint16_t* q, const uint16_t* k, cons
   a.items = attn::fwd_ctas(b, sq, Hq, Hkv);
   a.parts = 1;
   a.tiles = static_cast<int>(a.items / B / (Hq >> a.s.lgp));
-  const bool fine = attn::few_products(a.items, Sk);
+  const bool fine = attn::few_results(B * Sq * Hq, Sk);
   rc = attn::launch_bwd_any<true>(D, mode, fine, mq, mdo, mk, mv, a, st);
   if (rc) return rc;
   a.tiles = static_cast<int>(key_tiles);
