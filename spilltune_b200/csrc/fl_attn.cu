@@ -9,13 +9,15 @@
 // per row, so row maxima and sums need no exchange).  Two CTAs share an SM: one's
 // softmax runs under the other's products.
 //
-// What bounds it is the chain scores - softmax - values of a CTA.  With 128-key
-// tiles and one S buffer (P lies over S) the next scores waited for the product
-// that reads P: 530 us for 8192 causal tokens, 32/8 heads of 128.  With 64-key
-// tiles S(j + 1) is there before the softmax of S(j) ends: 472 us, 1163 TFLOP/s
-// (70% of the burst rate of a bf16 GEMM), although 64 columns leave the scores'
-// product bound by its operands' fetches (48 cycles where 32 would do).  Two
-// threads to a row instead of one gained nothing (they meet once a tile).
+// What bounds it is the chain scores - softmax - values of a CTA.  8192 causal
+// tokens, 32/8 heads of 128, take 550 us kept up for seconds (1000 TFLOP/s, 72% of
+// the sustained rate of a bf16 GEMM, both at the power cap) and 472 to 487 in short
+// runs (1130 to 1163, 70% of its burst rate).  With 128-key tiles and one S buffer
+// (P lies over S) the next scores waited for the product that reads P: 530 in short
+// runs.  With 64-key tiles S(j + 1) is there before the softmax of S(j) ends,
+// although 64 columns leave the scores' product bound by its operands' fetches (48
+// cycles where 32 would do).  Two threads to a row instead of one gained nothing
+// (they meet once a tile).
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 over the
 // one in use (the sums then stay far inside FP32's range); otherwise the old
@@ -465,8 +467,15 @@ __global__ void __launch_bounds__(128) join_kernel(const float* __restrict__ par
   if (sub == 0) lse[row] = sum == 0.f ? -INFINITY : top + log2f(sum) * kLn2;
 }
 
-// Splits of the key tiles: none while the row tiles fill half the SMs; else
-// towards two CTAs per SM, each keeping two key tiles at least.
+// Splits of the key tiles: none while the row tiles fill half the SMs of a B200
+// (its 148 are constants here: the workspace's size depends on the arguments
+// alone); else towards two CTAs per SM, each keeping two key tiles at least.
+// Measured unsplit / split, 32/8 heads of 128, one token in each sequence:
+//   8192 keys:  32 row tiles 117 / 35 us, 72 119 / 58, 80 119 / 69, 128 125 / 99, 144 130 / 104
+//   2048 keys:  32 31 / 21, 72 31 / 21, 80 33 / 25, 128 37 / 34
+// and causal tokens:  64 row tiles of 1024 keys 22 / 24, of 2048 33 / 24; 76 of 2432
+// 38 / 28; 128 of 2048 35 / 34.  So the border at half the SMs costs calls of 75 to
+// 148 row tiles up to 42% of their time with one token and 28% with more.
 int fwd_splits(int64_t ctas, int Sk) {
   const int64_t key_tiles = (Sk + kTile - 1) / kTile;
   if (ctas > 74 || key_tiles < 4) return 1;

@@ -30,9 +30,9 @@
 // S, P' and the accumulators fill TMEM, so nothing is double-buffered; the order
 // acc1(i), S(i + 1), acc2(i), P'(i + 1) keeps the tensor cores on one pair while
 // the sixteen element warps (four to each 32 columns) work on the other.  What
-// bounds a step is that chain (measured before the two steps at the end of this
-// list: S 720 cycles from issue to arrival, exponentials 1000 - 1500, acc1 900;
-// 3280 cycles a step in dq and 3570 in dk/dv, where the four products take 2048).
+// bounds a step is that chain: over 4 x 2048 causal tokens, 32/8 heads of 128, a
+// step takes 2.3 us in dq and 2.0 us in dk/dv, the ends of the walks included, where
+// its four products take 2048 cycles (1.1 us).
 // * Products are 128 columns wide: with 64, the fetch of the resident operand
 //   makes a product take 48 cycles where 32 would do (measured back to back).
 // * One elected lane of a warp that walks as one issues them: a divergent lane's
@@ -50,11 +50,13 @@
 //   make short walks; no gain for dq.
 // * Shared memory is declared aligned, not aligned by hand: a pointer that went
 //   through an integer is generic to the compiler (64-bit, and its accesses
-//   slower), and 96 registers had no room for that: dk/dv 278 -> 235 us, no
-//   spills.  The slack saved lets dq keep a third key tile (303 -> 280 us).
-// Measured at 4 x 2048 causal tokens, 32/8 heads of 128: dq 266 us, dk/dv 236 us
-// (five products at 685 TFLOP/s; the eight that run at 1096, 66% of the burst
-// rate of a bf16 GEMM).
+//   slower), and 96 registers had no room for that: dk/dv 278 -> 235 us; the
+//   128-wide forms without slopes no longer spill (others store up to 56 bytes,
+//   with operands in two parts up to 96).  The slack saved lets dq keep a third key
+//   tile (303 -> 280 us).
+// Measured at 4 x 2048 causal tokens, 32/8 heads of 128, in short runs: dq 266 us,
+// dk/dv 236 us (five products at 685 TFLOP/s; the eight that run at 1096, 66% of the
+// burst rate of a bf16 GEMM); both together 594 us kept up for seconds, at the power cap.
 // bf16 p and ds are the products' operands: half a step of each term, of the
 // same size as rounding the result; in two parts in small calls (few_results).
 #include <cuda_bf16.h>
@@ -934,9 +936,15 @@ __global__ void __launch_bounds__(256) parts_kernel(const float4* __restrict__ p
   }
 }
 
-// CTAs that share one key tile's walk: none while the key tiles fill half the
-// SMs; else towards one CTA per SM, each keeping four steps of the longest
-// walk (a step is about 2 us, the reduction's launch another).
+// CTAs that share one key tile's walk: none where two to each would be more than
+// the SMs; else towards one CTA per SM, each keeping four steps of the longest
+// walk (a step is about 2 us, the reduction's launch another).  Backward without /
+// with parts, 32/8 heads of 128 and, in brackets, every key seen instead of a causal
+// mask:  32 key tiles (512 tokens) 66 / 49 us (64 / 48), 64 91 / 76 (103 / 88), 72
+// 102 / 84 (112 / 95); two parts from 75 on, more CTAs than SMs:  80 117 / 95 (142 /
+// 158), 128 187 / 155 (240 / 262), 144 224 / 192 (280 / 304).  Past half the SMs two
+// parts gain 14 - 26% under a causal mask, whose walks differ, and lose 5 - 11% where
+// all are equal; which of the two a call is only its ranges say.
 int bwd_parts(int64_t key_ctas, int64_t steps) {
   if (key_ctas > 74) return 1;
   int64_t n = 148 / key_ctas;

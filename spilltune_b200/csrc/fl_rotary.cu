@@ -24,7 +24,8 @@
 // memory as neighbouring lanes read them, and rows per block leave few lanes
 // idle.  Measured at 8192 tokens: 32 + 8 heads of 128 30 us forward or backward
 // (168 MB: 5.5 TB/s, 85% of a copy's rate); with a norm 32 + 4 heads 34.5 us
-// forward (4.4 TB/s) and 49 us backward (226 MB: 4.7 TB/s).  Other shapes take
+// forward (4.4 TB/s) and 49 us backward (226 MB: 4.7 TB/s), 61 us with the weights'
+// gradients (128 registers, at most 296 blocks).  Other shapes take
 // the scalar form, a warp per head, which loads each column's partner as well
 // (1027 tokens, 16 heads of 80, 40 columns rotated: 11 us, 1.5 as a copy).
 #include <cuda_bf16.h>
